@@ -360,6 +360,91 @@ int  coli_cuda_gdn_full_route(int layer, const float *x_in, const float *resid, 
                               int KH, int KD, int VH, int VD, int conv_dim, int conv_k,
                               float eps, int Dout, int E);
 
+/* ==== Paged KV cache ====
+ * No counterpart in the reference, which keeps one contiguous cache per layer
+ * (c/backend_vulkan.h:114-116): a pool of pages that many requests share, for
+ * batched serving. A handle names the pool of all its layers,
+ * [layers][K, V][n_pages][KH][page][hd] bf16; token t of request r sits in
+ * page id table[r][t / page] at offset t % page. The page tables (int32
+ * [requests][max_pages]) and all other index arrays are the caller's, on the
+ * device. page is a multiple of 16 up to 1024, hd = 256, H / KH is 1, 2, 4
+ * or 8, n_pages <= 2^20, KH * page * n_pages < 2^31.
+ *
+ * Every call below takes device pointers and runs asynchronously on the
+ * backend stream; none allocates, frees or synchronises, so each can be
+ * captured into a graph. They use the handle's one workspace: calls on one
+ * handle that may overlap on the GPU (two streams, two graphs in flight) need
+ * a workspace of their own (set_workspace before the call or its capture),
+ * beside touching different pages.
+ * Page ids, positions, lengths and row offsets are checked on the device:
+ * what is out of range is left out (its outputs are undefined, no memory
+ * outside the arguments is touched), and the next coli_cuda_sync returns 0
+ * and says what was met; the backend stays usable. B, n, S or n_seq of 0 is
+ * a call that does nothing.
+ *
+ *   pages_bytes          size of the pool, 0 for an unsupported geometry
+ *   pages_create         kv_dev: the caller's memory (128-byte aligned, its
+ *                        contents kept) or NULL for a zeroed pool of the
+ *                        handle's own; up to 256 handles at a time
+ *   pages_free           waits for the backend stream, then releases
+ *   pages_norm_weight    q_norm / k_norm weights [hd] of a layer (host fp32)
+ *   pages_set_workspace  pages_workspace_bytes bytes of device memory, 256-byte
+ *                        aligned, for the calls from here on; NULL: the
+ *                        handle's own again */
+typedef struct ColiCudaPages ColiCudaPages;
+size_t coli_cuda_pages_bytes(int layers, int n_pages, int page, int KH, int hd);
+int    coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int page, int KH, int hd, void *kv_dev);
+void   coli_cuda_pages_free(ColiCudaPages *pages);
+int    coli_cuda_pages_device_ptr(const ColiCudaPages *pages, int layer, void **k, void **v);
+int    coli_cuda_pages_norm_weight(ColiCudaPages *pages, int layer, const float *qnw, const float *knw, int hd);
+size_t coli_cuda_pages_workspace_bytes(const ColiCudaPages *pages);
+int    coli_cuda_pages_set_workspace(ColiCudaPages *pages, void *ws, size_t bytes);
+
+/* Batched decode over pages: as coli_cuda_gqa_decode_dev (one new token of
+ * each request b < B <= 1024 at its own position pos[b]: q/k norm, RoPE, K/V
+ * append, attention over rows 0..pos[b], sigmoid gate), for requests whose
+ * rows are in pages. pos[b] < 0 names an idle slot: nothing is appended and
+ * its ctx row is left as it was. The page of position pos[b] has to be the
+ * request's alone (fork before). dtype 1: bf16 activations; q and the
+ * probabilities enter the tensor cores as bf16. dtype 0: fp32 activations; both
+ * enter as two bf16 parts, so ctx is good to about 2^-17. RoPE angles are
+ * formed in double. qg, k, v, ctx 16-byte aligned. */
+int  coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const void *qg, const void *k,
+                                    const void *v, const int *pos_dev, const int *table, int max_pages, void *ctx,
+                                    int H, int KH, int hd, int rot, float eps, float theta, int dtype);
+
+/* Ragged causal prefill over pages: n_seq <= 1024 requests' chunks in one
+ * call. Rows cu[r] .. cu[r + 1] - 1 (cu int32 [n_seq + 1], ascending, of the S
+ * rows of qg / k / v / ctx) are request r's next tokens, at positions
+ * pos_base[r] ..; they are appended to its pages and attend to rows
+ * 0..their own position. A chunk may be empty or a single token (a request
+ * that decodes beside others that prefill); rows outside all chunks are left
+ * as they were. bf16 activations (dtype 1) only. S <= 2^24. */
+int  coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, int S, const int *cu,
+                                     const int *pos_base, const void *qg, const void *k, const void *v,
+                                     const int *table, int max_pages, void *ctx, int H, int KH, int hd, int rot,
+                                     float eps, float theta, int dtype);
+
+/* Page src[i] over page dst[i] in every layer, i < n. A pair whose destination
+ * is named twice, or whose source is another pair's destination, is left out
+ * and reported. */
+int  coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const int *dst);
+/* Request child[i] becomes a copy of request parent[i], i < n < n_req: it
+ * shares the pages that the parent has filled, len[child] = len[parent], and
+ * where the parent's last page is only started, its rows are copied to page
+ * fresh[i] (else fresh[i] is not used). A parent may have many children; a
+ * child named twice or also as a parent, and a fresh page named twice, are
+ * left out and reported. len int32 [n_req], table int32 [n_req][max_pages]. */
+int  coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, const int *child, const int *fresh,
+                              int *len, int *table, int n_req, int max_pages);
+/* Renumber the pages that the requests hold (the first ceil(len / page) of
+ * each table row; len <= 0: none) to 0 .. *live - 1: the k-th held page at or
+ * behind *live moves to the k-th free page before it, in every layer. Pages
+ * *live .. are free afterwards. table_out gets the new table (entries behind
+ * a request's length as they were) and may be table itself. */
+int  coli_cuda_pages_compact_dev(ColiCudaPages *pages, int n_req, const int *len, const int *table, int max_pages,
+                                 int *table_out, int *live);
+
 /* ==== Snapshot loader (safetensors) ====
  * The reference's shard index (c/st.h:248-479) and the mixer part of
  * model_init (c/qwen.c:433-485): st_open indexes every *.safetensors file of

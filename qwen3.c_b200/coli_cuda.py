@@ -92,6 +92,18 @@ SIGNATURES = {
     "coli_cuda_gdn_full": ([_i, _fp, _i, _vp, _vp, _fp, _vp, _fp] + [_i] * 6 + [_f, _i], _i),
     "coli_cuda_gdn_full_seq": ([_i, _fp, _i, _i, _vp, _vp, _fp, _vp, _fp] + [_i] * 6 + [_f, _i], _i),
     "coli_cuda_gdn_full_ab": ([_i, _fp, _i, _i] + [_vp] * 5 + [_fp] + [_i] * 6 + [_f, _i], _i),
+    "coli_cuda_pages_bytes": ([_i] * 5, ctypes.c_size_t),
+    "coli_cuda_pages_create": ([ctypes.POINTER(_vp)] + [_i] * 5 + [_vp], _i),
+    "coli_cuda_pages_free": ([_vp], None),
+    "coli_cuda_pages_device_ptr": ([_vp, _i, ctypes.POINTER(_vp), ctypes.POINTER(_vp)], _i),
+    "coli_cuda_pages_norm_weight": ([_vp, _i, _fp, _fp, _i], _i),
+    "coli_cuda_pages_workspace_bytes": ([_vp], ctypes.c_size_t),
+    "coli_cuda_pages_set_workspace": ([_vp, _vp, ctypes.c_size_t], _i),
+    "coli_cuda_gqa_decode_pages_dev": ([_vp, _i, _i] + [_vp] * 5 + [_i, _vp] + [_i] * 4 + [_f, _f, _i], _i),
+    "coli_cuda_gqa_prefill_pages_dev": ([_vp, _i, _i, _i] + [_vp] * 6 + [_i, _vp] + [_i] * 4 + [_f, _f, _i], _i),
+    "coli_cuda_pages_copy_dev": ([_vp, _i, _vp, _vp], _i),
+    "coli_cuda_pages_fork_dev": ([_vp, _i] + [_vp] * 5 + [_i, _i], _i),
+    "coli_cuda_pages_compact_dev": ([_vp, _i, _vp, _vp, _i, _vp, _vp], _i),
     "coli_cuda_moe_route_available": ([], _i),
     "coli_cuda_st_open": ([ctypes.c_char_p], _i),
     "coli_cuda_st_close": ([_i], None),
@@ -417,6 +429,74 @@ class DenseTensor:
         if self.h:
             self.be.lib.coli_cuda_tensor_free(self.h)
             self.h = _vp()
+
+
+class PagedCache:
+    """A pool of KV pages for all layers, shared by many requests (coli_cuda_pages_*).
+
+    kv: device address of the caller's memory for the pool, bf16
+    [layers][2][n_pages][KH][page][hd] (None: the cache's own, zeroed). All
+    *_dev calls take device addresses, run on the backend stream and neither
+    allocate nor wait; table is int32 [requests][max_pages]."""
+
+    def __init__(self, be, layers, n_pages, page=64, KH=2, hd=256, kv=None):
+        self.be, self.layers, self.n_pages, self.page, self.KH, self.hd = be, layers, n_pages, page, KH, hd
+        self.h = _vp()
+        be._ok(be.lib.coli_cuda_pages_create(ctypes.byref(self.h), layers, n_pages, page, KH, hd, kv), "pages_create")
+
+    @staticmethod
+    def nbytes_for(be, layers, n_pages, page=64, KH=2, hd=256):
+        n = be.lib.coli_cuda_pages_bytes(layers, n_pages, page, KH, hd)
+        be._ok(int(n > 0), "pages_bytes")
+        return n
+
+    def free(self):
+        if self.h:
+            self.be.lib.coli_cuda_pages_free(self.h)
+            self.h = _vp()
+
+    __del__ = free
+
+    def device_ptr(self, layer):
+        k, v = _vp(), _vp()
+        self.be._ok(self.be.lib.coli_cuda_pages_device_ptr(self.h, layer, ctypes.byref(k), ctypes.byref(v)),
+                    "pages_device_ptr")
+        return k.value, v.value
+
+    def norm_weight(self, layer, qnw, knw):
+        qnw, qp = _f32(qnw)
+        knw, kp = _f32(knw)
+        if qnw.shape != (self.hd,) or knw.shape != (self.hd,):
+            raise BackendError(f"pages_norm_weight: the weights are [{self.hd}]")
+        self.be._ok(self.be.lib.coli_cuda_pages_norm_weight(self.h, layer, qp, kp, self.hd), "pages_norm_weight")
+
+    def workspace_bytes(self):
+        return self.be.lib.coli_cuda_pages_workspace_bytes(self.h)
+
+    def set_workspace(self, ws=None, nbytes=0):
+        self.be._ok(self.be.lib.coli_cuda_pages_set_workspace(self.h, ws, nbytes), "pages_set_workspace")
+
+    def decode_dev(self, layer, B, qg, k, v, pos, table, max_pages, ctx, H=16, rot=64, eps=1e-6, theta=1e7, dtype=1):
+        self.be._ok(self.be.lib.coli_cuda_gqa_decode_pages_dev(self.h, layer, B, qg, k, v, pos, table, max_pages, ctx, H,
+                                                               self.KH, self.hd, rot, eps, theta, dtype),
+                    "gqa_decode_pages_dev")
+
+    def prefill_dev(self, layer, n_seq, S, cu, pos_base, qg, k, v, table, max_pages, ctx, H=16, rot=64, eps=1e-6,
+                    theta=1e7, dtype=1):
+        self.be._ok(self.be.lib.coli_cuda_gqa_prefill_pages_dev(self.h, layer, n_seq, S, cu, pos_base, qg, k, v, table,
+                                                                max_pages, ctx, H, self.KH, self.hd, rot, eps, theta,
+                                                                dtype), "gqa_prefill_pages_dev")
+
+    def copy_dev(self, n, src, dst):
+        self.be._ok(self.be.lib.coli_cuda_pages_copy_dev(self.h, n, src, dst), "pages_copy_dev")
+
+    def fork_dev(self, n, parent, child, fresh, length, table, n_req, max_pages):
+        self.be._ok(self.be.lib.coli_cuda_pages_fork_dev(self.h, n, parent, child, fresh, length, table, n_req,
+                                                         max_pages), "pages_fork_dev")
+
+    def compact_dev(self, n_req, length, table, max_pages, table_out, live):
+        self.be._ok(self.be.lib.coli_cuda_pages_compact_dev(self.h, n_req, length, table, max_pages, table_out, live),
+                    "pages_compact_dev")
 
 
 def _block_methods():

@@ -26,6 +26,8 @@
 #include "gqa_prefill.cu"
 #include "gdn_prefill.cu"
 #include "linear.cu"
+#include "gqa_pages.cu"
+#include "page_moves.cu"
 
 namespace {
 
@@ -195,6 +197,11 @@ void *scratch(Slot s, size_t bytes)
     G.slot_bytes[s] = want;
     return G.slot[s];
 }
+
+// Page caches (pages.cu): the state of their device-side argument checks, and
+// their release at shutdown.
+int pages_check_error();
+void pages_shutdown();
 
 int check_layer(int layer) { return layer >= 0 && layer < MAX_LAYERS; }
 
@@ -594,6 +601,7 @@ void coli_cuda_shutdown(void)
     cudaSetDevice(G.device);
     cudaDeviceSynchronize();
     coli_cuda_kv_reset();
+    pages_shutdown();
     for (int i = 0; i < MAX_LAYERS; ++i) {
         GdnLayer &L = G.gdn[i];
         dev_free(L.state, (size_t)L.batch * L.VH * L.KD * L.VD * 4);
@@ -708,7 +716,8 @@ int coli_cuda_sync(void)
 {
     READY();
     CK(cudaStreamSynchronize(stream()));
-    return check_dev_error();
+    if (!check_dev_error()) return 0;
+    return pages_check_error();
 }
 
 void *coli_cuda_get_stream(void) { return (void *)stream(); }
@@ -1327,3 +1336,4 @@ int coli_cuda_gdn_prefill(int layer, int req, int S, const float *qkv, const flo
 #include "block.cu"
 #include "container.cu"
 #include "peer.cu"
+#include "pages.cu"

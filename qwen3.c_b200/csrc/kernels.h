@@ -168,3 +168,54 @@ cudaError_t launch_rmsnorm_zc_rows(const float *x, const float *delta, const flo
                                    float *nrm_out, __nv_bfloat16 *nrm_bf16, int S, int D, float eps,
                                    cudaStream_t st);
 }  // namespace coli
+
+namespace coli {
+// ---------------------------------------------------------------- paged KV cache
+// Rotary frequencies theta^(-2 j / rot) in double: a float32 product
+// pos * frequency is off by 2^-24 of the angle, 2e-3 rad at position 32768.
+struct RopeFreq {
+    double f[128];
+};
+// One layer's pages as the kernels see them: K and V rows of 256 bf16 at
+// ((page id * KH + head) * page + offset).
+struct PageView {
+    __nv_bfloat16 *k, *v;
+    const int *table;     // [requests][max_pages] page ids
+    int n_pages, page, KH, max_pages;
+};
+// Rows of one call: request r's query rows are cu[r] .. cu[r + 1] - 1 at
+// positions base[r] ..; decode (cu == nullptr) has one row per request, row r
+// at position base[r], and base[r] < 0 names an idle slot.
+struct GqaPagesArgs {
+    PageView pv;
+    const void *qg, *k, *v;   // [rows][H][2 hd], [rows][KH][hd]
+    const float *qnw, *knw;
+    const int *cu, *base;
+    void *ctx;                // [rows][H][hd]
+    int n_req, S, H, rot;
+    float eps, scale_log2;
+};
+cudaError_t launch_pages_append(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st);
+cudaError_t launch_pages_attend(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st);
+
+// Page moves over every layer's K and V (base: [layers][K, V][n_pages][page_bytes]).
+struct PageMoveArgs {
+    uint8_t *base;
+    size_t page_bytes;
+    int layers, n_pages, page, KH;
+};
+cudaError_t launch_pages_copy(const PageMoveArgs &m, int n, const int *src, const int *dst, cudaStream_t st);
+struct PageForkArgs {
+    const int *parent, *child, *fresh;
+    int *len, *table;
+    int n, n_req, max_pages;
+};
+cudaError_t launch_pages_fork(const PageMoveArgs &m, const PageForkArgs &f, cudaStream_t st);
+struct PageCompactArgs {
+    const int *len, *table;
+    int *table_out, *live;
+    int *src, *dst, *remap, *count;   // workspace: [n_pages] each, count[1]
+    int n_req, max_pages;
+};
+cudaError_t launch_pages_compact(const PageMoveArgs &m, const PageCompactArgs &c, cudaStream_t st);
+}  // namespace coli

@@ -1,0 +1,219 @@
+// Moving pages of the paged KV cache: copies of whole pages, forks of
+// requests, and compaction. One launch moves every layer's K and V; the
+// kernels are plain copies, bound by HBM (each moved byte read and written).
+//
+// Page ids, request indices and lengths are checked on the device; what is
+// out of range or in conflict raises g_pages_error and is left out.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace coli {
+
+constexpr int MV_THREADS = 256;
+
+// Page `id` of plane y = 2 * layer + (0 K, 1 V).
+__device__ __forceinline__ uint4 *page_at(const PageMoveArgs &m, int plane, int id)
+{
+    return reinterpret_cast<uint4 *>(m.base + ((size_t)plane * m.n_pages + id) * m.page_bytes);
+}
+
+// ------------------------------------------------------------------ copy
+// One CTA per (pair, plane). A pair is left out when its destination is
+// named by another pair too, or when its source is another pair's
+// destination: either would make the result a matter of timing.
+__global__ void __launch_bounds__(MV_THREADS)
+pages_copy_kernel(PageMoveArgs m, int n, const int *src, const int *dst)
+{
+    const int i = blockIdx.x, s = src[i], d = dst[i];
+    if ((unsigned)s >= (unsigned)m.n_pages || (unsigned)d >= (unsigned)m.n_pages) {
+        pages_error(PAGES_BAD_ID);
+        return;
+    }
+    int bad = 0;
+    for (int j = threadIdx.x; j < n; j += MV_THREADS)
+        if (j != i && (dst[j] == d || dst[j] == s)) bad = 1;
+    if (__syncthreads_or(bad)) {
+        pages_error(PAGES_CONFLICT);
+        return;
+    }
+    if (s == d) return;
+    const uint4 *from = page_at(m, blockIdx.y, s);
+    uint4 *to = page_at(m, blockIdx.y, d);
+    for (int j = threadIdx.x; j < (int)(m.page_bytes / 16); j += MV_THREADS) to[j] = from[j];
+}
+
+cudaError_t launch_pages_copy(const PageMoveArgs &m, int n, const int *src, const int *dst, cudaStream_t st)
+{
+    pages_copy_kernel<<<dim3(n, 2 * m.layers), MV_THREADS, 0, st>>>(m, n, src, dst);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ fork
+// One CTA per (fork, plane): the parent's started page is copied as far as
+// it is filled; the CTAs of plane 0 write the child's table row and length.
+__global__ void __launch_bounds__(MV_THREADS)
+pages_fork_kernel(PageMoveArgs m, PageForkArgs f)
+{
+    const int i = blockIdx.x, a = f.parent[i], c = f.child[i];
+    if ((unsigned)a >= (unsigned)f.n_req || (unsigned)c >= (unsigned)f.n_req) {
+        pages_error(PAGES_BAD_REQ);
+        return;
+    }
+    const int len = f.len[a];
+    if (len < 0 || (long long)len > (long long)f.max_pages * m.page) {
+        pages_error(PAGES_BAD_POS);
+        return;
+    }
+    const int full = len / m.page, tail = len - full * m.page;
+    const int *row = f.table + (size_t)a * f.max_pages;
+    const int to_id = f.fresh[i], from_id = tail ? row[full] : -1;
+    if (tail && ((unsigned)to_id >= (unsigned)m.n_pages || (unsigned)from_id >= (unsigned)m.n_pages)) {
+        pages_error(PAGES_BAD_ID);
+        return;
+    }
+    // A child named twice, one that is also a parent, or a fresh page named
+    // twice: left out.
+    int bad = a == c || (tail && to_id == from_id);
+    for (int j = threadIdx.x; j < f.n; j += MV_THREADS) {
+        if (f.parent[j] == c || (j != i && (f.child[j] == c || f.child[j] == a))) bad = 1;
+        if (tail && j != i && f.fresh[j] == to_id) bad = 1;
+    }
+    if (__syncthreads_or(bad)) {
+        pages_error(PAGES_CONFLICT);
+        return;
+    }
+    if (blockIdx.y == 0) {
+        int *out = f.table + (size_t)c * f.max_pages;
+        for (int j = threadIdx.x; j < full; j += MV_THREADS) out[j] = row[j];
+        if (threadIdx.x == 0) {
+            if (tail) out[full] = to_id;
+            f.len[c] = len;
+        }
+    }
+    const int per = m.page * 32;         // 16-byte words of one head's rows in a page
+    const uint4 *from = tail ? page_at(m, blockIdx.y, from_id) : nullptr;
+    uint4 *to = tail ? page_at(m, blockIdx.y, to_id) : nullptr;
+    for (int j = threadIdx.x; j < m.KH * tail * 32; j += MV_THREADS) {
+        const int kh = j / (tail * 32), at = kh * per + j - kh * tail * 32;
+        to[at] = from[at];
+    }
+}
+
+cudaError_t launch_pages_fork(const PageMoveArgs &m, const PageForkArgs &f, cudaStream_t st)
+{
+    pages_fork_kernel<<<dim3(f.n, 2 * m.layers), MV_THREADS, 0, st>>>(m, f);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ compact
+constexpr int CP_THREADS = 1024;
+
+// Exclusive prefix sum over the CTA's threads; `total` is every thread's sum.
+__device__ __forceinline__ int block_scan(int x, int &total)
+{
+    __shared__ int part[CP_THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inc = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += y;
+    }
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < CP_THREADS / 32; ++w) {
+        if (w < warp) before += part[w];
+        all += part[w];
+    }
+    __syncthreads();
+    total = all;
+    return before + inc - x;
+}
+
+// Pages that request r holds, 0 where its length is impossible.
+__device__ __forceinline__ int pages_held(const PageMoveArgs &m, const PageCompactArgs &c, int r)
+{
+    const int len = c.len[r];
+    if (len <= 0) return 0;
+    if ((long long)len > (long long)c.max_pages * m.page) { pages_error(PAGES_BAD_POS); return 0; }
+    return (len + m.page - 1) / m.page;
+}
+
+// One CTA, a bit per page in shared memory: mark what a request holds, count
+// the live pages, then pair the k-th live page behind the count (a mover)
+// with the k-th dead page before it (a hole). As many of the one as of the
+// other: dead pages before n_live = n_live - (live pages before it).
+__global__ void __launch_bounds__(CP_THREADS, 1)
+pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
+{
+    extern __shared__ uint32_t bits[];
+    const int words = (m.n_pages + 31) / 32, tid = threadIdx.x;
+    for (int w = tid; w < words; w += CP_THREADS) bits[w] = 0;
+    __syncthreads();
+    for (int r = tid >> 5; r < c.n_req; r += CP_THREADS / 32) {
+        const int held = pages_held(m, c, r);
+        for (int j = tid & 31; j < held; j += 32) {
+            const int id = c.table[(size_t)r * c.max_pages + j];
+            if ((unsigned)id < (unsigned)m.n_pages) atomicOr(&bits[id >> 5], 1u << (id & 31));
+            else pages_error(PAGES_BAD_ID);
+        }
+    }
+    __syncthreads();
+    const int per = (words + CP_THREADS - 1) / CP_THREADS, w0 = min(words, tid * per), w1 = min(words, w0 + per);
+    int mine = 0, live, holes, movers;
+    for (int w = w0; w < w1; ++w) mine += __popc(bits[w]);
+    block_scan(mine, live);
+    int nh = 0, nm = 0;
+    for (int w = w0; w < w1; ++w)
+        for (int b = 0; b < 32 && w * 32 + b < m.n_pages; ++b) {
+            const bool on = bits[w] >> b & 1u, low = w * 32 + b < live;
+            nh += !on && low;
+            nm += on && !low;
+        }
+    int h = block_scan(nh, holes), v = block_scan(nm, movers);
+    for (int w = w0; w < w1; ++w)
+        for (int b = 0; b < 32 && w * 32 + b < m.n_pages; ++b) {
+            const int id = w * 32 + b;
+            const bool on = bits[w] >> b & 1u, low = id < live;
+            if (!on && low) c.dst[h++] = id;
+            if (on && !low) { c.remap[id] = v; c.src[v++] = id; }
+        }
+    if (tid == 0) { *c.count = movers; *c.live = live; }
+}
+
+// Moves the pages and writes the new table: every entry, those behind a
+// request's length as they are.
+__global__ void __launch_bounds__(MV_THREADS)
+pages_compact_move_kernel(PageMoveArgs m, PageCompactArgs c)
+{
+    const int movers = *c.count, live = *c.live, planes = 2 * m.layers;
+    for (int i = blockIdx.x; i < movers * planes; i += gridDim.x) {
+        const int plane = i / movers, k = i - plane * movers;
+        const uint4 *from = page_at(m, plane, c.src[k]);
+        uint4 *to = page_at(m, plane, c.dst[k]);
+        for (int j = threadIdx.x; j < (int)(m.page_bytes / 16); j += MV_THREADS) to[j] = from[j];
+    }
+    const long long cells = (long long)c.n_req * c.max_pages;
+    for (long long i = blockIdx.x * (long long)MV_THREADS + threadIdx.x; i < cells; i += (long long)gridDim.x * MV_THREADS) {
+        const int r = (int)(i / c.max_pages), j = (int)(i - (long long)r * c.max_pages);
+        int id = c.table[i];
+        if (j < pages_held(m, c, r) && id >= live && id < m.n_pages) id = c.dst[c.remap[id]];
+        c.table_out[i] = id;
+    }
+}
+
+cudaError_t launch_pages_compact(const PageMoveArgs &m, const PageCompactArgs &c, cudaStream_t st)
+{
+    const size_t smem = (size_t)(m.n_pages + 31) / 32 * 4;     // 128 KiB at 2^20 pages
+    cudaError_t e = cudaFuncSetAttribute(pages_compact_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 << 10);
+    if (e != cudaSuccess) return e;
+    pages_compact_plan_kernel<<<1, CP_THREADS, smem, st>>>(m, c);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    pages_compact_move_kernel<<<148 * 8, MV_THREADS, 0, st>>>(m, c);
+    return cudaGetLastError();
+}
+
+}  // namespace coli

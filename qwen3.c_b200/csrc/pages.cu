@@ -1,0 +1,312 @@
+// Host side of the paged KV cache: the handle, its argument checks and the
+// launches of gqa_pages.cu and page_moves.cu.
+//
+// A handle names one pool of pages for all its layers, [layers][K, V]
+// [n_pages][KH][page][256] bf16, in the caller's device memory or its own, the
+// layers' q/k norm weights, and one workspace of a fixed size, so that no
+// call after coli_cuda_pages_create allocates, frees or waits: every call can
+// be captured into a graph.
+//
+// Included by backend.cu (one translation unit), after the backend state.
+#include <cmath>
+#include <new>
+
+struct ColiCudaPages {
+    int layers, n_pages, page, KH;
+    uint8_t *base;
+    bool own_base;
+    float *norm_w;            // [layers][2][256]
+    unsigned char *norm_set;  // [layers] (host)
+    uint8_t *ws, *own_ws;
+    int rot;                  // rotary frequencies as last used
+    float theta;
+    RopeFreq freq;
+};
+
+namespace {
+
+constexpr int PAGES_MAX_LAYERS = MAX_LAYERS, PAGES_MAX_REQ = 1024, PAGES_MAX_PAGES = 1 << 20;
+constexpr int PAGES_MAX_HANDLES = 256;
+ColiCudaPages *g_pages[PAGES_MAX_HANDLES] = {};   // live handles; a call with another pointer is refused
+bool g_pages_ran = false;                         // an operator ran since the last look at g_pages_error
+
+size_t pages_page_bytes(int KH, int page) { return (size_t)KH * page * GQA_HD * 2; }
+size_t pages_norm_bytes(int layers) { return (size_t)layers * 2 * GQA_HD * 4; }
+size_t pages_list_bytes(int n_pages) { return ((size_t)n_pages * 4 + 255) & ~size_t(255); }
+size_t pages_ws_bytes(int n_pages) { return 3 * pages_list_bytes(n_pages) + 256; }
+
+int pages_geometry(int layers, int n_pages, int page, int KH, int hd)
+{
+    if (layers < 1 || layers > PAGES_MAX_LAYERS) return fail("pages: layers %d out of 1..%d", layers, PAGES_MAX_LAYERS);
+    if (n_pages < 1 || n_pages > PAGES_MAX_PAGES) return fail("pages: n_pages %d out of 1..%d", n_pages, PAGES_MAX_PAGES);
+    if (page < 16 || page > 1024 || page % 16) return fail("pages: page %d is not a multiple of 16 up to 1024", page);
+    if (KH < 1 || KH > 64 || hd != GQA_HD) return fail("pages: unsupported shape KH=%d hd=%d (needs KH 1..64, hd=256)", KH, hd);
+    if ((long long)n_pages * page * KH > 0x7fffffffLL) return fail("pages: %d pages of %d x %d rows pass 2^31 rows", n_pages, page, KH);
+    return 1;
+}
+
+int pages_handle(const ColiCudaPages *p)
+{
+    READY();
+    bool known = false;
+    for (int i = 0; p && i < PAGES_MAX_HANDLES && !known; ++i) known = g_pages[i] == p;
+    if (!known) return fail("pages: not a live handle (coli_cuda_pages_create)");
+    int dev = -1;
+    CK(cudaGetDevice(&dev));
+    if (dev != G.device) return fail("pages: device %d is current, the backend runs on device %d", dev, G.device);
+    return 1;
+}
+
+void pages_release(ColiCudaPages *p)
+{
+    if (p->own_base) dev_free(p->base, (size_t)p->layers * 2 * p->n_pages * pages_page_bytes(p->KH, p->page));
+    dev_free(p->norm_w, pages_norm_bytes(p->layers));
+    dev_free(p->own_ws, pages_ws_bytes(p->n_pages));
+    delete[] p->norm_set;
+    delete p;
+}
+
+void pages_shutdown()
+{
+    for (int i = 0; i < PAGES_MAX_HANDLES; ++i) {
+        if (g_pages[i]) pages_release(g_pages[i]);
+        g_pages[i] = nullptr;
+    }
+    g_pages_ran = false;
+}
+
+int pages_check_error()
+{
+    if (!g_pages_ran) return 1;
+    int h = 0;
+    CK(cudaMemcpyFromSymbolAsync(&h, g_pages_error, sizeof(int), 0, cudaMemcpyDeviceToHost, stream()));
+    CK(cudaStreamSynchronize(stream()));
+    if (h == PAGES_OK) return 1;
+    const int zero = 0;
+    CK(cudaMemcpyToSymbolAsync(g_pages_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream()));
+    CK(cudaStreamSynchronize(stream()));
+    static const char *const what[] = {"", "a page id outside the pool", "a position or length beyond the page table",
+                                       "row offsets that do not ascend within the rows given",
+                                       "pages or requests named twice, or both read and written",
+                                       "a request index out of range"};
+    return fail("pages: a call met %s (error %d); what it names was left out", h >= 1 && h <= 5 ? what[h] : "an error", h);
+}
+
+PageMoveArgs pages_move_args(const ColiCudaPages *p)
+{
+    PageMoveArgs m{};
+    m.base = p->base; m.page_bytes = pages_page_bytes(p->KH, p->page);
+    m.layers = p->layers; m.n_pages = p->n_pages; m.page = p->page; m.KH = p->KH;
+    return m;
+}
+
+// The checks that the two attention calls share, and their kernel arguments.
+int pages_attend_args(GqaPagesArgs &a, ColiCudaPages *p, int layer, const void *qg, const void *k, const void *v,
+                      const int *base, const int *table, int max_pages, void *ctx, int H, int KH, int hd, int rot,
+                      float eps, float theta)
+{
+    if (layer < 0 || layer >= p->layers) return fail("pages: layer %d out of range", layer);
+    const int group = KH > 0 ? H / KH : 0;
+    if (hd != GQA_HD || KH != p->KH || H != group * KH || (group != 1 && group != 2 && group != 4 && group != 8))
+        return fail("pages: unsupported GQA shape H=%d KH=%d hd=%d (needs hd=256, KH=%d, H / KH 1, 2, 4 or 8)", H, KH, hd, p->KH);
+    if (!p->norm_set[layer]) return fail("pages: q/k norm weights of layer %d not set (coli_cuda_pages_norm_weight)", layer);
+    if (rot < 2 || rot > hd || (rot & 1)) return fail("pages: bad rot %d", rot);
+    if (!(eps >= 0.f) || !(theta > 0.f) || std::isinf(eps) || std::isinf(theta)) return fail("pages: bad eps or theta");
+    if (max_pages < 1 || (long long)max_pages * p->page > 0x7fffffffLL) return fail("pages: bad max_pages %d", max_pages);
+    if (!qg || !k || !v || !base || !table || !ctx) return fail("pages: a null pointer among the arguments");
+    if (((uintptr_t)qg | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ctx) & 15)
+        return fail("pages: qg, k, v and ctx must be 16-byte aligned");
+    if (p->rot != rot || p->theta != theta) {
+        for (int j = 0; j < rot / 2; ++j) p->freq.f[j] = std::pow((double)theta, -2.0 * j / rot);
+        p->rot = rot;
+        p->theta = theta;
+    }
+    const size_t plane = (size_t)p->n_pages * pages_page_bytes(p->KH, p->page);
+    a.pv.k = (__nv_bfloat16 *)(p->base + 2 * layer * plane);
+    a.pv.v = (__nv_bfloat16 *)(p->base + (2 * layer + 1) * plane);
+    a.pv.table = table; a.pv.n_pages = p->n_pages; a.pv.page = p->page; a.pv.KH = KH; a.pv.max_pages = max_pages;
+    a.qg = qg; a.k = k; a.v = v; a.ctx = ctx; a.base = base;
+    a.qnw = p->norm_w + (size_t)layer * 2 * GQA_HD; a.knw = a.qnw + GQA_HD;
+    a.H = H; a.rot = rot; a.eps = eps;
+    a.scale_log2 = (1.f / sqrtf((float)hd)) * 1.4426950408889634f;
+    return 1;
+}
+
+int pages_attend_run(const ColiCudaPages *p, const GqaPagesArgs &a, int bf16)
+{
+    g_pages_ran = true;
+    CK(launch_pages_append(a, p->freq, bf16, stream()));
+    CK(launch_pages_attend(a, p->freq, bf16, stream()));
+    g_launches += 2;
+    return 1;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t coli_cuda_pages_bytes(int layers, int n_pages, int page, int KH, int hd)
+{
+    if (!pages_geometry(layers, n_pages, page, KH, hd)) return 0;
+    return (size_t)layers * 2 * n_pages * pages_page_bytes(KH, page);
+}
+
+int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int page, int KH, int hd, void *kv_dev)
+{
+    READY();
+    if (!pages) return fail("pages: null handle");
+    if (!pages_geometry(layers, n_pages, page, KH, hd)) return 0;
+    if ((uintptr_t)kv_dev & 127) return fail("pages: kv_dev must be 128-byte aligned");
+    int slot = 0;
+    while (slot < PAGES_MAX_HANDLES && g_pages[slot]) ++slot;
+    if (slot == PAGES_MAX_HANDLES) return fail("pages: %d handles are alive already", PAGES_MAX_HANDLES);
+    ColiCudaPages *p = new (std::nothrow) ColiCudaPages();
+    if (!p) return fail("pages: out of host memory");
+    p->layers = layers; p->n_pages = n_pages; p->page = page; p->KH = KH;
+    p->base = (uint8_t *)kv_dev;
+    p->norm_set = new (std::nothrow) unsigned char[layers]();
+    const size_t bytes = (size_t)layers * 2 * n_pages * pages_page_bytes(KH, page);
+    int ok = p->norm_set != nullptr;
+    if (!ok) fail("pages: out of host memory");
+    if (ok && !kv_dev) {
+        ok = dev_alloc((void **)&p->base, bytes);
+        p->own_base = ok;
+        if (ok && cudaMemsetAsync(p->base, 0, bytes, stream()) != cudaSuccess) ok = cuda_fail(cudaGetLastError(), "pages memset");
+    }
+    ok = ok && dev_alloc((void **)&p->norm_w, pages_norm_bytes(layers)) && dev_alloc((void **)&p->own_ws, pages_ws_bytes(n_pages));
+    p->ws = p->own_ws;
+    if (!ok) { pages_release(p); return 0; }
+    g_pages[slot] = p;
+    *pages = p;
+    return 1;
+}
+
+void coli_cuda_pages_free(ColiCudaPages *pages)
+{
+    if (!pages) return;
+    for (int i = 0; i < PAGES_MAX_HANDLES; ++i) {
+        if (g_pages[i] != pages) continue;
+        cudaStreamSynchronize(stream());   // queued calls may still use the pool and the workspace
+        pages_release(pages);
+        g_pages[i] = nullptr;
+    }
+}
+
+int coli_cuda_pages_device_ptr(const ColiCudaPages *pages, int layer, void **k, void **v)
+{
+    if (!pages_handle(pages)) return 0;
+    if (layer < 0 || layer >= pages->layers) return fail("pages: layer %d out of range", layer);
+    const size_t plane = (size_t)pages->n_pages * pages_page_bytes(pages->KH, pages->page);
+    if (k) *k = pages->base + 2 * layer * plane;
+    if (v) *v = pages->base + (2 * layer + 1) * plane;
+    return 1;
+}
+
+int coli_cuda_pages_norm_weight(ColiCudaPages *pages, int layer, const float *qnw, const float *knw, int hd)
+{
+    if (!pages_handle(pages)) return 0;
+    if (layer < 0 || layer >= pages->layers) return fail("pages: layer %d out of range", layer);
+    if (hd != GQA_HD || !qnw || !knw) return fail("pages: bad norm weights (hd=%d)", hd);
+    float *d = pages->norm_w + (size_t)layer * 2 * GQA_HD;
+    CK(cudaMemcpyAsync(d, qnw, GQA_HD * 4, cudaMemcpyHostToDevice, stream()));
+    CK(cudaMemcpyAsync(d + GQA_HD, knw, GQA_HD * 4, cudaMemcpyHostToDevice, stream()));
+    CK(cudaStreamSynchronize(stream()));
+    pages->norm_set[layer] = 1;
+    return 1;
+}
+
+size_t coli_cuda_pages_workspace_bytes(const ColiCudaPages *pages)
+{
+    return pages_handle(pages) ? pages_ws_bytes(pages->n_pages) : 0;
+}
+
+int coli_cuda_pages_set_workspace(ColiCudaPages *pages, void *ws, size_t bytes)
+{
+    if (!pages_handle(pages)) return 0;
+    if (ws && (bytes < pages_ws_bytes(pages->n_pages) || ((uintptr_t)ws & 255)))
+        return fail("pages: the workspace needs %zu bytes, 256-byte aligned", pages_ws_bytes(pages->n_pages));
+    pages->ws = ws ? (uint8_t *)ws : pages->own_ws;
+    return 1;
+}
+
+int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const void *qg, const void *k, const void *v,
+                                   const int *pos_dev, const int *table, int max_pages, void *ctx, int H, int KH, int hd,
+                                   int rot, float eps, float theta, int dtype)
+{
+    if (!pages_handle(pages)) return 0;
+    if (dtype != 0 && dtype != 1) return fail("dtype must be 0 (fp32) or 1 (bf16)");
+    if (B < 0 || B > PAGES_MAX_REQ) return fail("pages: batch %d out of 0..%d", B, PAGES_MAX_REQ);
+    if (B == 0) return 1;
+    GqaPagesArgs a{};
+    if (!pages_attend_args(a, pages, layer, qg, k, v, pos_dev, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
+    a.n_req = a.S = B;
+    return pages_attend_run(pages, a, dtype);
+}
+
+int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, int S, const int *cu, const int *pos_base,
+                                    const void *qg, const void *k, const void *v, const int *table, int max_pages,
+                                    void *ctx, int H, int KH, int hd, int rot, float eps, float theta, int dtype)
+{
+    if (!pages_handle(pages)) return 0;
+    if (dtype != 1) return fail("pages: prefill takes bf16 activations (dtype 1)");
+    if (n_seq < 0 || n_seq > PAGES_MAX_REQ) return fail("pages: %d sequences out of 0..%d", n_seq, PAGES_MAX_REQ);
+    if (S < 0 || S > 1 << 24) return fail("pages: %d rows out of 0..2^24", S);
+    if (n_seq == 0 || S == 0) return 1;
+    if (!cu) return fail("pages: a null pointer among the arguments");
+    GqaPagesArgs a{};
+    if (!pages_attend_args(a, pages, layer, qg, k, v, pos_base, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
+    a.cu = cu;
+    a.n_req = n_seq; a.S = S;
+    return pages_attend_run(pages, a, 1);
+}
+
+int coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const int *dst)
+{
+    if (!pages_handle(pages)) return 0;
+    if (n < 0 || n > pages->n_pages) return fail("pages: %d pairs for %d pages", n, pages->n_pages);
+    if (n == 0) return 1;
+    if (!src || !dst) return fail("pages: a null pointer among the arguments");
+    g_pages_ran = true;
+    CK(launch_pages_copy(pages_move_args(pages), n, src, dst, stream()));
+    g_launches += 1;
+    return 1;
+}
+
+int coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, const int *child, const int *fresh, int *len,
+                             int *table, int n_req, int max_pages)
+{
+    if (!pages_handle(pages)) return 0;
+    if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 0x7fffffffLL)
+        return fail("pages: bad table %d x %d", n_req, max_pages);
+    if (n < 0 || n >= n_req) return fail("pages: %d forks among %d requests", n, n_req);
+    if (n == 0) return 1;
+    if (!parent || !child || !fresh || !len || !table) return fail("pages: a null pointer among the arguments");
+    PageForkArgs f{};
+    f.parent = parent; f.child = child; f.fresh = fresh; f.len = len; f.table = table;
+    f.n = n; f.n_req = n_req; f.max_pages = max_pages;
+    g_pages_ran = true;
+    CK(launch_pages_fork(pages_move_args(pages), f, stream()));
+    g_launches += 1;
+    return 1;
+}
+
+int coli_cuda_pages_compact_dev(ColiCudaPages *pages, int n_req, const int *len, const int *table, int max_pages,
+                                int *table_out, int *live)
+{
+    if (!pages_handle(pages)) return 0;
+    if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 0x7fffffffLL)
+        return fail("pages: bad table %d x %d", n_req, max_pages);
+    if (!len || !table || !table_out || !live) return fail("pages: a null pointer among the arguments");
+    PageCompactArgs c{};
+    const size_t list = pages_list_bytes(pages->n_pages);
+    c.len = len; c.table = table; c.table_out = table_out; c.live = live;
+    c.src = (int *)pages->ws; c.dst = (int *)(pages->ws + list); c.remap = (int *)(pages->ws + 2 * list);
+    c.count = (int *)(pages->ws + 3 * list);
+    c.n_req = n_req; c.max_pages = max_pages;
+    g_pages_ran = true;
+    CK(launch_pages_compact(pages_move_args(pages), c, stream()));
+    g_launches += 2;
+    return 1;
+}
+
+}  // extern "C"

@@ -1,0 +1,494 @@
+"""The paged KV cache on the GPU: decode and ragged prefill over pages, page
+copies, forks and compaction, against a 64-bit restatement (pages_ref)."""
+import numpy as np
+import pytest
+
+import pages_ref as ref
+from conftest import load_pkg
+from helpers import assert_close
+
+pytestmark = pytest.mark.gpu
+
+HD, ROT, EPS, THETA = 256, 64, 1e-6, 1e7
+
+
+@pytest.fixture(scope="module")
+def be():
+    import torch
+    pkg = load_pkg()
+    pkg.build()
+    b = pkg.Backend(0)
+    b.set_stream(torch.cuda.current_stream().cuda_stream or 1)   # 1: the legacy default stream
+    yield b
+    b.shutdown()
+
+
+def ints(x):
+    import torch
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+
+
+class Pool:
+    """A paged cache over a torch tensor, with norm weights per layer."""
+
+    def __init__(self, be, n_pages, page, KH, layers=1, seed=0):
+        import torch
+        self.torch, self.be, self.page, self.KH = torch, be, page, KH
+        self.g = torch.Generator(device="cuda").manual_seed(seed)
+        self.kv = self.randn(layers, 2, n_pages, KH, page, HD, dtype=torch.bfloat16)
+        self.cache = load_pkg().PagedCache(be, layers, n_pages, page, KH, kv=self.kv.data_ptr())
+        self.qnw, self.knw = ((self.randn(HD) * 0.1).cpu().numpy() for _ in range(2))
+        for layer in range(layers):
+            self.cache.norm_weight(layer, self.qnw, self.knw)
+
+    def randn(self, *shape, dtype=None):
+        return self.torch.randn(shape, generator=self.g, device="cuda").to(dtype or self.torch.float32)
+
+    def inputs(self, rows, H, dtype):
+        t = self.torch.bfloat16 if dtype else self.torch.float32
+        qg, k, v = (self.randn(rows, n, w, dtype=t) for n, w in ((H, 2 * HD), (self.KH, HD), (self.KH, HD)))
+        return qg, k, v, self.torch.full((rows, H, HD), 7.0, dtype=t, device="cuda")
+
+    def host(self, layer=0):
+        return self.kv[layer].float().cpu().numpy().astype(np.float64)
+
+
+def pages_for(lens, page, n_pages, seed, spare=0):
+    """A random table with pages of their own for each length; behind them, ids that must not be used."""
+    rng = np.random.default_rng(seed)
+    counts = [max(0, -(-int(n) // page)) for n in lens]
+    ids = rng.permutation(n_pages)
+    table = np.full((len(lens), max(1, max(counts)) + spare), 1 << 30, np.int32)
+    at = 0
+    for r, c in enumerate(counts):
+        table[r, :c] = ids[at:at + c]
+        at += c
+    assert at <= n_pages
+    return table
+
+
+def poison(P, table, lens):
+    """NaN and infinities in every cache row that no request holds."""
+    t = P.torch
+    held = t.zeros(P.kv.shape[2], P.page, dtype=t.bool, device="cuda")
+    for r, n in enumerate(lens):
+        at = t.arange(max(0, int(n)), device="cuda")
+        held[ints(table[r]).long()[at // P.page], at % P.page] = True
+    junk = t.where(P.randn(*P.kv.shape) > 0, float("nan"), float("inf")).bfloat16()
+    P.kv.copy_(t.where(held[None, None, :, None, :, None], P.kv, junk))
+
+
+def check_rows(P, before, qg, k, v, ctx, table, placed, group, dtype, rot=ROT, theta=THETA):
+    """placed: (row, request, position) of every row the call was to compute, in cache order."""
+    after = P.host()
+    u, u_out = (2.0 ** -8, 2.0 ** -8) if dtype else (2.0 ** -16, 2.0 ** -24)
+    qg64, k64, v64 = (x.double().cpu().numpy() for x in (qg, k, v))
+    got = ctx.double().cpu().numpy()
+    row, req, pos = (np.array(x) for x in zip(*placed))
+    kn = ref.norm_rope(k64[row], P.knw, pos, rot, EPS, theta)
+    at = table[req, pos // P.page], pos % P.page
+    # the appended rows: rounded to bf16 from values good to about 2^-20
+    np.testing.assert_allclose(after[0][at[0], :, at[1]], kn, rtol=2.0 ** -8 + 2.0 ** -16, atol=1e-4)
+    np.testing.assert_array_equal(after[1][at[0], :, at[1]], ref.bf16(v64[row]))
+    # no other row changed, bit for bit
+    want = before.copy()
+    for which in (0, 1):
+        want[which][at[0], :, at[1]] = after[which][at[0], :, at[1]]
+    np.testing.assert_array_equal(after, want)
+    q = ref.norm_rope(qg64[row][..., :HD], P.qnw, pos, rot, EPS, theta)
+    outs, refs = [], []
+    for i, (n, r, t) in enumerate(placed):
+        o, tol = ref.attend(q[i], qg64[n][..., HD:], ref.rows_of(after, table[r], P.page, t + 1), group, u, u_out)
+        assert np.all(np.abs(got[n] - o) <= tol), f"row {n} request {r} position {t}: {np.max(np.abs(got[n] - o) / tol)}"
+        outs.append(got[n]); refs.append(o)
+    assert_close(np.array(outs), np.array(refs), max_abs=2e-2 if dtype else 2e-4, what="ctx")
+
+
+DECODE = [
+    # lengths (0: an idle slot), page, KH, group, dtype
+    ([1], 16, 2, 8, 1),
+    ([16, 17, 15, 1], 16, 2, 8, 1),
+    ([64, 65, 0, 63, 1, 128], 64, 2, 8, 1),
+    ([300, 0, 0, 4093], 48, 2, 8, 1),
+    ([5000], 256, 1, 8, 1),
+    ([257, 31, 1000], 32, 4, 4, 0),
+    ([1, 2, 777], 16, 2, 8, 0),
+    ([129, 500], 128, 3, 1, 1),
+    ([129, 500], 1024, 2, 2, 0),
+    (list(range(1, 66)), 16, 1, 4, 1),
+    ([20000, 3], 64, 2, 8, 1),
+]
+
+
+@pytest.mark.parametrize("lens,page,KH,group,dtype", DECODE)
+def test_decode(be, lens, page, KH, group, dtype):
+    n_pages = sum(-(-n // page) for n in lens) + 3
+    P = Pool(be, n_pages, page, KH, seed=len(lens) * 131 + lens[0])
+    table = pages_for(lens, page, n_pages, seed=lens[0], spare=2)
+    poison(P, table, lens)
+    before = P.host()
+    qg, k, v, ctx = P.inputs(len(lens), KH * group, dtype)
+    pos = ints([n - 1 for n in lens])
+    td = ints(table)
+    P.cache.decode_dev(0, len(lens), qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), table.shape[1],
+                       ctx.data_ptr(), H=KH * group, rot=ROT, eps=EPS, theta=THETA, dtype=dtype)
+    be.sync()
+    placed = [(r, r, n - 1) for r, n in enumerate(lens) if n]
+    check_rows(P, before, qg, k, v, ctx, table, placed, group, dtype)
+    for r, n in enumerate(lens):
+        if not n:
+            assert (ctx[r] == 7).all(), "an idle slot's row was written"
+
+
+@pytest.mark.parametrize("rot,theta", [(256, 1e7), (2, 1e4), (36, 5e5)])
+def test_decode_rotary_widths(be, rot, theta):
+    lens, page, KH, group = [900, 33], 32, 2, 8
+    P = Pool(be, 40, page, KH, seed=rot)
+    table = pages_for(lens, page, 40, seed=1)
+    before = P.host()
+    qg, k, v, ctx = P.inputs(2, 16, 1)
+    pos, td = ints([n - 1 for n in lens]), ints(table)
+    P.cache.decode_dev(0, 2, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), table.shape[1],
+                       ctx.data_ptr(), rot=rot, eps=EPS, theta=theta)
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, table, [(0, 0, 899), (1, 1, 32)], group, 1, rot, theta)
+
+
+PREFILL = [
+    # rows and context of each chunk, page, KH, group, rows behind the last chunk
+    ([(1, 0)], 16, 2, 8, 0),
+    ([(16, 0)], 16, 2, 8, 3),
+    ([(17, 0), (0, 50), (1, 127), (1, 128), (33, 100)], 16, 2, 8, 5),
+    ([(130, 0)], 64, 2, 8, 0),
+    ([(200, 300), (3, 1000), (1, 0)], 48, 2, 8, 1),
+    ([(70, 59), (129, 1)], 128, 1, 1, 2),
+    ([(70, 59), (129, 1)], 32, 3, 2, 0),
+    ([(65, 190), (64, 64), (1, 31)], 1024, 2, 4, 0),
+    ([(300, 2100)], 256, 2, 8, 0),
+    ([(1, n) for n in range(0, 600, 7)], 16, 1, 8, 0),
+    ([(2, 9000)], 64, 2, 8, 0),
+]
+
+
+@pytest.mark.parametrize("chunks,page,KH,group,behind", PREFILL)
+def test_prefill(be, chunks, page, KH, group, behind):
+    total = [n + c if n else 0 for n, c in chunks]
+    n_pages = sum(-(-n // page) for n in total) + 2
+    P = Pool(be, n_pages, page, KH, seed=chunks[0][0] * 7 + len(chunks))
+    table = pages_for(total, page, n_pages, seed=3, spare=1)
+    poison(P, table, total)
+    before = P.host()
+    cu = np.concatenate([[0], np.cumsum([n for n, _ in chunks])])
+    S = int(cu[-1]) + behind
+    qg, k, v, ctx = P.inputs(S, KH * group, 1)
+    cu_d, base, td = ints(cu), ints([c for _, c in chunks]), ints(table)
+    P.cache.prefill_dev(0, len(chunks), S, cu_d.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(),
+                        td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group, rot=ROT, eps=EPS, theta=THETA)
+    be.sync()
+    placed = [(int(cu[r]) + i, r, c + i) for r, (n, c) in enumerate(chunks) for i in range(n)]
+    check_rows(P, before, qg, k, v, ctx, table, placed, group, 1)
+    assert (ctx[int(cu[-1]):] == 7).all(), "rows behind the last chunk were written"
+
+
+def test_bad_ids_and_positions_are_reported_and_left_out(be):
+    """A page id outside the pool, a position beyond the table, offsets that
+    descend: reported once by the next sync, the other requests computed."""
+    BackendError = load_pkg().BackendError
+    P = Pool(be, 8, 16, 2, seed=5)
+    table = np.array([[0, 1], [8, 2], [3, -1], [4, 5]], np.int32)
+    pos = [20, 3, 30, 32]                      # ok, bad id, bad id, beyond 2 pages
+    before = P.host()
+    qg, k, v, ctx = P.inputs(4, 16, 1)
+    pd, td = ints(pos), ints(table)
+    P.cache.decode_dev(0, 4, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pd.data_ptr(), td.data_ptr(), 2, ctx.data_ptr())
+    with pytest.raises(BackendError, match="page id outside|beyond the page table"):
+        be.sync()
+    be.sync()                                  # reported once, still usable
+    check_rows(P, before, qg, k, v, ctx, table, [(0, 0, 20)], 8, 1)
+    assert (ctx[3] == 7).all()
+    before = P.host()
+    cu, base = ints([0, 3, 1, 4, 9]), ints([0, 0, 2, 0])
+    qg, k, v, ctx = P.inputs(4, 16, 1)
+    table = np.array([[0, 1], [2, 3], [4, 5], [6, 7]], np.int32)
+    td = ints(table)
+    P.cache.prefill_dev(0, 4, 4, cu.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(), td.data_ptr(), 2,
+                        ctx.data_ptr())
+    with pytest.raises(BackendError, match="offsets"):
+        be.sync()
+    be.sync()
+
+
+# ------------------------------------------------------------------ page moves
+@pytest.mark.parametrize("n,page,KH,layers", [(1, 16, 1, 1), (3, 48, 2, 3), (7, 1024, 1, 2), (60, 16, 2, 10)])
+def test_copy(be, n, page, KH, layers):
+    P = Pool(be, 2 * n + 3, page, KH, layers, seed=n)
+    ids = np.random.default_rng(n).permutation(2 * n + 3)
+    src, dst = ids[:n].copy(), ids[n:2 * n]
+    src[-1] = src[0]                           # one source, two destinations
+    want = P.kv.clone()
+    want[:, :, dst] = P.kv[:, :, src]
+    s, d = ints(src), ints(dst)
+    P.cache.copy_dev(n, s.data_ptr(), d.data_ptr())
+    be.sync()
+    assert P.torch.equal(P.kv.view(P.torch.int16), want.view(P.torch.int16))
+
+
+def test_copy_leaves_out_conflicts(be):
+    BackendError = load_pkg().BackendError
+    P = Pool(be, 16, 16, 2, 2, seed=2)
+    #        ok  dup  dup  chain reads 5 -> left out; 4 -> 5 stays; out of the pool; onto itself
+    src, dst = [0, 1, 2, 5, 4, 6, 16, 9], [8, 3, 3, 7, 5, 99, 10, 9]
+    want = P.kv.clone()
+    want[:, :, [8, 5]] = P.kv[:, :, [0, 4]]
+    s, d = ints(src), ints(dst)
+    P.cache.copy_dev(8, s.data_ptr(), d.data_ptr())
+    with pytest.raises(BackendError, match="named twice|page id outside"):
+        be.sync()
+    be.sync()
+    assert P.torch.equal(P.kv.view(P.torch.int16), want.view(P.torch.int16))
+
+
+def fork_want(P, table, lens, parent, child, fresh):
+    kv, table, lens = P.kv.clone(), table.copy(), list(lens)
+    for a, c, f in zip(parent, child, fresh):
+        full, tail = divmod(lens[a], P.page)
+        table[c, :full] = table[a, :full]
+        if tail:
+            table[c, full] = f
+            kv[:, :, f, :, :tail] = P.kv[:, :, table[a, full], :, :tail]
+        lens[c] = lens[a]
+    return kv, table, lens
+
+
+@pytest.mark.parametrize("page,KH,layers,lens", [(16, 2, 2, [0, 1, 15, 16, 17, 100]), (64, 1, 10, [63, 64, 65, 640]), (1024, 2, 1, [1023, 1])])
+def test_fork(be, page, KH, layers, lens):
+    kids = 2 * len(lens)
+    held = sum(-(-n // page) for n in lens)
+    P = Pool(be, held + kids, page, KH, layers, seed=page)
+    table = np.full((len(lens) + kids, max(-(-n // page) for n in lens)), -5, np.int32)
+    ids = np.random.default_rng(0).permutation(held + kids)
+    at = 0
+    for r, n in enumerate(lens):
+        c = -(-n // page)
+        table[r, :c] = ids[at:at + c]
+        at += c
+    parent = [i % len(lens) for i in range(kids)]
+    child, fresh = list(range(len(lens), len(lens) + kids)), ids[at:]
+    all_lens = lens + [0] * kids
+    kv, want_table, want_lens = fork_want(P, table, all_lens, parent, child, fresh)
+    p, c, f, td, ld = ints(parent), ints(child), ints(fresh), ints(table), ints(all_lens)
+    P.cache.fork_dev(kids, p.data_ptr(), c.data_ptr(), f.data_ptr(), ld.data_ptr(), td.data_ptr(), len(all_lens), table.shape[1])
+    be.sync()
+    np.testing.assert_array_equal(td.cpu().numpy(), want_table)
+    assert ld.tolist() == want_lens
+    assert P.torch.equal(P.kv.view(P.torch.int16), kv.view(P.torch.int16))
+
+
+def test_fork_leaves_out_conflicts(be):
+    BackendError = load_pkg().BackendError
+    P = Pool(be, 12, 16, 1, 1, seed=4)
+    lens = [20, 5, 0, 0, 0, 0, 0, 0]
+    table = np.array([[0, 1], [2, 9]] + [[-1, -1]] * 6, np.int32)
+    # ok; child twice (both out); child that is a parent (both out); fresh page twice (both out); request 8; length beyond
+    parent, child, fresh = [0, 1, 1, 4, 1, 0], [2, 3, 3, 6, 4, 8], [5, 6, 7, 8, 10, 11]
+    want_kv, want_table, want_lens = fork_want(P, table, lens, [0], [2], [5])
+    p, c, f, td, ld = ints(parent), ints(child), ints(fresh), ints(table), ints(lens)
+    P.cache.fork_dev(6, p.data_ptr(), c.data_ptr(), f.data_ptr(), ld.data_ptr(), td.data_ptr(), 8, 2)
+    with pytest.raises(BackendError, match="named twice|request index"):
+        be.sync()
+    be.sync()
+    np.testing.assert_array_equal(td.cpu().numpy(), want_table)
+    assert ld.tolist() == want_lens
+    assert P.torch.equal(P.kv.view(P.torch.int16), want_kv.view(P.torch.int16))
+
+
+@pytest.mark.parametrize("n_pages,page,lens,shared", [
+    (1, 16, [1], False), (33, 16, [0, 100, -3, 17], False), (64, 48, [400, 1000, 48, 47], True),
+    (200, 16, [3200], False), (90, 16, [0, 0], False), (1100, 16, [500] * 12, True)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_compact(be, n_pages, page, lens, shared, in_place):
+    P = Pool(be, n_pages, page, 2, 2, seed=n_pages)
+    table = pages_for(lens, page, n_pages, seed=n_pages, spare=1)
+    table[table == 1 << 30] = -1
+    if shared:                                 # a forked request's pages count once
+        table[-1, 0] = table[0, 0]
+    want_table, live, moves = ref.compact(table, lens, page, n_pages)
+    want = P.kv.clone()
+    if moves:
+        src, dst = (list(x) for x in zip(*moves))
+        want[:, :, dst] = P.kv[:, :, src]
+    ld, td, lv = ints(lens), ints(table), ints([-1])
+    out = td if in_place else ints(np.zeros_like(table))
+    P.cache.compact_dev(len(lens), ld.data_ptr(), td.data_ptr(), table.shape[1], out.data_ptr(), lv.data_ptr())
+    be.sync()
+    assert lv.item() == live
+    np.testing.assert_array_equal(out.cpu().numpy(), want_table)
+    assert P.torch.equal(P.kv.view(P.torch.int16), want.view(P.torch.int16))
+
+
+def test_zero_sized_calls_do_nothing(be):
+    P = Pool(be, 4, 16, 2, seed=1)
+    want = P.kv.clone()
+    P.cache.decode_dev(0, 0, 0, 0, 0, 0, 0, 1, 0)
+    P.cache.prefill_dev(0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 0)
+    P.cache.copy_dev(0, 0, 0)
+    P.cache.fork_dev(0, 0, 0, 0, 0, 0, 1, 1)
+    be.sync()
+    assert P.torch.equal(P.kv, want)
+
+
+def test_refusals(be):
+    pkg = load_pkg()
+    BackendError = pkg.BackendError
+    import torch
+    P = Pool(be, 4, 16, 2, seed=1)
+    c = P.cache
+    x = torch.zeros(1 << 16, dtype=torch.float32, device="cuda")
+    p = x.data_ptr()
+    ok = dict(H=16)
+    with pytest.raises(BackendError, match="layer"):
+        c.decode_dev(1, 1, p, p, p, p, p, 1, p, **ok)
+    with pytest.raises(BackendError, match="shape"):
+        c.decode_dev(0, 1, p, p, p, p, p, 1, p, H=12)
+    with pytest.raises(BackendError, match="shape"):
+        c.decode_dev(0, 1, p, p, p, p, p, 1, p, H=32)
+    with pytest.raises(BackendError, match="batch"):
+        c.decode_dev(0, 1025, p, p, p, p, p, 1, p, **ok)
+    with pytest.raises(BackendError, match="batch"):
+        c.decode_dev(0, -1, p, p, p, p, p, 1, p, **ok)
+    with pytest.raises(BackendError, match="rot"):
+        c.decode_dev(0, 1, p, p, p, p, p, 1, p, rot=7, **ok)
+    with pytest.raises(BackendError, match="dtype"):
+        c.decode_dev(0, 1, p, p, p, p, p, 1, p, dtype=2, **ok)
+    with pytest.raises(BackendError, match="eps or theta"):
+        c.decode_dev(0, 1, p, p, p, p, p, 1, p, theta=0.0, **ok)
+    with pytest.raises(BackendError, match="aligned"):
+        c.decode_dev(0, 1, p + 2, p, p, p, p, 1, p, **ok)
+    with pytest.raises(BackendError, match="null"):
+        c.decode_dev(0, 1, p, p, p, 0, p, 1, p, **ok)
+    with pytest.raises(BackendError, match="max_pages"):
+        c.decode_dev(0, 1, p, p, p, p, p, 1 << 30, p, **ok)
+    with pytest.raises(BackendError, match="bf16"):
+        c.prefill_dev(0, 1, 1, p, p, p, p, p, p, 1, p, dtype=0, **ok)
+    with pytest.raises(BackendError, match="sequences"):
+        c.prefill_dev(0, 1025, 1, p, p, p, p, p, p, 1, p, **ok)
+    with pytest.raises(BackendError, match="pairs"):
+        c.copy_dev(5, p, p)
+    with pytest.raises(BackendError, match="forks"):
+        c.fork_dev(2, p, p, p, p, p, 2, 1)
+    with pytest.raises(BackendError, match="workspace"):
+        c.set_workspace(p, 16)
+    bare = pkg.PagedCache(be, 1, 4, 16, 2)
+    with pytest.raises(BackendError, match="norm weights"):
+        bare.decode_dev(0, 1, p, p, p, p, p, 1, p, **ok)
+    bare.free()
+    with pytest.raises(BackendError, match="live handle"):
+        bare.copy_dev(1, p, p)
+    for bad in (dict(page=24), dict(page=8), dict(n_pages=0), dict(KH=0), dict(hd=128), dict(layers=0), dict(n_pages=1 << 21)):
+        with pytest.raises(BackendError, match="pages"):
+            pkg.PagedCache(be, **{**dict(layers=1, n_pages=4, page=16, KH=2), **bad})
+    be.sync()
+
+
+# ------------------------------------------------------------------ as used together
+def test_serving_run_matches_contiguous_cache(be):
+    """Two prompts prefilled together in two chunks, one forked into three
+    samples, six steps decoded from a captured graph, a request dropped and the
+    pool compacted, three more steps: each step equals the contiguous cache's
+    decode of the same tokens."""
+    import torch
+    page, KH, H, layers, R = 16, 2, 16, 2, 6
+    P = Pool(be, 64, page, KH, layers, seed=9)
+    st = torch.cuda.Stream()
+    lens = [45, 80]
+    ids = list(np.random.default_rng(1).permutation(64))
+    table = np.full((R, 8), -1, np.int32)
+    for r, n in enumerate(lens):
+        for j in range(-(-(n + 12) // page)):
+            table[r, j] = ids.pop()
+    td = ints(table)
+    tokens = {r: [P.inputs(n, H, 1)[:3] for _ in range(layers)] for r, n in enumerate(lens)}   # per layer q|gate, k, v
+    for lo, hi in ((0, 30), (30, 80)):
+        part = [(max(0, min(n, hi) - lo)) for n in lens]
+        cu, base = ints(np.concatenate([[0], np.cumsum(part)])), ints([lo if p else 0 for p in part])
+        for layer in range(layers):
+            x = [torch.cat([tokens[r][layer][i][lo:lo + p] for r, p in enumerate(part)]) for i in range(3)]
+            ctx = torch.zeros(sum(part), H, HD, dtype=torch.bfloat16, device="cuda")
+            P.cache.prefill_dev(layer, 2, sum(part), cu.data_ptr(), base.data_ptr(), *(t.data_ptr() for t in x), td.data_ptr(),
+                                8, ctx.data_ptr())
+            be.sync()
+    # the contiguous cache, fed with the same prompts
+    be.kv_reset()
+    for layer in range(layers):
+        be.kv_ensure(layer, R, KH, 128)
+        be.gqa_norm_weight(layer, P.qnw, P.knw)
+    heir = {0: 0, 1: 1, 2: 0, 3: 0, 4: 0}
+    for r, a in heir.items():
+        for layer in range(layers):
+            x = tokens[a][layer]
+            out = torch.zeros(lens[a], H, HD, dtype=torch.bfloat16, device="cuda")
+            be.gqa_step_dev(layer, r, lens[a], 0, *(t.data_ptr() for t in x), out.data_ptr())
+            be.sync()
+    # fork request 0 into 2, 3 and 4
+    ld = ints(lens + [0] * 4)
+    for r in (2, 3, 4):
+        for j in range(2, 4):
+            table[r, j] = ids.pop()
+    td[2:5, 3] = ints(table[2:5, 3])
+    parent, child, fresh = ints([0, 0, 0]), ints([2, 3, 4]), ints(table[2:5, 2])
+    P.cache.fork_dev(3, parent.data_ptr(), child.data_ptr(), fresh.data_ptr(), ld.data_ptr(), td.data_ptr(), R, 8)
+    be.sync()
+    assert ld.tolist() == [45, 80, 45, 45, 45, 0]
+    pos = torch.where(ld > 0, ld, -1).int()
+    x = [[t.clone() for t in P.inputs(R, H, 1)] for _ in range(layers)]
+
+    def step():
+        for layer in range(layers):
+            qg, k, v, ctx = (t.data_ptr() for t in x[layer])
+            P.cache.decode_dev(layer, R, qg, k, v, pos.data_ptr(), td.data_ptr(), 8, ctx)
+
+    def contiguous(layer):
+        qg, k, v, _ = x[layer]
+        out = torch.zeros(R, H, HD, dtype=torch.bfloat16, device="cuda")
+        at = pos.clamp(min=0)
+        be.gqa_decode_dev(layer, R, qg.data_ptr(), k.data_ptr(), v.data_ptr(), at.data_ptr(), out.data_ptr())
+        be.sync()
+        return out
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    be.set_stream(st.cuda_stream)
+    with torch.cuda.graph(graph, stream=st, capture_error_mode="thread_local"):
+        step()
+    be.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+
+    def steps(n):
+        for _ in range(n):
+            for layer in range(layers):
+                for t, new in zip(x[layer][:3], P.inputs(R, H, 1)[:3]):
+                    t.copy_(new)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            be.sync()
+            live = pos >= 0
+            for layer in range(layers):
+                want = contiguous(layer)
+                # both round q, p and the output to bf16: 2 x 2^-8 of the values on average well below the bound
+                assert_close(x[layer][3][live].float().cpu().numpy(), want[live].float().cpu().numpy(), what=f"layer {layer}")
+            pos.copy_(torch.where(live, pos + 1, pos))
+
+    steps(6)
+    pos[1] = -1                                # request 1 ends
+    ld.copy_(pos.clamp(min=0))
+    want_table, live, _ = ref.compact(td.cpu().numpy(), ld.tolist(), page, 64)
+    lv = ints([0])
+    # the next token's pages are part of what a request holds
+    hold = torch.where(pos >= 0, pos + 4, 0).int()
+    want_table, live, _ = ref.compact(td.cpu().numpy(), hold.tolist(), page, 64)
+    P.cache.compact_dev(R, hold.data_ptr(), td.data_ptr(), 8, td.data_ptr(), lv.data_ptr())
+    be.sync()
+    assert lv.item() == live
+    np.testing.assert_array_equal(td.cpu().numpy(), want_table)
+    steps(3)
+    be.kv_reset()
