@@ -195,6 +195,15 @@ struct GqaPagesArgs {
     int n_req, S, H, rot;
     float eps, scale_log2;
 };
+// Pieces of units that more than one CTA works on (workspace): piece slot
+// 2 c is CTA c's first (begun by an earlier CTA), 2 c + 1 its last (begun here).
+struct PagesPart {
+    float *o;             // [2 ctas][rows of a unit][hd]
+    float2 *ml;           // [2 ctas][rows of a unit] (max, sum), log2 domain
+    int4 *units;          // [ctas] unit that begins in CTA c and goes on: (last CTA or -1, request, KV head, ..)
+};
+cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, const GqaPagesArgs &a, const PagesPart &part,
+                                const RopeFreq &f, int in_bf16, int ctas, cudaStream_t st);
 cudaError_t launch_pages_append(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st);
 cudaError_t launch_pages_attend(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st);
 

@@ -18,6 +18,7 @@ struct ColiCudaPages {
     float *norm_w;            // [layers][2][256]
     unsigned char *norm_set;  // [layers] (host)
     uint8_t *ws, *own_ws;
+    CUtensorMap *maps;        // [layers][K, V], boxes of 16 rows
     int rot;                  // rotary frequencies as last used
     float theta;
     RopeFreq freq;
@@ -33,7 +34,37 @@ bool g_pages_ran = false;                         // an operator ran since the l
 size_t pages_page_bytes(int KH, int page) { return (size_t)KH * page * GQA_HD * 2; }
 size_t pages_norm_bytes(int layers) { return (size_t)layers * 2 * GQA_HD * 4; }
 size_t pages_list_bytes(int n_pages) { return ((size_t)n_pages * 4 + 255) & ~size_t(255); }
-size_t pages_ws_bytes(int n_pages) { return 3 * pages_list_bytes(n_pages) + 256; }
+// the workspace serves one call at a time: a compaction's lists, or an attention call's pieces
+size_t pages_part_rows() { return (size_t)2 * G.num_sms * GQA_GRP; }
+size_t pages_part_bytes() { return pages_part_rows() * (GQA_HD * 4 + 8) + (size_t)G.num_sms * 16; }
+size_t pages_ws_bytes(int n_pages)
+{
+    return (std::max(3 * pages_list_bytes(n_pages) + 256, pages_part_bytes()) + 255) & ~size_t(255);
+}
+PagesPart pages_part(uint8_t *ws)
+{
+    PagesPart t{};
+    t.o = (float *)ws;
+    t.ml = (float2 *)(ws + pages_part_rows() * GQA_HD * 4);
+    t.units = (int4 *)(t.ml + pages_part_rows());
+    return t;
+}
+
+// Rows of 256 bf16 as (64 columns, 8 rows, 4 column blocks, groups of 8 rows):
+// one box is a run of whole row groups, [group][block][8 rows][128 B] in shared
+// memory, 128B-swizzled.
+int make_pages_tmap(CUtensorMap *m, void *base, long long rows, int box_rows)
+{
+    cuuint64_t dims[4] = {64, 8, 4, (cuuint64_t)(rows / 8)};
+    cuuint64_t strides[3] = {GQA_HD * 2, 128, 8 * GQA_HD * 2};
+    cuuint32_t box[4] = {64, 8, 4, (cuuint32_t)(box_rows / 8)};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = G.encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled (pages) failed (%d)", (int)r);
+    return 1;
+}
 
 int pages_geometry(int layers, int n_pages, int page, int KH, int hd)
 {
@@ -63,6 +94,7 @@ void pages_release(ColiCudaPages *p)
     dev_free(p->norm_w, pages_norm_bytes(p->layers));
     dev_free(p->own_ws, pages_ws_bytes(p->n_pages));
     delete[] p->norm_set;
+    delete[] p->maps;
     delete p;
 }
 
@@ -132,15 +164,6 @@ int pages_attend_args(GqaPagesArgs &a, ColiCudaPages *p, int layer, const void *
     return 1;
 }
 
-int pages_attend_run(const ColiCudaPages *p, const GqaPagesArgs &a, int bf16)
-{
-    g_pages_ran = true;
-    CK(launch_pages_append(a, p->freq, bf16, stream()));
-    CK(launch_pages_attend(a, p->freq, bf16, stream()));
-    g_launches += 2;
-    return 1;
-}
-
 }  // namespace
 
 extern "C" {
@@ -165,8 +188,9 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
     p->layers = layers; p->n_pages = n_pages; p->page = page; p->KH = KH;
     p->base = (uint8_t *)kv_dev;
     p->norm_set = new (std::nothrow) unsigned char[layers]();
+    p->maps = new (std::nothrow) CUtensorMap[2 * layers];
     const size_t bytes = (size_t)layers * 2 * n_pages * pages_page_bytes(KH, page);
-    int ok = p->norm_set != nullptr;
+    int ok = p->norm_set && p->maps;
     if (!ok) fail("pages: out of host memory");
     if (ok && !kv_dev) {
         ok = dev_alloc((void **)&p->base, bytes);
@@ -175,6 +199,8 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
     }
     ok = ok && dev_alloc((void **)&p->norm_w, pages_norm_bytes(layers)) && dev_alloc((void **)&p->own_ws, pages_ws_bytes(n_pages));
     p->ws = p->own_ws;
+    for (int i = 0; ok && i < 2 * layers; ++i)
+        ok = make_pages_tmap(p->maps + i, p->base + i * (bytes / (2 * layers)), (long long)n_pages * KH * page, GQA_TILE);
     if (!ok) { pages_release(p); return 0; }
     g_pages[slot] = p;
     *pages = p;
@@ -239,8 +265,14 @@ int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const
     if (B == 0) return 1;
     GqaPagesArgs a{};
     if (!pages_attend_args(a, pages, layer, qg, k, v, pos_dev, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
+    if ((long long)B * pages->KH * max_pages * (pages->page / 16) > 0x7fffffffLL)
+        return fail("pages: a table of %d x %d pages passes 2^31 tiles", B, max_pages);
     a.n_req = a.S = B;
-    return pages_attend_run(pages, a, dtype);
+    g_pages_ran = true;
+    CK(launch_pages_decode(pages->maps[2 * layer], pages->maps[2 * layer + 1], a, pages_part(pages->ws), pages->freq, dtype,
+                           G.num_sms, stream()));
+    g_launches += 2;
+    return 1;
 }
 
 int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, int S, const int *cu, const int *pos_base,
@@ -257,7 +289,11 @@ int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, 
     if (!pages_attend_args(a, pages, layer, qg, k, v, pos_base, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
     a.cu = cu;
     a.n_req = n_seq; a.S = S;
-    return pages_attend_run(pages, a, 1);
+    g_pages_ran = true;
+    CK(launch_pages_append(a, pages->freq, 1, stream()));
+    CK(launch_pages_attend(a, pages->freq, 1, stream()));
+    g_launches += 2;
+    return 1;
 }
 
 int coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const int *dst)
