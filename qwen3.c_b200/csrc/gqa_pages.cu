@@ -20,16 +20,14 @@ enum { PAGES_OK = 0, PAGES_BAD_ID = 1, PAGES_BAD_POS = 2, PAGES_BAD_ROWS = 3, PA
 __device__ int g_pages_error;
 __device__ __forceinline__ void pages_error(int code) { atomicCAS(&g_pages_error, 0, code); }
 
-// Angle table of position pos, entries [0, rot / 2): the product and its
-// reduction to a turn in double, the sine and cosine of what is left in float.
-__device__ __forceinline__ void pages_rope_table(float *cs, float *sn, int pos, int rot, const RopeFreq &f, int tid0,
-                                                 int nthr)
+// Angle table of position pos, entries [0, rot / 2): the angle in turns is the
+// fraction of an exact 64-bit product, so far positions lose nothing.
+__device__ __forceinline__ void pages_rope_table(float *cs, float *sn, int pos, int rot, const unsigned long long *turn,
+                                                 int tid0, int nthr)
 {
-    constexpr double TURN = 6.283185307179586476925286766559;
     for (int j = tid0; j < (rot >> 1); j += nthr) {
-        const double a = (double)pos * f.f[j];
-        const float r = (float)(a - rint(a * (1.0 / TURN)) * TURN);
-        sincosf(r, &sn[j], &cs[j]);
+        const int top = (int)(((unsigned long long)pos * turn[j]) >> 32);      // 2^-32 turns, [-1/2, 1/2)
+        sincospif((float)top * 4.656612873077393e-10f, &sn[j], &cs[j]);        // 2^-31: in half turns
     }
 }
 
@@ -73,78 +71,131 @@ __device__ __forceinline__ int pages_req_of(const GqaPagesArgs &p, int row)
 }
 
 // ------------------------------------------------------------------ decode
-// The work is one list of 16-token tiles, request by request and KV head by KV
-// head, cut into equal consecutive ranges, one per CTA: a batch of any lengths
-// keeps every SM streaming to the end, and a single long request is split over
-// all of them. A range covers pieces of consecutive units (a unit: one request
-// and KV head). A piece that is a whole unit writes ctx itself; the others
-// leave (O, max, sum) in the workspace and pages_join_kernel merges a unit's
-// pieces. A CTA has at most two such pieces, its first and its last, so the
-// workspace does not depend on the batch.
+// Units are (request, KV head) pairs, in that order. A unit is a run of ring
+// entries: its q rows, its 16-token tiles, its gate rows; the list of all
+// entries is cut into equal consecutive ranges, one per warp of the grid (4
+// warps per CTA, one CTA per SM): batches of any lengths keep every SM
+// streaming to the end, and one long request is spread over all of them.
 //
-// Inside a CTA warp w takes tiles w, w + 4, .. of the range through its own TMA
-// ring (one 8 KiB box per tile of K and of V, mbarrier completion), which
-// runs on across unit borders; the page ids of a warp's next 32 tiles are
-// looked up by its 32 lanes at once, a batch ahead of their use. Per tile
-// S^T[16 tok x 8 heads] = K Q^T and O^T += V^T P^T on bf16 mma.sync, the
-// (up to) 8 query heads of the KV head being the N of the MMA. At 8 heads that
-// is 8 FLOP per byte read: HBM bounds it, and tcgen05's 64-row minimum would
-// leave 7/8 of its rows empty.
+// A warp works on its own. Everything it reads comes through its own 3-stage
+// ring of 16 KiB (mbarrier completion), which runs on across units, so that no
+// unit waits for its own loads: tiles as one TMA box of K and one of V, q and
+// gate rows as bulk copies. 32 entries are looked up at once by the 32 lanes, a
+// batch ahead of their use. The warp norms and ropes q, and writes the ctx of
+// a unit that it holds whole. What warps of one CTA share of a unit is merged
+// in shared memory when the ranges are done; what CTAs share goes through the
+// workspace to pages_join_kernel: at most two pieces per CTA, whatever the
+// batch.
+//
+// Per tile S^T[16 tok x 8 heads] = K Q^T and O^T += V^T P^T on bf16 mma.sync,
+// the (up to) 8 query heads of the KV head being the N of the MMA: 8 FLOP per
+// byte read, so HBM bounds it, and tcgen05's 64-row minimum would leave 7/8 of
+// its rows empty. The tensor pipe has room to spare, so q and the softmax
+// numerators are not rounded to one bf16 but enter as PARTS of them (hi + lo,
+// 16 bits, for bf16 activations; three parts, 24 bits, for fp32 ones), one MMA
+// for each.
+//
 // The new token's K and V rows are normed, roped and appended by the warp that
 // owns the unit's last tile: to the page, and over the tile's copy in shared
 // memory, so no tile load waits for an append.
-// fp32 activations: q and the probabilities are two bf16 parts each (hi + lo,
-// 16 bits of mantissa), two MMAs instead of one per fragment.
-constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS;
-constexpr int PD_MIN_TILES = PD_WARPS;      // fewest tiles of a CTA: one per warp
-template <typename TI> struct PdSmem {
-    static constexpr bool SPLIT = sizeof(TI) == 4;
-    static constexpr int STAGES = SPLIT ? 2 : 3;   // 128 / 192 KiB of tiles in flight per SM
-    uint8_t ring[PD_WARPS][STAGES][2 * GQA_TILE_BYTES];
-    float4 merge[PD_WARPS][8][32];          // a half of a warp's accumulators; also its cs / sn / vw scratch
-    __nv_bfloat16 q[SPLIT ? 2 : 1][GQA_GRP * GQA_HD];
-    TI gate[GQA_GRP * GQA_HD];
-    float w[2][GQA_HD];                     // q / k norm weights
-    float ml[PD_WARPS][GQA_GRP][2];
-    int pre[1024 + 4];                      // tiles (of one KV head) before each request
-    int part[PD_WARPS];
-    uint64_t full[PD_WARPS][STAGES];
+//
+// Short calls are bound by latency, instruction fetch a large part of it: what
+// runs once per unit is kept in rolled loops over heads.
+constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_STAGES = 3, PD_STAGE = 2 * GQA_TILE_BYTES;
+constexpr int PD_OROW = 132;                 // floats between heads of O: 8 banks apart for the writers' heads
+template <typename TI> struct PdEntry {      // layout of the q entry and of the gate entry in a stage
+    static constexpr bool F32 = sizeof(TI) == 4;
+    static constexpr int BYTES = GQA_HD * (int)sizeof(TI);    // a head's q (or gate), the new k, the new v
+    static constexpr int ROW = BYTES + 8 * (int)sizeof(TI);   // apart: no bank conflicts between a quad's and the next head's reads
+    static constexpr int KV = GQA_GRP * ROW;
+    // the roped dims times 1 + w, fp32, in rows of YROW: behind the raw rows, or in their place
+    static constexpr int Y = F32 ? 0 : (GQA_GRP + 2) * ROW, YROW = F32 ? ROW / 4 : 264;
+    static constexpr int O = GQA_GRP * ROW;                   // gate entry: half of O, fp32, behind the gate rows
+    static_assert((GQA_GRP + 2) * ROW <= PD_STAGE && Y + (GQA_GRP + 1) * YROW * 4 <= PD_STAGE && O + GQA_GRP * PD_OROW * 4 <= PD_STAGE && ROW % 16 == 0, "");
 };
+struct PdSmem {
+    uint8_t ring[PD_WARPS][PD_STAGES][PD_STAGE];
+    float w1[2][GQA_HD];                    // 1 + q / k norm weights
+    float cs[PD_WARPS][GQA_HD / 2], sn[PD_WARPS][GQA_HD / 2];
+    unsigned long long turn[GQA_HD / 2];
+    float2 ml[PD_WARPS][2][GQA_GRP];        // (max, sum) of a warp's continued / opened piece
+    int4 cont[PD_WARPS], open[PD_WARPS];    // (there: 1, and ends here: 2; request; KV head; parked / last CTA)
+    int pre[1024 + 4];                      // entries (of one KV head) before each request
+    int part[PD_WARPS];
+    uint64_t full[PD_WARPS][PD_STAGES];
+};
+static_assert(sizeof(PdSmem) + 1024 <= 232448, "decode shared memory exceeds the 227 KiB per-CTA limit");
 
-// The range of CTA c is tiles [c * per, (c + 1) * per) of `total`.
-__device__ __forceinline__ int pd_per(int total, int ctas)
+__device__ __forceinline__ void load4(const __nv_bfloat16 *p, float (&x)[4])
 {
-    const int per = (total + ctas - 1) / ctas;
-    return max(PD_MIN_TILES, (per + PD_WARPS - 1) / PD_WARPS * PD_WARPS);
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.x));
+    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.y));
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
+__device__ __forceinline__ void load4(const float *p, float (&x)[4])
+{
+    const float4 a = *reinterpret_cast<const float4 *>(p);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+}
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&x)[4])
+{
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+__device__ __forceinline__ void store4(float *p, const float (&x)[4])
+{
+    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+// (x, y) as PARTS bf16 pairs whose sum is (x, y) to 8 PARTS bits
+template <int PARTS>
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&out)[PARTS])
+{
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        out[i] = pack_bf16(x, y);
+        x -= __uint_as_float(out[i] << 16);
+        y -= __uint_as_float(out[i] & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ float2 pair_of(const __nv_bfloat16 *p)
+{
+    const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ float2 pair_of(const float *p) { return *reinterpret_cast<const float2 *>(p); }
 
 template <typename TI>
 __global__ void __launch_bounds__(PD_THREADS, 1)
 pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, GqaPagesArgs p,
                     PagesPart part, const __grid_constant__ RopeFreq f)
 {
-    using Smem = PdSmem<TI>;
-    constexpr int STAGES = Smem::STAGES, QP = Smem::SPLIT ? 2 : 1;
+    using E = PdEntry<TI>;
+    constexpr int PARTS = E::F32 ? 3 : 2;
     extern __shared__ uint8_t smem_raw[];
-    Smem &sm = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    PdSmem &sm = *reinterpret_cast<PdSmem *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
     const int KH = p.pv.KH, G = p.H / KH, page = p.pv.page;
     griddep_launch();                       // the join may be scheduled; it waits for this grid
     if (lane == 0) {
-        for (int s = 0; s < STAGES; ++s) mbar_init(&sm.full[warp][s], 1);
+        for (int s = 0; s < PD_STAGES; ++s) mbar_init(&sm.full[warp][s], 1);
         fence_mbar_init();
+        sm.cont[warp] = sm.open[warp] = make_int4(0, 0, 0, 0);
     }
     if (tid == 0) { tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
 
-    // tiles before each request
+    // entries before each request: its tiles, a q and a gate entry
     {
-        const int each = (p.n_req + PD_THREADS - 1) / PD_THREADS, r0 = tid * each;
-        int n[8], mine = 0;
-        for (int i = 0; i < each; ++i) {
+        const int each = (p.n_req + PD_THREADS - 1) / PD_THREADS, r0 = min(p.n_req, tid * each), r1 = min(p.n_req, r0 + each);
+        auto entries = [&](int r) {
             int row0, pos0;
-            n[i & 7] = r0 + i < p.n_req && pages_rows_of(p, r0 + i, row0, pos0) ? pos0 / GQA_TILE + 1 : 0;
-            mine += n[i & 7];
-        }
+            return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 3 : 0;
+        };
+        int mine = 0;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) mine += entries(r);
+        if (tid < p.rot / 2) sm.turn[tid] = f.turn[tid];
+        for (int j = tid; j < 2 * GQA_HD; j += PD_THREADS) sm.w1[0][j] = 1.f + p.qnw[j];   // knw follows qnw
         int inc = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -152,309 +203,431 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             if (lane >= d) inc += y;
         }
         if (lane == 31) sm.part[warp] = inc;
-        for (int i = tid; i < 2 * GQA_HD; i += PD_THREADS) sm.w[i / GQA_HD][i % GQA_HD] = i < GQA_HD ? p.qnw[i] : p.knw[i - GQA_HD];
-        for (int i = tid; i < QP * GQA_GRP * GQA_HD / 8; i += PD_THREADS)
-            reinterpret_cast<uint4 *>(sm.q)[i] = make_uint4(0, 0, 0, 0);   // heads past the group's stay zero
         __syncthreads();
         int at = inc - mine;
         for (int w = 0; w < warp; ++w) at += sm.part[w];
-        for (int i = 0; i < each; ++i) {
-            if (r0 + i <= p.n_req) sm.pre[r0 + i] = at;
-            at += n[i & 7];
-        }
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) { sm.pre[r] = at; at += entries(r); }
         if (tid == PD_THREADS - 1) sm.pre[p.n_req] = at;
         __syncthreads();
     }
-    const int total = sm.pre[p.n_req] * KH;
-    const int per = pd_per(total, gridDim.x);
-    const int c0 = min(total, cta * per), c1 = min(total, c0 + per);
-    // request of flat tile t: the last r with pre[r] * KH <= t
-    auto find = [&](int t) {
+    const int total = sm.pre[p.n_req] * KH, workers = gridDim.x * PD_WARPS;
+    const int per = max(1, (total + workers - 1) / workers);
+    const int v0 = min(total, (cta * PD_WARPS + warp) * per), v1 = min(total, v0 + per);
+    // request of entry v: the last r with pre[r] * KH <= v
+    auto find = [&](int v) {
         int lo = 0, hi = p.n_req - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (sm.pre[mid] * KH <= t) lo = mid; else hi = mid - 1;
+            if (sm.pre[mid] * KH <= v) lo = mid; else hi = mid - 1;
         }
         return lo;
     };
 
-    // ---- the warp's tiles: ordinal i is flat tile c0 + warp + 4 i
-    const int mine = max(0, (c1 - c0 - warp + PD_WARPS - 1) / PD_WARPS);
-    int ahead_id = 0, ahead_row = 0, at_group = 0;        // of ordinals (batch of 32) + lane
-    auto look_up = [&](int batch) {
-        const int i = batch * 32 + lane;
-        if (i >= mine) return;
-        const int t = c0 + warp + PD_WARPS * i, r = find(t), nt = sm.pre[r + 1] - sm.pre[r];
-        const int rel = t - sm.pre[r] * KH, kh = rel / nt, tok = (rel - kh * nt) * GQA_TILE, pi = tok / page;
-        ahead_id = p.pv.table[(size_t)r * p.pv.max_pages + pi];
-        ahead_row = kh * page + tok - pi * page;
-    };
-    auto take = [&]() {                                   // the batch looked up becomes the one in use
-        if ((unsigned)ahead_id >= (unsigned)p.pv.n_pages) { pages_error(PAGES_BAD_ID); ahead_id = 0; }
-        at_group = (int)(((long long)ahead_id * KH * page + ahead_row) >> 3);
-    };
-    auto issue = [&](int i) {                             // whole warp; i < mine
-        const int group = __shfl_sync(0xffffffffu, at_group, i & 31), s = i % STAGES;
-        if (lane == 0) {
-            uint8_t *kb = sm.ring[warp][s];
-            mbar_expect_tx(&sm.full[warp][s], 2 * GQA_TILE_BYTES);
-            tma_load_4d(kb, &tmK, 0, 0, 0, group, &sm.full[warp][s]);
-            tma_load_4d(kb + GQA_TILE_BYTES, &tmV, 0, 0, 0, group, &sm.full[warp][s]);
+    // ---- the ring: what the warp reads for entries v0 .. v1 - 1. A piece that
+    // starts inside a unit needs the q rows too (as entry v0 - 1), and a unit
+    // whose tiles are all here the gate rows, though its last entry is the
+    // next range's (as entry v1).
+    int ahead = -1, ahead_id = 0, ahead_row = 0, what = 0, base_v = v0 - 1, issued = 0;   // ahead: -1 none, 0 tile, 1 q, 2 gate
+    uint32_t todo = 0;
+    auto look_up = [&](int base) {
+        const int v = base + lane, at = min(max(v, v0), v1 - 1);
+        ahead = -1;
+        if (v > v1 || v0 >= v1) return;
+        const int r = find(at), n = sm.pre[r + 1] - sm.pre[r], rel0 = at - sm.pre[r] * KH;
+        int kh = (int)__fdividef((float)rel0, (float)n);        // at most KH <= 64: off by one at most
+        kh -= kh * n > rel0;
+        kh += (kh + 1) * n <= rel0;
+        const int rel = rel0 - kh * n, nt = n - 2;
+        const bool begins = at - rel + 1 >= v0;                 // the unit's first tile is in the range
+        if (v < v0) ahead = rel >= 1 && rel <= nt ? 1 : -1;
+        else if (v == v1) ahead = rel == nt && begins ? 2 : -1;
+        else if (rel == 0) ahead = v + 1 < v1 ? 1 : -1;
+        else if (rel <= nt) ahead = 0;
+        else ahead = begins ? 2 : -1;
+        ahead_row = r * KH + kh;
+        if (ahead == 0) {
+            const int pi = p.pv.tiles_div(rel - 1);
+            ahead_id = p.pv.table[(size_t)r * p.pv.max_pages + pi];
+            ahead_row = kh * page + (rel - 1) * GQA_TILE - pi * page;
         }
     };
-    look_up(0);
-    take();
-    look_up(1);
-    for (int i = 0; i < STAGES && i < mine; ++i) issue(i);
-
-    float *cs = reinterpret_cast<float *>(sm.merge[warp]), *sn = cs + GQA_HD / 2, *vw = sn + GQA_HD / 2;
-    const TI *qg = static_cast<const TI *>(p.qg);
-    Raw8<TI> rq[2], rg[2], rk, rv;                        // the next unit's two heads of this warp
-    auto load_heads = [&](int r, int kh) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int h = 2 * warp + u;
-            if (h < G) {
-                const TI *src = qg + ((size_t)r * p.H + kh * G + h) * 2 * GQA_HD + lane * 8;
-                rq[u].load(src);
-                rg[u].load(src + GQA_HD);
-            }
-        }
+    auto take = [&]() {                     // the batch looked up becomes the one in use
+        if (ahead == 0 && (unsigned)ahead_id >= (unsigned)p.pv.n_pages) { pages_error(PAGES_BAD_ID); ahead_id = 0; }
+        what = ahead == 0 ? (int)(((long long)ahead_id * KH * page + ahead_row) >> 3) : -1 - (2 * ahead_row + (ahead & 1));
+        todo = __ballot_sync(0xffffffffu, ahead >= 0);
     };
-
-    int t = c0, r = 0, kh = 0, i = 0, join_to = -1;
-    if (t < c1) {
-        r = find(t);
-        kh = (t - sm.pre[r] * KH) / (sm.pre[r + 1] - sm.pre[r]);
-        load_heads(r, kh);
-    }
-    const int r8 = lane & 7, mi = lane >> 3, h0 = (lane & 3) * 2, dr = lane >> 2;
-    while (t < c1) {
-        const int nt = sm.pre[r + 1] - sm.pre[r], u0 = sm.pre[r] * KH + kh * nt, u1 = u0 + nt, end = min(u1, c1);
-        const int pos = p.base[r], T = pos + 1;
-        // ---- q of the unit's heads, normed and roped, and the gate
-        pages_rope_table(cs, sn, pos, p.rot, f, lane, 32);
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int h = 2 * warp + u;
-            if (h < G) {
-                float x[8], w[8], y[8];
-                rq[u].unpack(x);
-                load8<float>(sm.w[0] + lane * 8, w);
-                gqa_norm_rope(y, x, w, p.eps, p.rot, cs, sn, vw, lane);
-                // q to bf16 (a rounding of 2^-9 of each element; fp32 inputs: hi and lo parts)
-                store8(sm.q[0] + h * GQA_HD + lane * 8, y);
-                if constexpr (Smem::SPLIT) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] -= __bfloat162float(__float2bfloat16_rn(y[e]));
-                    store8(sm.q[QP - 1] + h * GQA_HD + lane * 8, y);
-                }
-                rg[u].store(sm.gate + h * GQA_HD + lane * 8);
-            }
+    auto issue_next = [&]() {               // whole warp: the next entry into the next stage
+        while (todo == 0) {
+            if (base_v > v1 + 32) return;
+            take();
+            look_up(base_v);
+            base_v += 32;
         }
-        // the last tile's owner fetches the row to append
-        const bool append = u1 <= c1 && ((u1 - 1 - c0) & (PD_WARPS - 1)) == warp;
-        if (append) {
-            const size_t in = ((size_t)r * KH + kh) * GQA_HD + lane * 8;
-            rk.load(static_cast<const TI *>(p.k) + in);
-            rv.load(static_cast<const TI *>(p.v) + in);
-        }
-        __syncthreads();
-        // Q^T as the B operand: b0 = (dim = 16kk + 2(lane&3) + {0,1}, head = lane>>2), b1 = dim + 8
-        uint32_t qf[QP][16][2];
-#pragma unroll
-        for (int q = 0; q < QP; ++q)
-#pragma unroll
-            for (int kk = 0; kk < 16; ++kk) {
-                const __nv_bfloat16 *src = sm.q[q] + (lane >> 2) * GQA_HD + kk * 16 + (lane & 3) * 2;
-                qf[q][kk][0] = *reinterpret_cast<const uint32_t *>(src);
-                qf[q][kk][1] = *reinterpret_cast<const uint32_t *>(src + 8);
+        const int e = __shfl_sync(0xffffffffu, what, __ffs(todo) - 1), s = issued % PD_STAGES;
+        todo &= todo - 1;
+        ++issued;
+        uint8_t *to = sm.ring[warp][s];
+        uint64_t *bar = &sm.full[warp][s];
+        if (e >= 0) {
+            if (lane == 0) {
+                mbar_expect_tx(bar, PD_STAGE);
+                tma_load_4d(to, &tmK, 0, 0, 0, e, bar);
+                tma_load_4d(to + GQA_TILE_BYTES, &tmV, 0, 0, 0, e, bar);
             }
-        // the next unit's heads, in flight during this unit's tiles
-        int nr = r, nkh = kh + 1;
-        if (nkh == KH) {
-            nkh = 0;
-            for (++nr; nr < p.n_req && sm.pre[nr + 1] == sm.pre[nr];) ++nr;
-        }
-        if (end < c1) load_heads(nr, nkh);
-
-        float acc[16][4];
-#pragma unroll
-        for (int mt = 0; mt < 16; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-        const float sl2 = p.scale_log2;
-        for (; i < mine && c0 + warp + PD_WARPS * i < end; ++i) {
-            const int s = i % STAGES, tile = c0 + warp + PD_WARPS * i - u0, tok0 = tile * GQA_TILE;
-            mbar_wait(&sm.full[warp][s], (i / STAGES) & 1);   // a time-out raises the error word; the rest runs on what is there
-            uint8_t *kt = sm.ring[warp][s], *vt = kt + GQA_TILE_BYTES;
-            const uint32_t kb = smem_u32(kt), vb = kb + GQA_TILE_BYTES;
-            const int valid = min(GQA_TILE, T - tok0);
-            if (append && tile == nt - 1) {
-                // position pos: into the page and over the loaded tile (whose row is the page's old contents)
-                float x[8], w[8], y[8], v[8];
-                rk.unpack(x);
-                rv.unpack(v);
-                load8<float>(sm.w[1] + lane * 8, w);
-                gqa_norm_rope(y, x, w, p.eps, p.rot, cs, sn, vw, lane);
-                const int row = pos - tok0, off = (row >> 3) * 4096 + (lane >> 3) * 1024 + (row & 7) * 128 + (((lane & 7) ^ (row & 7)) << 4);
-                store8(reinterpret_cast<__nv_bfloat16 *>(kt + off), y);
-                store8(reinterpret_cast<__nv_bfloat16 *>(vt + off), v);
-                const long long at = pages_row(p.pv, r, kh, pos);
-                if (at >= 0) {
-                    store8(p.pv.k + at * GQA_HD + lane * 8, y);
-                    store8(p.pv.v + at * GQA_HD + lane * 8, v);
-                }
-            }
-            if (valid < GQA_TILE) {
-                // rows past the end are never weighted; cleared so that stale
-                // non-finite cache contents cannot come through as 0 * inf
-                for (int j = lane; j < (GQA_TILE - valid) * 32; j += 32) {
-                    const int row = valid + (j >> 5), c = (j & 31) >> 3, ch = j & 7;
-                    *reinterpret_cast<uint4 *>(vt + (row >> 3) * 4096 + c * 1024 + (row & 7) * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
-                }
-            }
+        } else {                            // rows of unit `u`, a bulk copy per lane
+            const int u = (-1 - e) >> 1, is_q = (-1 - e) & 1, r = p.pv.heads_div(u), n = is_q ? G + 2 : G;
+            if (lane == 0) mbar_expect_tx(bar, n * E::BYTES);
             __syncwarp();
-            // S^T[16 tok x 8 heads] = K[16 x 256] . Q^T[256 x 8]
-            float sc[4] = {0.f, 0.f, 0.f, 0.f};
-            {
-                const uint32_t base = kb + (mi & 1) * 4096 + r8 * 128;
+            const TI *from = static_cast<const TI *>(p.qg) + ((size_t)r * p.H + (u - r * KH) * G + lane) * 2 * GQA_HD + (is_q ? 0 : GQA_HD);
+            if (lane == G) from = static_cast<const TI *>(p.k) + (size_t)u * GQA_HD;
+            if (lane == G + 1) from = static_cast<const TI *>(p.v) + (size_t)u * GQA_HD;
+            if (lane < n) bulk_load(to + (lane < G ? lane * E::ROW : E::KV + (lane - G) * E::ROW), from, E::BYTES, bar);
+        }
+    };
+    // ---- entry by entry; each leaves its stage to the one PD_STAGES behind it
+    float *cs = sm.cs[warp], *sn = sm.sn[warp];
+    const int r8 = lane & 7, mi = lane >> 3, h0 = (lane & 3) * 2, dr = lane >> 2;
+    const float sl2 = p.scale_log2;
+    // the unit in work: request, KV head, position, tiles, the tiles of this piece
+    int r = 0, kh = 0, pos = -1, nt = 0, u0 = 0, tile = 0, end_tile = 0, next_v = v0, next_r = 0, next_kh = 0;
+    bool begins = false, ends = false;
+    uint32_t qf[PARTS][16][2];              // q as the B operand: head lane / 4, dims 16kk + 2 (lane % 4) + {0, 1, 8, 9}
+    uint4 new_k = make_uint4(0, 0, 0, 0);   // the row to append, bf16
+    uint4 new_vb = make_uint4(0, 0, 0, 0);
+    float acc[16][4], m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
+    if (v0 < v1) {
+        next_r = find(v0);
+        next_kh = (v0 - sm.pre[next_r] * KH) / (sm.pre[next_r + 1] - sm.pre[next_r]);
+    }
+    enum { AT_Q, AT_TILE, AT_GATE } at = AT_Q;
+#pragma unroll 1
+    for (int i = -PD_STAGES;; ++i) {
+        if (i >= 0) {
+            if (at == AT_Q) {
+                // ---- the next unit with tiles in the range
+                for (;;) {
+                    if (next_v >= v1) break;
+                    r = next_r; kh = next_kh;
+                    const int n = sm.pre[r + 1] - sm.pre[r];
+                    nt = n - 2;
+                    u0 = sm.pre[r] * KH + kh * n;
+                    tile = max(next_v - u0 - 1, 0);
+                    end_tile = min(v1 - u0 - 1, nt);
+                    next_v = min(v1, u0 + n);
+                    if (++next_kh == KH) {
+                        next_kh = 0;
+                        for (++next_r; next_r < p.n_req && sm.pre[next_r + 1] == sm.pre[next_r];) ++next_r;
+                    }
+                    if (tile < end_tile) break;
+                    tile = end_tile = 0;
+                }
+                if (tile >= end_tile) break;
+            }
+            const int s = i % PD_STAGES;
+            mbar_wait(&sm.full[warp][s], (i / PD_STAGES) & 1);   // a time-out raises the error word; the rest runs on what is there
+            uint8_t *st = sm.ring[warp][s];
+            if (at == AT_Q) {
+                begins = tile == 0;
+                ends = end_tile == nt;
+                if (pos != p.base[r]) {
+                    pos = p.base[r];
+                    pages_rope_table(cs, sn, pos, p.rot, sm.turn, lane, 32);
+                }
+                __syncwarp();
+                // rs: the norm's factor of a row, which the rotation commutes with; lanes 4h .. 4h + 3
+                // hold the quarters of head h's fragments, and all 32 lanes 8 dims each of the new k
+                const int h = lane >> 2, d0 = 2 * (lane & 3), half = p.rot >> 1;
+                const TI *x = reinterpret_cast<const TI *>(st + min(h, G - 1) * E::ROW);
+                const TI *xk = reinterpret_cast<const TI *>(st + E::KV);
+                float s0 = 0.f, s1 = 0.f, sk = 0.f, k[8], val[8];
 #pragma unroll
                 for (int kk = 0; kk < 16; ++kk) {
-                    const int chunk = (kk & 3) * 2 + (mi >> 1);
-                    uint32_t a0, a1, a2, a3;
-                    ldsm_x4(base + (kk >> 2) * 1024 + ((chunk ^ r8) << 4), a0, a1, a2, a3);
-#pragma unroll
-                    for (int q = 0; q < QP; ++q) mma_bf16_16816(sc, a0, a1, a2, a3, qf[q][kk][0], qf[q][kk][1]);
+                    const float2 a = pair_of(x + 16 * kk + d0), b = pair_of(x + 16 * kk + 8 + d0);
+                    s0 += a.x * a.x + a.y * a.y;
+                    s1 += b.x * b.x + b.y * b.y;
                 }
-            }
-            // online softmax per head (heads h0, h0 + 1), log2 domain
-            const int ta = lane >> 2, tb = ta + 8;
-            const float x0 = ta < valid ? sc[0] * sl2 : -INFINITY, x1 = ta < valid ? sc[1] * sl2 : -INFINITY;
-            const float x2 = tb < valid ? sc[2] * sl2 : -INFINITY, x3 = tb < valid ? sc[3] * sl2 : -INFINITY;
-            float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+                load8<TI>(xk + lane * 8, k);
+                load8<TI>(reinterpret_cast<const TI *>(st + E::KV + E::ROW) + lane * 8, val);
 #pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) {
-                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
-                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
-            }
-            const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-            const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-            const float p0 = exp2f(x0 - b0), p1 = exp2f(x1 - b1), p2 = exp2f(x2 - b0), p3 = exp2f(x3 - b1);
-            if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-                const float al0 = exp2f(m0 - b0), al1 = exp2f(m1 - b1);
-                l0 *= al0;
-                l1 *= al1;
+                for (int e = 0; e < 8; ++e) sk += k[e] * k[e];
+                s0 += s1;
 #pragma unroll
-                for (int mt = 0; mt < 16; ++mt) { acc[mt][0] *= al0; acc[mt][1] *= al1; acc[mt][2] *= al0; acc[mt][3] *= al1; }
-                m0 = n0;
-                m1 = n1;
-            }
-            l0 += p0 + p2;
-            l1 += p1 + p3;
-            uint32_t pb[QP][2];
-            pb[0][0] = pack_bf16(p0, p1);
-            pb[0][1] = pack_bf16(p2, p3);
-            if constexpr (Smem::SPLIT) {
-                auto lo = [](float x) { return x - __bfloat162float(__float2bfloat16_rn(x)); };
-                pb[QP - 1][0] = pack_bf16(lo(p0), lo(p1));
-                pb[QP - 1][1] = pack_bf16(lo(p2), lo(p3));
-            }
-#pragma unroll
-            for (int q = 0; q < QP; ++q) { pb[q][0] = movmatrix_t(pb[q][0]); pb[q][1] = movmatrix_t(pb[q][1]); }
-            // O^T[256 dims x 8 heads] += V^T[256 x 16 tok] . P^T[16 tok x 8 heads]
-            {
-                const uint32_t base = vb + (mi >> 1) * 4096 + r8 * 128;
-#pragma unroll
-                for (int mt = 0; mt < 16; ++mt) {
-                    const int chunk = (mt & 3) * 2 + (mi & 1);
-                    uint32_t a0, a1, a2, a3;
-                    ldsm_x4_t(base + (mt >> 2) * 1024 + ((chunk ^ r8) << 4), a0, a1, a2, a3);
-#pragma unroll
-                    for (int q = 0; q < QP; ++q) mma_bf16_16816(acc[mt], a0, a1, a2, a3, pb[q][0], pb[q][1]);
+                for (int o = 1; o < 32; o <<= 1) {
+                    if (o < 4) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+                    sk += __shfl_xor_sync(0xffffffffu, sk, o);
                 }
+                const float rs = h < G ? 1.f / sqrtf(s0 / GQA_HD + p.eps) : 0.f;    // heads past the group's: q = 0
+                const float rk = 1.f / sqrtf(sk / GQA_HD + p.eps);
+                __syncwarp();               // (fp32: the roped dims take the place of what has been read)
+                float *y = reinterpret_cast<float *>(st + E::Y);
+                for (int j = lane; j < half; j += 32) {
+                    const float c = cs[j], sv = sn[j];
+#pragma unroll 3
+                    for (int row = 0; row < GQA_GRP + 1; ++row) {               // the heads, then k
+                        const TI *in = reinterpret_cast<const TI *>(st + row * E::ROW);
+                        const float *w = sm.w1[row == GQA_GRP];
+                        const float a = to_f32(in[j]) * w[j], b = to_f32(in[j + half]) * w[j + half];
+                        y[row * E::YROW + j] = a * c - b * sv;
+                        y[row * E::YROW + j + half] = b * c + a * sv;
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int kk = 0; kk < 16; ++kk)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int d = 16 * kk + 8 * e + d0;
+                        float2 v;
+                        if (d < p.rot) {
+                            v = *reinterpret_cast<const float2 *>(y + h * E::YROW + d);
+                        } else {
+                            const float2 w = *reinterpret_cast<const float2 *>(&sm.w1[0][d]);
+                            v = pair_of(x + d);
+                            v.x *= w.x;
+                            v.y *= w.y;
+                        }
+                        uint32_t parts[PARTS];
+                        split_bf16<PARTS>(h < G ? v.x * rs : 0.f, h < G ? v.y * rs : 0.f, parts);
+#pragma unroll
+                        for (int q = 0; q < PARTS; ++q) qf[q][kk][e] = parts[q];
+                    }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = lane * 8 + e;
+                    k[e] = (d < p.rot ? y[GQA_GRP * E::YROW + d] : k[e] * sm.w1[1][d]) * rk;
+                }
+                new_k = make_uint4(pack_bf16(k[0], k[1]), pack_bf16(k[2], k[3]), pack_bf16(k[4], k[5]), pack_bf16(k[6], k[7]));
+                new_vb = make_uint4(pack_bf16(val[0], val[1]), pack_bf16(val[2], val[3]), pack_bf16(val[4], val[5]), pack_bf16(val[6], val[7]));
+#pragma unroll
+                for (int mt = 0; mt < 16; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
+                m0 = m1 = -INFINITY;
+                l0 = l1 = 0.f;
+                at = AT_TILE;
+            } else if (at == AT_TILE) {
+                uint8_t *vt = st + GQA_TILE_BYTES;
+                const uint32_t kb = smem_u32(st), vb = kb + GQA_TILE_BYTES;
+                const int tok0 = tile * GQA_TILE, valid = min(GQA_TILE, pos + 1 - tok0);
+                if (tile == nt - 1) {
+                    // position pos: into the page and over the loaded tile (whose row is the page's old contents)
+                    const int row = pos - tok0, off = (row >> 3) * 4096 + (lane >> 3) * 1024 + (row & 7) * 128 + (((lane & 7) ^ (row & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(st + off) = new_k;
+                    *reinterpret_cast<uint4 *>(vt + off) = new_vb;
+                    const long long to = pages_row(p.pv, r, kh, pos);
+                    if (to >= 0) {
+                        *reinterpret_cast<uint4 *>(p.pv.k + to * GQA_HD + lane * 8) = new_k;
+                        *reinterpret_cast<uint4 *>(p.pv.v + to * GQA_HD + lane * 8) = new_vb;
+                    }
+                    // rows past the end are never weighted; cleared so that stale
+                    // non-finite cache contents cannot come through as 0 * inf
+                    for (int j = lane; j < (GQA_TILE - valid) * 32; j += 32) {
+                        const int dead = valid + (j >> 5), c = (j & 31) >> 3, ch = j & 7;
+                        *reinterpret_cast<uint4 *>(vt + (dead >> 3) * 4096 + c * 1024 + (dead & 7) * 128 + ch * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    __syncwarp();
+                }
+                // S^T[16 tok x 8 heads] = K[16 x 256] . Q^T[256 x 8]
+                // in 2 PARTS independent sums, so that no MMA waits for the one before
+                float part_s[2][PARTS][4] = {};
+                {
+                    const uint32_t base = kb + (mi & 1) * 4096 + r8 * 128;
+#pragma unroll
+                    for (int kk = 0; kk < 16; ++kk) {
+                        const int chunk = (kk & 3) * 2 + (mi >> 1);
+                        uint32_t a0, a1, a2, a3;
+                        ldsm_x4(base + (kk >> 2) * 1024 + ((chunk ^ r8) << 4), a0, a1, a2, a3);
+#pragma unroll
+                        for (int q = 0; q < PARTS; ++q) mma_bf16_16816(part_s[kk & 1][q], a0, a1, a2, a3, qf[q][kk][0], qf[q][kk][1]);
+                    }
+                }
+                float sc[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[e] = 0.f;
+#pragma unroll
+                    for (int q = PARTS - 1; q >= 0; --q) sc[e] += part_s[0][q][e] + part_s[1][q][e];
+                }
+                // online softmax per head (heads h0, h0 + 1), log2 domain
+                const int ta = lane >> 2, tb = ta + 8;
+                const float x0 = ta < valid ? sc[0] * sl2 : -INFINITY, x1 = ta < valid ? sc[1] * sl2 : -INFINITY;
+                const float x2 = tb < valid ? sc[2] * sl2 : -INFINITY, x3 = tb < valid ? sc[3] * sl2 : -INFINITY;
+                float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+#pragma unroll
+                for (int o = 4; o <= 16; o <<= 1) {
+                    t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+                    t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+                }
+                const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+                const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
+                const float p0 = exp2f(x0 - b0), p1 = exp2f(x1 - b1), p2 = exp2f(x2 - b0), p3 = exp2f(x3 - b1);
+                if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+                    const float al0 = exp2f(m0 - b0), al1 = exp2f(m1 - b1);
+                    l0 *= al0;
+                    l1 *= al1;
+#pragma unroll
+                    for (int mt = 0; mt < 16; ++mt) { acc[mt][0] *= al0; acc[mt][1] *= al1; acc[mt][2] *= al0; acc[mt][3] *= al1; }
+                    m0 = n0;
+                    m1 = n1;
+                }
+                l0 += p0 + p2;
+                l1 += p1 + p3;
+                uint32_t pa[PARTS], pb[PARTS];
+                split_bf16<PARTS>(p0, p1, pa);
+                split_bf16<PARTS>(p2, p3, pb);
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) { pa[q] = movmatrix_t(pa[q]); pb[q] = movmatrix_t(pb[q]); }
+                // O^T[256 dims x 8 heads] += V^T[256 x 16 tok] . P^T[16 tok x 8 heads]
+                {
+                    const uint32_t base = vb + (mi >> 1) * 4096 + r8 * 128;
+#pragma unroll
+                    for (int mt = 0; mt < 16; ++mt) {
+                        const int chunk = (mt & 3) * 2 + (mi & 1);
+                        uint32_t a0, a1, a2, a3;
+                        ldsm_x4_t(base + (mt >> 2) * 1024 + ((chunk ^ r8) << 4), a0, a1, a2, a3);
+#pragma unroll
+                        for (int q = PARTS - 1; q >= 0; --q) mma_bf16_16816(acc[mt], a0, a1, a2, a3, pa[q], pb[q]);
+                    }
+                }
+                if (++tile == end_tile) {
+#pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1) {
+                        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+                        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+                    }
+                    at = AT_GATE;
+                    if (!(begins && ends)) {
+                        // ---- a piece: to the CTA's merge below, through shared memory if it is
+                        // the range's last (its loads have all landed), else parked in the workspace
+                        at = AT_Q;
+                        const int kind = begins ? 1 : 0;
+                        const bool last = next_v >= v1;
+                        if (lane == 0) {
+                            if (begins) sm.open[warp] = make_int4(1, r, kh, (u0 + nt) / per / PD_WARPS);
+                            else sm.cont[warp] = make_int4(ends ? 3 : 1, r, kh, last ? 0 : 1);
+                        }
+                        if (lane < 4) { sm.ml[warp][kind][h0] = make_float2(m0, l0); sm.ml[warp][kind][h0 + 1] = make_float2(m1, l1); }
+                        float4 *o = last ? reinterpret_cast<float4 *>(sm.ring[warp][0])
+                                         : part.park + (size_t)(cta * PD_WARPS + warp) * 512;
+                        if (last) __syncwarp();       // this stage may be the one: other lanes have read it
+#pragma unroll
+                        for (int mt = 0; mt < 16; ++mt) o[mt * 32 + lane] = make_float4(acc[mt][0], acc[mt][1], acc[mt][2], acc[mt][3]);
+                    }
+                }
+            } else {
+                // ---- the whole unit: ctx = O / l * sigmoid(gate), turned to rows behind the gate rows, half the dims at a time
+                const float i0 = 1.f / l0, i1 = 1.f / l1;
+                float *o_ = reinterpret_cast<float *>(st + E::O);
+                const uint8_t *gate = st + 4 * lane * sizeof(TI);
+                TI *out = static_cast<TI *>(p.ctx) + ((size_t)r * p.H + kh * G) * GQA_HD + 4 * lane;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int mt = 0; mt < 8; ++mt) {
+                        const float (&a)[4] = acc[half * 8 + mt];
+                        float *o = o_ + h0 * PD_OROW + mt * 16 + dr;
+                        o[0] = a[0] * i0; o[PD_OROW] = a[1] * i1; o[8] = a[2] * i0; o[PD_OROW + 8] = a[3] * i1;
+                    }
+                    __syncwarp();
+#pragma unroll 4
+                    for (int h = 0; h < GQA_GRP; ++h) {
+                        float o[4], g[4];
+                        load4(reinterpret_cast<const TI *>(gate + h * E::ROW) + half * 128, g);
+                        load4(o_ + h * PD_OROW + 4 * lane, o);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] *= sigmoidf_(g[e]);
+                        if (h < G) store4(out + (size_t)h * GQA_HD + half * 128, o);
+                    }
+                    __syncwarp();
+                }
+                at = AT_Q;
             }
             __syncwarp();
-            const int next = i + STAGES;
-            if (next < mine) {
-                if ((next & 31) == 0) { take(); look_up(next / 32 + 1); }
-                if (lane == 0) fence_proxy_async();
-                issue(next);
-            }
+            fence_proxy_async();
         }
-#pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-        }
-        // ---- merge the warps' parts, half of the accumulators at a time:
-        // warp w adds the 16-dim blocks 2w and 2w + 1 of each half
-        if (lane < 4) {
-            sm.ml[warp][h0][0] = m0; sm.ml[warp][h0][1] = l0;
-            sm.ml[warp][h0 + 1][0] = m1; sm.ml[warp][h0 + 1][1] = l1;
-        }
-        const bool first = t == u0, whole = first && end == u1;
-        const int slot = 2 * cta + (first ? 1 : 0);
-        float f0[PD_WARPS], f1[PD_WARPS], L0 = 0.f, L1 = 0.f, M0 = -INFINITY, M1 = -INFINITY;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
-                const float (&a)[4] = acc[half * 8 + mt];
-                sm.merge[warp][mt][lane] = make_float4(a[0], a[1], a[2], a[3]);
-            }
-            __syncthreads();
-            if (half == 0) {
-#pragma unroll
-                for (int w = 0; w < PD_WARPS; ++w) { M0 = fmaxf(M0, sm.ml[w][h0][0]); M1 = fmaxf(M1, sm.ml[w][h0 + 1][0]); }
-#pragma unroll
-                for (int w = 0; w < PD_WARPS; ++w) {
-                    const float a = sm.ml[w][h0][0], b = sm.ml[w][h0 + 1][0];
-                    f0[w] = a == -INFINITY ? 0.f : exp2f(a - M0);
-                    f1[w] = b == -INFINITY ? 0.f : exp2f(b - M1);
-                    L0 += sm.ml[w][h0][1] * f0[w];
-                    L1 += sm.ml[w][h0 + 1][1] * f1[w];
-                }
-                if (!whole && warp == 0 && lane < 4) {
-                    float2 *ml = part.ml + (size_t)slot * GQA_GRP + h0;
-                    ml[0] = make_float2(M0, L0);
-                    ml[1] = make_float2(M1, L1);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int w = 0; w < PD_WARPS; ++w) {
-                    const float4 a = sm.merge[w][2 * warp + u][lane];
-                    o.x += a.x * f0[w]; o.y += a.y * f1[w]; o.z += a.z * f0[w]; o.w += a.w * f1[w];
-                }
-                const int d = (half * 8 + 2 * warp + u) * 16 + dr;
-                if (whole) {
-                    TI *out = static_cast<TI *>(p.ctx) + ((size_t)r * p.H + kh * G + h0) * GQA_HD + d;
-                    const TI *g = sm.gate + h0 * GQA_HD + d;
-                    if (h0 < G) {
-                        out[0] = from_f32<TI>(o.x / L0 * sigmoidf_(to_f32(g[0])));
-                        out[8] = from_f32<TI>(o.z / L0 * sigmoidf_(to_f32(g[8])));
-                    }
-                    if (h0 + 1 < G) {
-                        out[GQA_HD] = from_f32<TI>(o.y / L1 * sigmoidf_(to_f32(g[GQA_HD])));
-                        out[GQA_HD + 8] = from_f32<TI>(o.w / L1 * sigmoidf_(to_f32(g[GQA_HD + 8])));
-                    }
-                } else {
-                    float *out = part.o + ((size_t)slot * GQA_GRP + h0) * GQA_HD + d;
-                    out[0] = o.x; out[8] = o.z;
-                    out[GQA_HD] = o.y; out[GQA_HD + 8] = o.w;
-                }
-            }
-            __syncthreads();                // the area, q and the gate are written again
-        }
-        if (first && !whole) join_to = (u1 - 1) / per;
-        t = end;
-        if (t < c1) { r = nr; kh = nkh; }
+        issue_next();
     }
-    // the unit that begins in this CTA and goes on: its pieces are this CTA's last and the firsts of cta + 1 .. join_to
-    if (tid == 0) part.units[cta] = make_int4(join_to, r, kh, 0);
+    // ---- the runs of pieces of one unit, added up by the whole CTA
+    __syncthreads();
+    int from = 0, n = 0;                    // the run: n pieces, warp `from`'s first
+    bool opened = false;                    // .. which was opened there
+    int4 unit = make_int4(-1, 0, 0, -1);
+#pragma unroll 1
+    for (int step = 0; step < 2 * PD_WARPS + 1; ++step) {
+        const int w = step >> 1;
+        bool whole = false;
+        if (step == 2 * PD_WARPS) {         // what goes on in the next CTA
+            if (n == 0) break;
+        } else if (step & 1) {
+            if (sm.open[w].x) { from = w; n = 1; opened = true; unit = sm.open[w]; }
+            continue;
+        } else {
+            const int4 c = sm.cont[w];
+            if (!c.x) continue;
+            if (n++ == 0) from = w;
+            if (!(c.x & 2)) continue;
+            whole = opened;
+        }
+        // pieces: warps from .. from + n - 1, none of those between empty
+        float f0[PD_WARPS], f1[PD_WARPS], M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < PD_WARPS; ++j) {
+            if (j >= n) continue;
+            M0 = fmaxf(M0, sm.ml[from + j][opened && j == 0][h0].x);
+            M1 = fmaxf(M1, sm.ml[from + j][opened && j == 0][h0 + 1].x);
+        }
+#pragma unroll
+        for (int j = 0; j < PD_WARPS; ++j) {
+            f0[j] = f1[j] = 0.f;
+            if (j >= n) continue;
+            const float2 a = sm.ml[from + j][opened && j == 0][h0], b = sm.ml[from + j][opened && j == 0][h0 + 1];
+            f0[j] = a.x == -INFINITY ? 0.f : exp2f(a.x - M0);
+            f1[j] = b.x == -INFINITY ? 0.f : exp2f(b.x - M1);
+            L0 += a.y * f0[j];
+            L1 += b.y * f1[j];
+        }
+        const int slot = 2 * cta + (opened ? 1 : 0);
+        const float i0 = 1.f / L0, i1 = 1.f / L1;
+        if (!whole && warp == 0 && lane < 4) {
+            float2 *ml = part.ml + (size_t)slot * GQA_GRP + h0;
+            ml[0] = make_float2(M0, L0);
+            ml[1] = make_float2(M1, L1);
+        }
+#pragma unroll
+        for (int u = 0; u < 16 / PD_WARPS; ++u) {
+            const int mt = warp + PD_WARPS * u, d = mt * 16 + dr;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < PD_WARPS; ++j) {
+                if (j >= n) continue;
+                const bool parked = !(opened && j == 0) && sm.cont[from + j].w;
+                const float4 a = parked ? part.park[(size_t)(cta * PD_WARPS + from + j) * 512 + mt * 32 + lane]
+                                        : reinterpret_cast<const float4 *>(sm.ring[from + j][0])[mt * 32 + lane];
+                o.x += a.x * f0[j]; o.y += a.y * f1[j]; o.z += a.z * f0[j]; o.w += a.w * f1[j];
+            }
+            if (whole) {
+                const size_t row = (size_t)unit.y * p.H + unit.z * G + h0;
+                TI *out = static_cast<TI *>(p.ctx) + row * GQA_HD + d;
+                const TI *g = static_cast<const TI *>(p.qg) + row * 2 * GQA_HD + GQA_HD + d;
+                if (h0 < G) {
+                    out[0] = from_f32<TI>(o.x * i0 * sigmoidf_(to_f32(g[0])));
+                    out[8] = from_f32<TI>(o.z * i0 * sigmoidf_(to_f32(g[8])));
+                }
+                if (h0 + 1 < G) {
+                    out[GQA_HD] = from_f32<TI>(o.y * i1 * sigmoidf_(to_f32(g[2 * GQA_HD])));
+                    out[GQA_HD + 8] = from_f32<TI>(o.w * i1 * sigmoidf_(to_f32(g[2 * GQA_HD + 8])));
+                }
+            } else {
+                float *out = part.o + ((size_t)slot * GQA_GRP + h0) * GQA_HD + d;
+                out[0] = o.x; out[8] = o.z;
+                out[GQA_HD] = o.y; out[GQA_HD + 8] = o.w;
+            }
+        }
+        if (step == 2 * PD_WARPS) break;
+        n = 0;
+        opened = false;
+    }
+    // a unit that begins in this CTA and goes on: its pieces are this CTA's last and the firsts of cta + 1 .. unit.w
+    if (tid == 0) part.units[cta] = make_int4(n > 0 && opened ? unit.w : -1, unit.y, unit.z, 0);
 }
 
 // One CTA per (first CTA of a split unit, query head): merges the unit's
@@ -522,8 +695,7 @@ template <typename TI>
 static cudaError_t pages_decode_run(const CUtensorMap &tk, const CUtensorMap &tv, const GqaPagesArgs &a, const PagesPart &part,
                                     const RopeFreq &f, int ctas, cudaStream_t st)
 {
-    const int smem = (int)sizeof(PdSmem<TI>) + 1024;
-    static_assert(sizeof(PdSmem<TI>) + 1024 <= 232448, "decode shared memory exceeds the 227 KiB per-CTA limit");
+    const int smem = (int)sizeof(PdSmem) + 1024;
     cudaError_t e = cudaFuncSetAttribute(pages_decode_kernel<TI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     pages_decode_kernel<TI><<<ctas, PD_THREADS, smem, st>>>(tk, tv, a, part, f);
@@ -562,7 +734,7 @@ pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
     const int n = pages_rows_of(p, r, row0, pos0);
     if (n == 0) return;
     const int pos = pos0 + row - row0;
-    pages_rope_table(cs[warp], sn[warp], pos, p.rot, f, lane, 32);
+    pages_rope_table(cs[warp], sn[warp], pos, p.rot, f.turn, lane, 32);
     __syncwarp();
     for (int kh = warp; kh < p.pv.KH; kh += 4) {
         const long long at = pages_row(p.pv, r, kh, pos);
@@ -594,7 +766,7 @@ pages_attend_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
     const int n = pages_rows_of(p, r, row0, pos0);
     if (n == 0) return;
     const int pos = pos0 + row - row0, kh = h / (p.H / p.pv.KH);
-    pages_rope_table(cs[warp], sn[warp], pos, p.rot, f, lane, 32);
+    pages_rope_table(cs[warp], sn[warp], pos, p.rot, f.turn, lane, 32);
     __syncwarp();
     const TI *qg = static_cast<const TI *>(p.qg) + ((size_t)row * p.H + h) * 2 * GQA_HD + lane * 8;
     float x[8], w[8], q[8], g[8], o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};

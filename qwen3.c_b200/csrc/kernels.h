@@ -171,10 +171,25 @@ cudaError_t launch_rmsnorm_zc_rows(const float *x, const float *delta, const flo
 
 namespace coli {
 // ---------------------------------------------------------------- paged KV cache
-// Rotary frequencies theta^(-2 j / rot) in double: a float32 product
-// pos * frequency is off by 2^-24 of the angle, 2e-3 rad at position 32768.
+// Rotary frequencies theta^(-2 j / rot) in turns per position, the fraction in
+// units of 2^-64: a float32 product pos * frequency is off by 2^-24 of the
+// angle, 2e-3 rad at position 32768.
 struct RopeFreq {
-    double f[128];
+    unsigned long long turn[128];
+};
+// x / d for 0 <= x < 2^31 by a multiplication: with 2^shift >= d > 2^(shift - 1),
+// floor(2^32 (2^shift - d) / d) + 1 and one shift are exact.
+struct FastDiv {
+    unsigned mul, shift;
+    static FastDiv of(unsigned d)
+    {
+        unsigned s = 0;
+        while ((1ull << s) < d) ++s;
+        return {(unsigned)((((1ull << s) - d) << 32) / d + 1), s};
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int operator()(int x) const { return (int)((__umulhi(mul, (unsigned)x) + (unsigned)x) >> shift); }
+#endif
 };
 // One layer's pages as the kernels see them: K and V rows of 256 bf16 at
 // ((page id * KH + head) * page + offset).
@@ -182,6 +197,8 @@ struct PageView {
     __nv_bfloat16 *k, *v;
     const int *table;     // [requests][max_pages] page ids
     int n_pages, page, KH, max_pages;
+    FastDiv tiles_div;    // by the 16-token tiles of a page
+    FastDiv heads_div;    // by KH
 };
 // Rows of one call: request r's query rows are cu[r] .. cu[r + 1] - 1 at
 // positions base[r] ..; decode (cu == nullptr) has one row per request, row r
@@ -200,6 +217,7 @@ struct GqaPagesArgs {
 struct PagesPart {
     float *o;             // [2 ctas][rows of a unit][hd]
     float2 *ml;           // [2 ctas][rows of a unit] (max, sum), log2 domain
+    float4 *park;         // [4 ctas][512] a warp's piece, in its own layout, until its range is done
     int4 *units;          // [ctas] unit that begins in CTA c and goes on: (last CTA or -1, request, KV head, ..)
 };
 cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, const GqaPagesArgs &a, const PagesPart &part,

@@ -36,7 +36,7 @@ size_t pages_norm_bytes(int layers) { return (size_t)layers * 2 * GQA_HD * 4; }
 size_t pages_list_bytes(int n_pages) { return ((size_t)n_pages * 4 + 255) & ~size_t(255); }
 // the workspace serves one call at a time: a compaction's lists, or an attention call's pieces
 size_t pages_part_rows() { return (size_t)2 * G.num_sms * GQA_GRP; }
-size_t pages_part_bytes() { return pages_part_rows() * (GQA_HD * 4 + 8) + (size_t)G.num_sms * 16; }
+size_t pages_part_bytes() { return pages_part_rows() * (GQA_HD * 4 + 8) + (size_t)G.num_sms * (4 * 512 + 1) * 16; }
 size_t pages_ws_bytes(int n_pages)
 {
     return (std::max(3 * pages_list_bytes(n_pages) + 256, pages_part_bytes()) + 255) & ~size_t(255);
@@ -46,7 +46,8 @@ PagesPart pages_part(uint8_t *ws)
     PagesPart t{};
     t.o = (float *)ws;
     t.ml = (float2 *)(ws + pages_part_rows() * GQA_HD * 4);
-    t.units = (int4 *)(t.ml + pages_part_rows());
+    t.park = (float4 *)(t.ml + pages_part_rows());
+    t.units = (int4 *)(t.park + (size_t)G.num_sms * 4 * 512);
     return t;
 }
 
@@ -149,7 +150,10 @@ int pages_attend_args(GqaPagesArgs &a, ColiCudaPages *p, int layer, const void *
     if (((uintptr_t)qg | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ctx) & 15)
         return fail("pages: qg, k, v and ctx must be 16-byte aligned");
     if (p->rot != rot || p->theta != theta) {
-        for (int j = 0; j < rot / 2; ++j) p->freq.f[j] = std::pow((double)theta, -2.0 * j / rot);
+        for (int j = 0; j < rot / 2; ++j) {
+            const double t = std::pow((double)theta, -2.0 * j / rot) / 6.283185307179586476925286766559;
+            p->freq.turn[j] = (unsigned long long)((t - std::floor(t)) * 18446744073709551616.0);
+        }
         p->rot = rot;
         p->theta = theta;
     }
@@ -157,6 +161,7 @@ int pages_attend_args(GqaPagesArgs &a, ColiCudaPages *p, int layer, const void *
     a.pv.k = (__nv_bfloat16 *)(p->base + 2 * layer * plane);
     a.pv.v = (__nv_bfloat16 *)(p->base + (2 * layer + 1) * plane);
     a.pv.table = table; a.pv.n_pages = p->n_pages; a.pv.page = p->page; a.pv.KH = KH; a.pv.max_pages = max_pages;
+    a.pv.tiles_div = FastDiv::of(p->page / GQA_TILE); a.pv.heads_div = FastDiv::of(KH);
     a.qg = qg; a.k = k; a.v = v; a.ctx = ctx; a.base = base;
     a.qnw = p->norm_w + (size_t)layer * 2 * GQA_HD; a.knw = a.qnw + GQA_HD;
     a.H = H; a.rot = rot; a.eps = eps;
