@@ -11,6 +11,7 @@
 // bad one raises g_pages_error, is left out, and touches no memory.
 #include "common.cuh"
 #include "kernels.h"
+#include "tc05.cuh"
 
 namespace coli {
 
@@ -58,16 +59,6 @@ __device__ __forceinline__ int pages_rows_of(const GqaPagesArgs &p, int r, int &
     }
     if ((long long)pos0 + n > (long long)p.pv.max_pages * p.pv.page) { pages_error(PAGES_BAD_POS); return 0; }
     return n;
-}
-
-// Request of a row (the last r with cu[r] <= row < cu[r + 1]), -1 for a row
-// behind the last sequence.
-__device__ __forceinline__ int pages_req_of(const GqaPagesArgs &p, int row)
-{
-    if (!p.cu) return row;
-    for (int r = 0; r < p.n_req; ++r)
-        if (row >= p.cu[r] && row < p.cu[r + 1]) return r;
-    return -1;
 }
 
 // ------------------------------------------------------------------ decode
@@ -716,100 +707,666 @@ cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, co
                    : pages_decode_run<float>(tk, tv, a, part, f, ctas, st);
 }
 
-// ------------------------------------------------------------------ append
-// A warp per (row, KV head), lane = 8 dims: k normed and roped, v as it is,
-// both rounded to bf16, the cache's type.
-template <typename TI>
-__global__ void __launch_bounds__(128)
-pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
+// ------------------------------------------------------------------ prefill
+// A unit is 128 query rows of one request and KV head: 128 / group tokens x
+// the group's heads, so all heads of the group share each K / V tile and a
+// tile of rows spans few positions (little of it is masked). Its work is its
+// 128-key tiles plus PP_SETUP. The units of all requests, end to end, are cut into
+// equal ranges, one per CTA (one CTA per SM): no tail wave, and few rows on a
+// long context are spread over the GPU. A piece of a unit leaves its O, max and sum in the
+// workspace, and pages_prefill_join_kernel merges them (two at most per CTA).
+//
+//   pages_plan_kernel     block 0 lays the ranges out; the others norm, rope and
+//                         append k (and v), a warp per (row, KV head)
+//   pages_prefill_kernel  tcgen05, 352 threads:
+//     warp 0      K tiles into a 2-stage ring, up to 8 TMA boxes of whole pages
+//                 each (a lane per box, its page id looked up there), and the gate
+//                 tile into the stage that the piece's last K tile leaves
+//     warp 1      V tiles, one buffer (which first stages Q)
+//     warp 2      MMA issuer, TMEM owner: S = Q K^T (M = N = 128, A = Q from
+//                 TMEM), O += P V (N = 256); S(j + 1) is issued before PV(j)
+//     warps 3..10 q norm + RoPE and Q into TMEM; softmax, 16 rows per warp
+//                 through the 16x256b TMEM shape, log2 domain, O corrected only
+//                 where the running maximum grew by more than 2^8; epilogue
+//   A page is a run of whole row groups, so one box of its rows lands as
+//   [8-row group][64-column block][8 rows][128 B]: groups 4 KiB apart, column blocks
+//   1 KiB, for K (K-major) and V (MN-major) alike, whatever the page size.
+//   Keys behind the request's end: K scores are masked, V rows read as zeros
+//   (boxes outside the pool; the last few rows of a group cleared in shared memory),
+//   so non-finite stale rows cannot come through as 0 * inf.
+// TMEM (512 columns): scores 128 | O 256 | Q 128 (bf16 pairs). Q and P are
+// rounded to bf16 (2^-9 of each element): a second part of either would double
+// its MMAs, and the tensor pipe is the bound here.
+constexpr int PP_BM = 128, PP_BN = 128;
+constexpr int PP_TILE = PP_BN * GQA_HD * 2, PP_P = PP_BM * PP_BN * 2;
+constexpr int PP_SOFTMAX = 256, PP_THREADS = 96 + PP_SOFTMAX;
+constexpr int PP_SETUP = 4;                 // a unit's start and end in tiles' time
+constexpr int PP_MIN = PP_SETUP + 2;        // least work of a CTA
+struct PpBars {
+    uint64_t q_tmem, k_full[2], k_empty[2], v_full, v_empty, s_full, s_free, p_full, pv_done, g_full, epi_done;
+    uint32_t tmem_base;
+    float lsum[PP_BM];
+};
+constexpr int PP_SMEM = 3 * PP_TILE + PP_P + (int)sizeof(PpBars);
+static_assert(PP_SMEM <= 232448, "prefill shared memory exceeds the 227 KiB per-CTA limit");
+
+// k / q row in registers, lane = 8 dims: norm and partial RoPE, sums in fp32.
+// vw: 256 floats of this warp, for rotation widths whose half is no multiple of 8.
+__device__ __forceinline__ void pages_norm_rope(float (&y)[8], const float (&x)[8], const float *w, float eps, int rot,
+                                                const float *cs, const float *sn, float *vw, int lane)
 {
-    __shared__ __align__(16) float cs[4][GQA_HD / 2], sn[4][GQA_HD / 2];
-    __shared__ float vec[4][GQA_HD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int row0, pos0;
-    if (blockIdx.x == 0)                     // what no row belongs to is looked over here
-        for (int i = threadIdx.x; i < p.n_req; i += 128) pages_rows_of(p, i, row0, pos0);
-    const int row = blockIdx.x, r = pages_req_of(p, row);
-    if (r < 0) return;
-    const int n = pages_rows_of(p, r, row0, pos0);
-    if (n == 0) return;
-    const int pos = pos0 + row - row0;
-    pages_rope_table(cs[warp], sn[warp], pos, p.rot, f.turn, lane, 32);
-    __syncwarp();
-    for (int kh = warp; kh < p.pv.KH; kh += 4) {
-        const long long at = pages_row(p.pv, r, kh, pos);
-        if (at < 0) continue;
-        const size_t in = ((size_t)row * p.pv.KH + kh) * GQA_HD + lane * 8;
-        float x[8], w[8], y[8], v[8];
-        load8<TI>(static_cast<const TI *>(p.k) + in, x);
-        load8<TI>(static_cast<const TI *>(p.v) + in, v);
-        load8<float>(p.knw + lane * 8, w);
-        gqa_norm_rope(y, x, w, p.eps, p.rot, cs[warp], sn[warp], vec[warp], lane);
-        store8(p.pv.k + at * GQA_HD + lane * 8, y);
-        store8(p.pv.v + at * GQA_HD + lane * 8, v);
+    float s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s2 = fmaf(x[i], x[i], s2);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+    const float rs = 1.f / sqrtf(s2 / GQA_HD + eps);
+    float wv[8];
+    load8<float>(w + lane * 8, wv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i] * rs * (1.f + wv[i]);
+    const int half = rot >> 1, d0 = lane * 8;
+    if ((half & 7) == 0) {                  // the partner dims are one other lane's
+        const int hl = half >> 3, src = lane < hl ? lane + hl : lane - hl, j = d0 < half ? d0 : d0 - half;
+        float z[8], c[8], sv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = __shfl_sync(0xffffffffu, y[i], src);
+        if (d0 < rot) {
+            load8<float>(cs + j, c);
+            load8<float>(sn + j, sv);
+            const float sign = d0 < half ? -1.f : 1.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = y[i] * c[i] + sign * z[i] * sv[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vw[d0 + i] = y[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = d0 + i;
+            if (d < rot) {
+                const int j = d < half ? d : d - half;
+                y[i] = d < half ? y[i] * cs[j] - vw[d + half] * sn[j] : y[i] * cs[j] + vw[j] * sn[j];
+            }
+        }
+        __syncwarp();
     }
 }
 
-// ------------------------------------------------------------------ attention
-// A warp per (row, query head), lane = 8 dims, one key at a time with a
-// running maximum and sum; fp32 throughout.
-template <typename TI>
-__global__ void __launch_bounds__(128)
-pages_attend_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
+// Tiles of query tile qt of a chunk of n rows at position b.
+__device__ __forceinline__ int pp_tiles(int n, int b, int qt, int tokens)
 {
-    __shared__ __align__(16) float cs[4][GQA_HD / 2], sn[4][GQA_HD / 2];
-    __shared__ float vec[4][GQA_HD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x, h = blockIdx.y * 4 + warp, r = pages_req_of(p, row);
-    if (r < 0 || h >= p.H) return;
-    int row0, pos0;
-    const int n = pages_rows_of(p, r, row0, pos0);
-    if (n == 0) return;
-    const int pos = pos0 + row - row0, kh = h / (p.H / p.pv.KH);
-    pages_rope_table(cs[warp], sn[warp], pos, p.rot, f.turn, lane, 32);
+    return (b + min(n, (qt + 1) * tokens) - 1) / PP_BN + 1;
+}
+// Work of its query tiles before qt (all of them whole): sum over j < qt of
+// floor((a + j) / group) + 1 + PP_SETUP with a = floor((b - 1 + tokens) / tokens).
+__device__ __forceinline__ long long pp_work(int b, int qt, int tokens, int group)
+{
+    const long long a = (b - 1 + tokens) / tokens, e = a + qt;
+    const long long ka = a / group, ke = e / group;
+    const long long pa = group * ka * (ka - 1) / 2 + ka * (a - ka * group), pe = group * ke * (ke - 1) / 2 + ke * (e - ke * group);
+    return pe - pa + (long long)qt * (1 + PP_SETUP);
+}
+
+constexpr int PL_THREADS = 256;
+template <int NT> __device__ __forceinline__ long long scan64(long long x, long long &total)   // exclusive, over the CTA
+{
+    __shared__ long long part[NT / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long inc = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += y;
+    }
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    long long before = 0, all = 0;
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) before += part[w];
+        all += part[w];
+    }
+    total = all;
+    return before + inc - x;
+}
+
+__global__ void __launch_bounds__(PL_THREADS)
+pages_plan_kernel(GqaPagesArgs p, PagesPart part, int ctas, const __grid_constant__ RopeFreq f)
+{
+    __shared__ union {
+        struct { float cs[PL_THREADS / 32][GQA_HD / 2], sn[PL_THREADS / 32][GQA_HD / 2], vw[PL_THREADS / 32][GQA_HD]; } a;
+        long long pre[1024 + 1];
+    } sm;
+    griddep_launch();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, KH = p.pv.KH, group = p.H / KH, tokens = PP_BM / group;
+    if (blockIdx.x == 0) {
+        auto work = [&](int r) {            // of one KV head
+            int row0, b;
+            const int n = pages_rows_of(p, r, row0, b);
+            if (n == 0) return 0ll;
+            const int last = (n - 1) / tokens;
+            return pp_work(b, last, tokens, group) + pp_tiles(n, b, last, tokens) + PP_SETUP;
+        };
+        const int each = (p.n_req + PL_THREADS - 1) / PL_THREADS, r0 = min(p.n_req, tid * each), r1 = min(p.n_req, r0 + each);
+        long long mine = 0, total;
+        for (int r = r0; r < r1; ++r) mine += work(r);
+        long long at = scan64<PL_THREADS>(mine, total);
+        for (int r = r0; r < r1; ++r) { sm.pre[r] = at; at += work(r); }
+        if (tid == 0) sm.pre[p.n_req] = total;
+        __syncthreads();
+        const long long all = total * KH, per = max((long long)PP_MIN, (all + ctas - 1) / ctas);
+        for (int c = tid; c <= ctas; c += PL_THREADS) {
+            const long long v = c * per;
+            int4 u = make_int4(p.n_req, 0, 0, 0);               // (request, KV head, query tile, key tile)
+            if (v < all) {
+                int lo = 0, hi = p.n_req - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (sm.pre[mid] * KH <= v) lo = mid; else hi = mid - 1;
+                }
+                const long long head = sm.pre[lo + 1] - sm.pre[lo];
+                long long rel = v - sm.pre[lo] * KH;
+                u.x = lo;
+                u.y = (int)(rel / head);
+                rel -= u.y * head;
+                int row0, b, q0 = 0;
+                const int n = pages_rows_of(p, lo, row0, b);
+                int q1 = (n - 1) / tokens;
+                while (q0 < q1) {           // the last query tile that starts at or before rel
+                    const int mid = (q0 + q1 + 1) >> 1;
+                    if (pp_work(b, mid, tokens, group) <= rel) q0 = mid; else q1 = mid - 1;
+                }
+                u.z = q0;
+                u.w = max(0, (int)(rel - pp_work(b, q0, tokens, group)) - PP_SETUP);
+            }
+            part.plan[c] = u;
+        }
+        return;
+    }
+    const int item = (blockIdx.x - 1) * (PL_THREADS / 32) + warp, row = item / KH, kh = item - row * KH;
+    if (row >= p.S) return;
+    int lo = 0, hi = p.n_req - 1, row0, b;
+    while (lo < hi) {                       // the last request that starts at or before the row
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.cu[mid] <= row) lo = mid; else hi = mid - 1;
+    }
+    if (row < p.cu[lo] || row >= p.cu[lo + 1] || pages_rows_of(p, lo, row0, b) == 0) return;
+    const int pos = b + row - row0;
+    const size_t in = (size_t)item * GQA_HD + lane * 8;
+    float x[8], y[8], v[8];
+    load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.k) + in, x);
+    load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.v) + in, v);
+    const long long at = pages_row(p.pv, lo, kh, pos);
+    pages_rope_table(sm.a.cs[warp], sm.a.sn[warp], pos, p.rot, f.turn, lane, 32);
     __syncwarp();
-    const TI *qg = static_cast<const TI *>(p.qg) + ((size_t)row * p.H + h) * 2 * GQA_HD + lane * 8;
-    float x[8], w[8], q[8], g[8], o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    load8<TI>(qg, x);
-    load8<TI>(qg + GQA_HD, g);
-    load8<float>(p.qnw + lane * 8, w);
-    gqa_norm_rope(q, x, w, p.eps, p.rot, cs[warp], sn[warp], vec[warp], lane);
+    pages_norm_rope(y, x, p.knw, p.eps, p.rot, sm.a.cs[warp], sm.a.sn[warp], sm.a.vw[warp], lane);
+    if (at < 0) return;
+    store8(p.pv.k + at * GQA_HD + lane * 8, y);
+    store8(p.pv.v + at * GQA_HD + lane * 8, v);
+}
+
+// A CTA's pieces, one after the other.
+struct PpWalk {
+    int4 at, stop;
+    int n, row0, base, nt, t1;              // of the piece in work: rows, first row, first position, tiles, end tile
+    bool ends;
+    __device__ __forceinline__ PpWalk(const GqaPagesArgs &p, const PagesPart &part, int cta)
+    {
+        at = part.plan[cta];
+        stop = part.plan[cta + 1];
+        n = at.x < p.n_req ? pages_rows_of(p, at.x, row0, base) : 0;
+    }
+    __device__ __forceinline__ bool piece(int tokens)
+    {
+        const bool last = at.x == stop.x && at.y == stop.y && at.z == stop.z;
+        if (n == 0 || (last && at.w >= stop.w)) return false;
+        nt = pp_tiles(n, base, at.z, tokens);
+        t1 = last ? stop.w : nt;
+        ends = t1 == nt;
+        return true;
+    }
+    __device__ __forceinline__ void next(const GqaPagesArgs &p, int tokens)
+    {
+        if (!ends) { n = 0; return; }       // the rest is the next CTA's
+        at.w = 0;
+        if (++at.z * tokens < n) return;
+        at.z = 0;
+        if (++at.y < p.pv.KH) return;
+        at.y = 0;
+        n = 0;
+        while (n == 0 && ++at.x < p.n_req && at.x <= stop.x) n = pages_rows_of(p, at.x, row0, base);
+    }
+};
+
+// K-major 128B-swizzled operand whose 8-row groups are 4 KiB apart.
+__device__ __forceinline__ uint64_t pp_desc_k(uint32_t addr)
+{
+    return (tc::desc_k_sw128(addr) & ~((uint64_t)0x3FFF << 32)) | (uint64_t)(4096 >> 4) << 32;
+}
+
+__global__ void __launch_bounds__(PP_THREADS, 1)
+pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const __grid_constant__ CUtensorMap tmV8, const __grid_constant__ CUtensorMap tmG, GqaPagesArgs p,
+                     PagesPart part, const __grid_constant__ RopeFreq f)
+{
+    // all shared memory is dynamic, so the window starts 1024-byte aligned as
+    // the swizzled boxes and descriptors need (checked: the budget leaves no padding)
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *sK = smem_raw, *sV = sK + 2 * PP_TILE, *sP = sV + PP_TILE;
+    PpBars &bars = *reinterpret_cast<PpBars *>(sP + PP_P);
+    if (smem_u32(smem_raw) & 1023) {        // uniform across the CTA: nothing has started yet
+        if (threadIdx.x == 0) raise_error(2);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+    const int KH = p.pv.KH, group = p.H / KH, gs = __ffs(group) - 1, tokens = PP_BM / group;
+    griddep_launch();
+    if (threadIdx.x == 0) {
+        mbar_init(&bars.q_tmem, PP_SOFTMAX);
+        for (int i = 0; i < 2; ++i) { mbar_init(&bars.k_full[i], 1); mbar_init(&bars.k_empty[i], 1); }
+        mbar_init(&bars.v_full, 1); mbar_init(&bars.v_empty, 1);
+        mbar_init(&bars.s_full, 1); mbar_init(&bars.s_free, PP_SOFTMAX);
+        mbar_init(&bars.p_full, PP_SOFTMAX); mbar_init(&bars.pv_done, 1);
+        mbar_init(&bars.g_full, 1); mbar_init(&bars.epi_done, PP_SOFTMAX);
+        fence_mbar_init();
+    }
+    if (warp == 2) tc::alloc(&bars.tmem_base, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tbase = bars.tmem_base;
+    const uint32_t tS = tbase, tO = tbase + 128, tQ = tbase + 384;
+    griddep_wait();                         // the plan and the appended rows
+    PpWalk w(p, part, cta);
+    int jj = 0;                             // key tiles of this CTA so far
+
+    if (warp < 2) {
+        // ------------------------------------------------ TMA producers (a lane per box)
+        if (lane == 0) { tma_prefetch_desc(warp ? &tmV : &tmK); tma_prefetch_desc(warp ? &tmV8 : &tmG); }
+        fence_proxy_async_global();         // rows appended by the kernel before, read through the async proxy here
+        const int box = p.box_rows, boxes = PP_BN / box, beyond = (int)((long long)p.pv.n_pages * KH * p.pv.page >> 3);
+        bool ok = true;
+        int gate_of[2] = {-1, -1}, wholes = 0, pc = 0;
+        for (; ok && w.piece(tokens); w.next(p, tokens), ++pc) {
+            const int end = w.base + w.n;   // the request's rows
+            if (warp == 1) ok = mbar_wait(&bars.q_tmem, pc & 1);   // Q has left the V buffer
+            for (int j = w.at.w; ok && j < w.t1; ++j, ++jj) {
+                const int s = jj & 1;
+                // a lane's box: `rows` of them from key `key`; 8-row boxes where V ends inside the tile
+                const bool tail = warp == 1 && (j + 1) * PP_BN > end;
+                const int rows = tail ? 8 : box, key = j * PP_BN + lane * rows, n_box = tail ? PP_BN / 8 : boxes;
+                int at = beyond;
+                if (lane < n_box && key < end) {
+                    const long long row = pages_row(p.pv, w.at.x, w.at.y, key);
+                    if (row >= 0) at = (int)(row >> 3);
+                }
+                if (warp == 0) {
+                    if (jj >= 2) ok = mbar_wait(&bars.k_empty[s], ((jj >> 1) - 1) & 1);
+                    if (ok && gate_of[s] >= 0) { ok = mbar_wait(&bars.epi_done, gate_of[s] & 1); gate_of[s] = -1; }
+                } else if (jj >= 1) {
+                    ok = mbar_wait(&bars.v_empty, (jj - 1) & 1);
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                uint64_t *bar = warp == 0 ? &bars.k_full[s] : &bars.v_full;
+                uint8_t *to = warp == 0 ? sK + s * PP_TILE : sV;
+                if (lane == 0) mbar_expect_tx(bar, PP_TILE);
+                __syncwarp();
+                if (lane < n_box) tma_load_4d(to + lane * rows * 512, warp == 0 ? &tmK : tail ? &tmV8 : &tmV, 0, 0, 0, at, bar);
+                __syncwarp();
+            }
+            if (warp == 0 && ok && w.ends && w.at.w == 0) {
+                // the gate tile, into the stage of the last K tile once S has read it
+                const int s = (jj - 1) & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.k_empty[s], ((jj - 1) >> 1) & 1));
+                if (ok && lane == 0) {
+                    mbar_expect_tx(&bars.g_full, PP_TILE);
+                    for (int c = 0; c < 4; ++c)
+                        tma_load_3d(sK + s * PP_TILE + c * (PP_BM * 128), &tmG, GQA_HD + 64 * c, w.at.y * group,
+                                    w.row0 + w.at.z * tokens, &bars.g_full);
+                }
+                gate_of[s] = wholes++;
+            }
+        }
+    } else if (warp == 2) {
+        // ------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            constexpr uint32_t ID_QK = tc::idesc_bf16(PP_BM, PP_BN, 0, 0);
+            constexpr uint32_t ID_PV = tc::idesc_bf16(PP_BM, GQA_HD, 0, 1);
+            const uint32_t aK = smem_u32(sK), aV = smem_u32(sV), aP = smem_u32(sP);
+            auto issue_s = [&](int j) -> bool {
+                const int s = j & 1;
+                if (!mbar_wait(&bars.k_full[s], (j >> 1) & 1)) return false;
+                if (j >= 1 && !mbar_wait(&bars.s_free, (j - 1) & 1)) return false;   // S(j-1) read out
+                tc::fence_after();
+#pragma unroll
+                for (int kk = 0; kk < GQA_HD / 16; ++kk)
+                    tc::mma_bf16_ts(tS, tQ + kk * 8, pp_desc_k(aK + s * PP_TILE + (kk >> 2) * 1024 + (kk & 3) * 32), ID_QK,
+                                    kk > 0 ? 1u : 0u);
+                tc::commit(&bars.s_full);
+                tc::commit(&bars.k_empty[s]);
+                return true;
+            };
+            auto issue_pv = [&](int j, bool fresh) -> bool {
+                if (!mbar_wait(&bars.p_full, j & 1)) return false;
+                if (!mbar_wait(&bars.v_full, j & 1)) return false;
+                tc::fence_after();
+#pragma unroll
+                for (int kk = 0; kk < PP_BN / 16; ++kk) {
+                    const uint64_t da = tc::desc_k_sw128(aP + (kk >> 2) * (PP_BM * 128) + (kk & 3) * 32);
+                    const uint64_t db = tc::desc_mn_sw128(aV + kk * 8192, 1024, 4096);
+                    tc::mma_bf16(tO, da, db, ID_PV, (!fresh || kk > 0) ? 1u : 0u);
+                }
+                tc::commit(&bars.pv_done);
+                tc::commit(&bars.v_empty);
+                return true;
+            };
+            bool ok = true;
+            for (int pc = 0; ok && w.piece(tokens); w.next(p, tokens), ++pc) {
+                ok = mbar_wait(&bars.q_tmem, pc & 1);
+                tc::fence_after();
+                if (ok) ok = issue_s(jj);
+                for (int j = w.at.w; ok && j < w.t1; ++j, ++jj) {
+                    if (j + 1 < w.t1) ok = issue_s(jj + 1);
+                    if (ok) ok = issue_pv(jj, j == w.at.w);
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------ q, softmax, epilogue
+        // Waits never break out of the loops here (a time-out raises the error
+        // word and they run on): all 256 threads meet at the named barrier.
+        const int quarter = warp & 3, sw = warp - 3, u = sw >> 2;
+        const int g = lane >> 2, tq = lane & 3;
+        const int rbase = 32 * quarter + 16 * u;
+        const uint32_t lane_off = (uint32_t)rbase << 16;
+        const int row0 = rbase + g, row1 = row0 + 8;
+        const float sl2 = p.scale_log2;
+        const __nv_bfloat16 *qg = static_cast<const __nv_bfloat16 *>(p.qg);
+        int wholes = 0;
+        for (int pc = 0; w.piece(tokens); w.next(p, tokens), ++pc) {
+            const int tok0 = w.at.z * tokens, end = w.base + w.n;
+            {   // ---- q: a warp norms and ropes 16 rows (row = token * group + head), through
+                // the V buffer (128B-swizzled 64-column blocks) into TMEM as bf16 pairs
+                float *cs = reinterpret_cast<float *>(sP + sw * 4096), *sn = cs + GQA_HD / 2, *vw = sn + GQA_HD / 2;
+                int known = -1;
+#pragma unroll 1
+                for (int r4 = 0; r4 < 16; r4 += 4) {
+                    Raw8<__nv_bfloat16> raw[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 16 * sw + r4 + i, t = min(tok0 + (r >> gs), w.n - 1);
+                        raw[i].load(qg + ((size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1))) * 2 * GQA_HD + lane * 8);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 16 * sw + r4 + i, t = min(tok0 + (r >> gs), w.n - 1);
+                        if (t != known) {
+                            __syncwarp();
+                            pages_rope_table(cs, sn, w.base + t, p.rot, f.turn, lane, 32);
+                            __syncwarp();
+                            known = t;
+                        }
+                        float x[8], y[8];
+                        raw[i].unpack(x);
+                        pages_norm_rope(y, x, p.qnw, p.eps, p.rot, cs, sn, vw, lane);
+                        store8(reinterpret_cast<__nv_bfloat16 *>(sV + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), y);
+                    }
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
+                const int row = 32 * quarter + lane;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    float v[32];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const int d = 128 * u + 64 * hh + 8 * c;
+                        const uint4 x = *reinterpret_cast<const uint4 *>(
+                            sV + (d >> 6) * (PP_BM * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4));
+                        v[4 * c] = __uint_as_float(x.x); v[4 * c + 1] = __uint_as_float(x.y);
+                        v[4 * c + 2] = __uint_as_float(x.z); v[4 * c + 3] = __uint_as_float(x.w);
+                    }
+                    tc::st32(tQ + 64 * u + 32 * hh + ((uint32_t)(32 * quarter) << 16), v);
+                }
+                tc::wait_st();
+                tc::fence_before();
+                fence_proxy_async();        // what was written and read here before V tiles land in its place
+                mbar_arrive(&bars.q_tmem);
+            }
+            const int qpos0 = w.base + tok0 + (row0 >> gs), qpos1 = w.base + tok0 + (row1 >> gs);
+            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+            for (int i = w.at.w; i < w.t1; ++i, ++jj) {
+                mbar_wait(&bars.s_full, jj & 1);
+                tc::fence_after();
+                float x[64];
+                {
+                    float xa[32], xb[32];
+                    tc::ld16x256_x8(tS + lane_off, xa);
+                    tc::ld16x256_x8(tS + 64 + lane_off, xb);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) { x[e] = xa[e]; x[32 + e] = xb[e]; }
+                }
+                tc::fence_before();
+                mbar_arrive(&bars.s_free);
+                // x[4j + 0/1]: row0, keys 8j + 2tq, +1; x[4j + 2/3]: row1. Raw scores; the
+                // scale is applied inside the exponent (it is positive: the maximum commutes)
+                const int key0 = i * PP_BN;
+                if (key0 + PP_BN - 1 > qpos0) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int k = key0 + 8 * j + 2 * tq;
+                        if (k > qpos0) x[4 * j] = -INFINITY;
+                        if (k + 1 > qpos0) x[4 * j + 1] = -INFINITY;
+                        if (k > qpos1) x[4 * j + 2] = -INFINITY;
+                        if (k + 1 > qpos1) x[4 * j + 3] = -INFINITY;
+                    }
+                }
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    mx0 = fmaxf(mx0, fmaxf(x[4 * j], x[4 * j + 1]));
+                    mx1 = fmaxf(mx1, fmaxf(x[4 * j + 2], x[4 * j + 3]));
+                }
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2)) * sl2;
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2)) * sl2;
+                const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+                if (i == w.at.w) {
+                    m0 = mn0; m1 = mn1;
+                } else {
+                    const bool need0 = mn0 > m0 + PF_RESCALE_LOG2, need1 = mn1 > m1 + PF_RESCALE_LOG2;
+                    if (__any_sync(0xffffffffu, need0 || need1)) {
+                        mbar_wait(&bars.pv_done, (jj - 1) & 1);        // O complete up to the tile before
+                        tc::fence_after();
+                        const float a0 = need0 ? exp2f(m0 - mn0) : 1.f, a1 = need1 ? exp2f(m1 - mn1) : 1.f;
+#pragma unroll 1
+                        for (int c = 0; c < GQA_HD / 64; ++c) {
+                            float o[32];
+                            tc::ld16x256_x8(tO + 64 * c + lane_off, o);
+                            tc::wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                o[4 * j] *= a0; o[4 * j + 1] *= a0; o[4 * j + 2] *= a1; o[4 * j + 3] *= a1;
+                            }
+                            tc::st16x256_x8(tO + 64 * c + lane_off, o);
+                        }
+                        tc::wait_st();
+                        if (need0) { l0 *= a0; m0 = mn0; }
+                        if (need1) { l1 *= a1; m1 = mn1; }
+                    }
+                }
+                const float mu0 = (m0 == -INFINITY) ? 0.f : m0, mu1 = (m1 == -INFINITY) ? 0.f : m1;
+                uint32_t pk0[16], pk1[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float p00 = ex2_approx(fmaf(x[4 * j], sl2, -mu0)), p01 = ex2_approx(fmaf(x[4 * j + 1], sl2, -mu0));
+                    const float p10 = ex2_approx(fmaf(x[4 * j + 2], sl2, -mu1)), p11 = ex2_approx(fmaf(x[4 * j + 3], sl2, -mu1));
+                    l0 += p00 + p01;
+                    l1 += p10 + p11;
+                    pk0[j] = pack_bf16(p00, p01);
+                    pk1[j] = pack_bf16(p10, p11);
+                }
+                if (i > w.at.w) mbar_wait(&bars.pv_done, (jj - 1) & 1);   // the P buffer's last reader
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int at = (j >> 3) * (PP_BM * 128);
+                    *reinterpret_cast<uint32_t *>(sP + at + row0 * 128 + (((j & 7) ^ (row0 & 7)) << 4) + 4 * tq) = pk0[j];
+                    *reinterpret_cast<uint32_t *>(sP + at + row1 * 128 + (((j & 7) ^ (row1 & 7)) << 4) + 4 * tq) = pk1[j];
+                }
+                if (key0 + PP_BN > end && (end & 7) && end > key0 && sw == 0) {
+                    // V rows end .. end | 7 of the tile's last group hold what the page held before
+                    mbar_wait(&bars.v_full, jj & 1);
+                    const int from = end - key0, n = 8 - (end & 7);
+                    for (int j = lane; j < n * 32; j += 32) {
+                        const int r = from + (j >> 5), c = (j & 31) >> 3;
+                        *reinterpret_cast<uint4 *>(sV + (r >> 3) * 4096 + c * 1024 + (r & 7) * 128 + (j & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                fence_proxy_async();
+                mbar_arrive(&bars.p_full);
+            }
+            l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+            l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+            const bool whole = w.ends && w.at.w == 0;
+            const size_t slot = 2 * cta + (w.at.w == 0 ? 1 : 0);
+            if (tq == 0) {
+                bars.lsum[row0] = l0; bars.lsum[row1] = l1;
+                if (!whole) {
+                    part.ml[slot * PP_BM + row0] = make_float2(m0, l0);
+                    part.ml[slot * PP_BM + row1] = make_float2(m1, l1);
+                }
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
+            mbar_wait(&bars.pv_done, (jj - 1) & 1);
+            tc::fence_after();
+            const int row = 32 * quarter + lane;
+            const uint32_t qoff = (uint32_t)(32 * quarter) << 16;
+            if (whole) {
+                // thread = tile row, O columns 128 u ..; gate and staged ctx share the
+                // layout of 128B-swizzled 64 x 128 boxes; then a warp per row to memory
+                const float inv_l = 1.f / bars.lsum[row];
+                const uint8_t *gt = sK + ((jj - 1) & 1) * PP_TILE;
+                mbar_wait(&bars.g_full, wholes++ & 1);
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float o[32];
+                    const int d0 = 128 * u + 32 * c;
+                    tc::ld32(tO + d0 + qoff, o);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int chunk = ((d0 & 63) >> 3) + k;
+                        const uint32_t off = (d0 >> 6) * (PP_BM * 128) + row * 128 + ((chunk ^ (row & 7)) << 4);
+                        float gv[8], y[8];
+                        load8v(reinterpret_cast<const __nv_bfloat16 *>(gt + off), gv);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = o[8 * k + e] * inv_l * sigmoidf_(gv[e]);
+                        store8v(reinterpret_cast<__nv_bfloat16 *>(sV + off), y);
+                    }
+                }
+                fence_proxy_async();        // the gate has been read: its stage takes K tiles again
+                mbar_arrive(&bars.epi_done);
+                asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
+#pragma unroll 4
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 16 * sw + i, t = tok0 + (r >> gs);
+                    if (t >= w.n) break;
+                    const uint4 x = *reinterpret_cast<const uint4 *>(sV + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                    *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.ctx) +
+                                               ((size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1))) * GQA_HD + lane * 8) = x;
+                }
+            } else {
+                // O as it is, [16-byte column chunk][row]: a warp writes 512 bytes at a time
+                float4 *out = reinterpret_cast<float4 *>(part.o) + slot * (PP_BM * GQA_HD / 4) + quarter * 32 + lane;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    float o[32];
+                    tc::ld32(tO + 128 * u + 32 * c + qoff, o);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        out[(32 * u + 8 * c + j) * PP_BM] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
+            }
+            tc::fence_before();             // O read: the next piece's products overwrite it
+            asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc::fence_after();
+        tc::dealloc(tbase, 512);
+    }
+}
+
+// One CTA per (first CTA of a split unit, 32 rows, 32 dims): adds the pieces
+// up, lane = row, warp = 4 dims, then turns the block to write 64-byte runs.
+constexpr int PJ_THREADS = 256;
+__global__ void __launch_bounds__(PJ_THREADS)
+pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
+{
+    __shared__ float turned[32][33];
+    const int a = blockIdx.x, quarter = blockIdx.y & 3, block = blockIdx.y >> 2, tid = threadIdx.x, j = tid >> 5, lane = tid & 31;
+    griddep_wait();
+    const int4 unit = part.plan[a + 1], first = part.plan[a];
+    if (unit.w == 0) return;                // no unit is cut between CTA a and the next
+    auto same = [&](const int4 &x) { return x.x == unit.x && x.y == unit.y && x.z == unit.z && x.w > 0; };
+    if (same(first)) return;                // .. or its first piece is an earlier CTA's
+    const int n = 1 + __syncthreads_count(a + 1 + tid <= (int)gridDim.x && same(part.plan[a + 1 + tid]));
+    const int row = quarter * 32 + lane;
     float m = -INFINITY, l = 0.f;
-    for (int t = 0; t <= pos; ++t) {
-        const long long at = pages_row(p.pv, r, kh, t);
-        if (at < 0) continue;
-        float kk[8], vv[8], s = 0.f;
-        load8<__nv_bfloat16>(p.pv.k + at * GQA_HD + lane * 8, kk);
-        load8<__nv_bfloat16>(p.pv.v + at * GQA_HD + lane * 8, vv);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(q[i], kk[i], s);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= p.scale_log2;
-        const float mn = fmaxf(m, s), al = exp2f(m - mn), e = exp2f(s - mn);
-        l = l * al + e;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = o[i] * al + e * vv[i];
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+        const size_t slot = s ? 2 * (a + s) : 2 * a + 1;
+        const float2 ml = part.ml[slot * PP_BM + row];
+        const float4 x = reinterpret_cast<const float4 *>(part.o)[slot * (PP_BM * GQA_HD / 4) + (8 * block + j) * PP_BM + row];
+        if (ml.x == -INFINITY) continue;
+        const float mn = fmaxf(m, ml.x), fo = m == -INFINITY ? 0.f : exp2f(m - mn), fs = exp2f(ml.x - mn);
+        o.x = o.x * fo + x.x * fs; o.y = o.y * fo + x.y * fs; o.z = o.z * fo + x.z * fs; o.w = o.w * fo + x.w * fs;
+        l = l * fo + ml.y * fs;
         m = mn;
     }
-    TI *out = static_cast<TI *>(p.ctx) + ((size_t)row * p.H + h) * GQA_HD + lane * 8;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = 1.f / l;
+    turned[lane][4 * j] = o.x * inv; turned[lane][4 * j + 1] = o.y * inv;
+    turned[lane][4 * j + 2] = o.z * inv; turned[lane][4 * j + 3] = o.w * inv;
+    __syncthreads();
+    int row0, base;
+    const int rows = pages_rows_of(p, unit.x, row0, base);
+    const int group = p.H / p.pv.KH, tokens = PP_BM / group, r = tid >> 3, c = (tid & 7) * 4;
+    const int tile_row = quarter * 32 + r, t = unit.z * tokens + tile_row / group;
+    if (t >= rows) return;
+    const size_t at = (size_t)(row0 + t) * p.H + unit.y * group + tile_row % group;
+    float g[4], y[4];
+    load4(static_cast<const __nv_bfloat16 *>(p.qg) + at * 2 * GQA_HD + GQA_HD + block * 32 + c, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = from_f32<TI>(o[i] * inv * sigmoidf_(g[i]));
+    for (int e = 0; e < 4; ++e) y[e] = turned[r][c + e] * sigmoidf_(g[e]);
+    store4(static_cast<__nv_bfloat16 *>(p.ctx) + at * GQA_HD + block * 32 + c, y);
 }
 
-cudaError_t launch_pages_append(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st)
+cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tv8, const CUtensorMap &tg,
+                                 const GqaPagesArgs &a, const PagesPart &part, const RopeFreq &f, int ctas, cudaStream_t st)
 {
-    if (in_bf16) pages_append_kernel<__nv_bfloat16><<<a.S, 128, 0, st>>>(a, f);
-    else pages_append_kernel<float><<<a.S, 128, 0, st>>>(a, f);
-    return cudaGetLastError();
-}
-cudaError_t launch_pages_attend(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st)
-{
-    const dim3 grid(a.S, (a.H + 3) / 4);
-    if (in_bf16) pages_attend_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a, f);
-    else pages_attend_kernel<float><<<grid, 128, 0, st>>>(a, f);
-    return cudaGetLastError();
+    cudaError_t e = cudaFuncSetAttribute(pages_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PP_SMEM);
+    if (e != cudaSuccess) return e;
+    const int rows_per = PL_THREADS / 32;
+    pages_plan_kernel<<<1 + (int)(((long long)a.S * a.pv.KH + rows_per - 1) / rows_per), PL_THREADS, 0, st>>>(a, part, ctas, f);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(PP_THREADS); cfg.dynamicSmemBytes = PP_SMEM;
+    if ((e = cudaLaunchKernelEx(&cfg, pages_prefill_kernel, tk, tv, tv8, tg, a, part, f)) != cudaSuccess) return e;
+    cfg.gridDim = dim3(ctas, 32); cfg.blockDim = dim3(PJ_THREADS); cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, pages_prefill_join_kernel, a, part);
 }
 
 }  // namespace coli

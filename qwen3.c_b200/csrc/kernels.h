@@ -210,6 +210,7 @@ struct GqaPagesArgs {
     const int *cu, *base;
     void *ctx;                // [rows][H][hd]
     int n_req, S, H, rot;
+    int box_rows;             // prefill: rows of a K / V box (the largest power of two in a page, at most 128)
     float eps, scale_log2;
 };
 // Pieces of units that more than one CTA works on (workspace): piece slot
@@ -218,12 +219,13 @@ struct PagesPart {
     float *o;             // [2 ctas][rows of a unit][hd]
     float2 *ml;           // [2 ctas][rows of a unit] (max, sum), log2 domain
     float4 *park;         // [4 ctas][512] a warp's piece, in its own layout, until its range is done
-    int4 *units;          // [ctas] unit that begins in CTA c and goes on: (last CTA or -1, request, KV head, ..)
+    int4 *plan;           // prefill: [ctas + 1] where each CTA's range starts (request, KV head, query tile, key tile)
+    int4 *units;          // decode: [ctas] unit that begins in CTA c and goes on: (last CTA or -1, request, KV head, ..)
 };
 cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, const GqaPagesArgs &a, const PagesPart &part,
                                 const RopeFreq &f, int in_bf16, int ctas, cudaStream_t st);
-cudaError_t launch_pages_append(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st);
-cudaError_t launch_pages_attend(const GqaPagesArgs &a, const RopeFreq &f, int in_bf16, cudaStream_t st);
+cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tv8, const CUtensorMap &tg,
+                                 const GqaPagesArgs &a, const PagesPart &part, const RopeFreq &f, int ctas, cudaStream_t st);
 
 // Page moves over every layer's K and V (base: [layers][K, V][n_pages][page_bytes]).
 struct PageMoveArgs {

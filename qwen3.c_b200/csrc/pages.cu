@@ -18,7 +18,8 @@ struct ColiCudaPages {
     float *norm_w;            // [layers][2][256]
     unsigned char *norm_set;  // [layers] (host)
     uint8_t *ws, *own_ws;
-    CUtensorMap *maps;        // [layers][K, V], boxes of 16 rows
+    CUtensorMap *maps;        // [layers][K, V] in boxes of 16 rows, K and V of box_rows, V of 8
+    int box_rows;
     int rot;                  // rotary frequencies as last used
     float theta;
     RopeFreq freq;
@@ -35,8 +36,8 @@ size_t pages_page_bytes(int KH, int page) { return (size_t)KH * page * GQA_HD * 
 size_t pages_norm_bytes(int layers) { return (size_t)layers * 2 * GQA_HD * 4; }
 size_t pages_list_bytes(int n_pages) { return ((size_t)n_pages * 4 + 255) & ~size_t(255); }
 // the workspace serves one call at a time: a compaction's lists, or an attention call's pieces
-size_t pages_part_rows() { return (size_t)2 * G.num_sms * GQA_GRP; }
-size_t pages_part_bytes() { return pages_part_rows() * (GQA_HD * 4 + 8) + (size_t)G.num_sms * (4 * 512 + 1) * 16; }
+size_t pages_part_rows() { return (size_t)2 * G.num_sms * PP_BM; }   // decode: 8 rows to a piece, prefill: 128
+size_t pages_part_bytes() { return pages_part_rows() * (GQA_HD * 4 + 8) + (size_t)G.num_sms * (4 * 512 + 2) * 16 + 16; }
 size_t pages_ws_bytes(int n_pages)
 {
     return (std::max(3 * pages_list_bytes(n_pages) + 256, pages_part_bytes()) + 255) & ~size_t(255);
@@ -48,6 +49,7 @@ PagesPart pages_part(uint8_t *ws)
     t.ml = (float2 *)(ws + pages_part_rows() * GQA_HD * 4);
     t.park = (float4 *)(t.ml + pages_part_rows());
     t.units = (int4 *)(t.park + (size_t)G.num_sms * 4 * 512);
+    t.plan = t.units + G.num_sms;
     return t;
 }
 
@@ -145,7 +147,7 @@ int pages_attend_args(GqaPagesArgs &a, ColiCudaPages *p, int layer, const void *
     if (!p->norm_set[layer]) return fail("pages: q/k norm weights of layer %d not set (coli_cuda_pages_norm_weight)", layer);
     if (rot < 2 || rot > hd || (rot & 1)) return fail("pages: bad rot %d", rot);
     if (!(eps >= 0.f) || !(theta > 0.f) || std::isinf(eps) || std::isinf(theta)) return fail("pages: bad eps or theta");
-    if (max_pages < 1 || (long long)max_pages * p->page > 0x7fffffffLL) return fail("pages: bad max_pages %d", max_pages);
+    if (max_pages < 1 || (long long)max_pages * p->page > 1 << 30) return fail("pages: bad max_pages %d (max_pages * page up to 2^30)", max_pages);
     if (!qg || !k || !v || !base || !table || !ctx) return fail("pages: a null pointer among the arguments");
     if (((uintptr_t)qg | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ctx) & 15)
         return fail("pages: qg, k, v and ctx must be 16-byte aligned");
@@ -166,6 +168,20 @@ int pages_attend_args(GqaPagesArgs &a, ColiCudaPages *p, int layer, const void *
     a.qnw = p->norm_w + (size_t)layer * 2 * GQA_HD; a.knw = a.qnw + GQA_HD;
     a.H = H; a.rot = rot; a.eps = eps;
     a.scale_log2 = (1.f / sqrtf((float)hd)) * 1.4426950408889634f;
+    return 1;
+}
+
+// The gate halves of q|gate [S][H][2 hd] in boxes of 64 columns x the group's heads x 128 / group tokens.
+int make_pages_gate_tmap(CUtensorMap *m, const void *qg, int S, int H, int group)
+{
+    cuuint64_t dims[3] = {2 * GQA_HD, (cuuint64_t)H, (cuuint64_t)S};
+    cuuint64_t strides[2] = {2 * GQA_HD * 2, (cuuint64_t)H * 2 * GQA_HD * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(PP_BM / group)};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = G.encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(qg), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled (gate) failed (%d)", (int)r);
     return 1;
 }
 
@@ -193,7 +209,7 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
     p->layers = layers; p->n_pages = n_pages; p->page = page; p->KH = KH;
     p->base = (uint8_t *)kv_dev;
     p->norm_set = new (std::nothrow) unsigned char[layers]();
-    p->maps = new (std::nothrow) CUtensorMap[2 * layers];
+    p->maps = new (std::nothrow) CUtensorMap[5 * layers];
     const size_t bytes = (size_t)layers * 2 * n_pages * pages_page_bytes(KH, page);
     int ok = p->norm_set && p->maps;
     if (!ok) fail("pages: out of host memory");
@@ -204,8 +220,15 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
     }
     ok = ok && dev_alloc((void **)&p->norm_w, pages_norm_bytes(layers)) && dev_alloc((void **)&p->own_ws, pages_ws_bytes(n_pages));
     p->ws = p->own_ws;
-    for (int i = 0; ok && i < 2 * layers; ++i)
-        ok = make_pages_tmap(p->maps + i, p->base + i * (bytes / (2 * layers)), (long long)n_pages * KH * page, GQA_TILE);
+    p->box_rows = std::min(PP_BN, page & -page);
+    for (int i = 0; ok && i < layers; ++i) {
+        uint8_t *k = p->base + (size_t)i * (bytes / layers), *v = k + bytes / layers / 2;
+        const long long rows = (long long)n_pages * KH * page;
+        CUtensorMap *m = p->maps + 5 * i;
+        ok = make_pages_tmap(m, k, rows, GQA_TILE) && make_pages_tmap(m + 1, v, rows, GQA_TILE) &&
+             make_pages_tmap(m + 2, k, rows, p->box_rows) && make_pages_tmap(m + 3, v, rows, p->box_rows) &&
+             make_pages_tmap(m + 4, v, rows, 8);
+    }
     if (!ok) { pages_release(p); return 0; }
     g_pages[slot] = p;
     *pages = p;
@@ -274,7 +297,7 @@ int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const
         return fail("pages: a table of %d x %d pages passes 2^31 tiles", B, max_pages);
     a.n_req = a.S = B;
     g_pages_ran = true;
-    CK(launch_pages_decode(pages->maps[2 * layer], pages->maps[2 * layer + 1], a, pages_part(pages->ws), pages->freq, dtype,
+    CK(launch_pages_decode(pages->maps[5 * layer], pages->maps[5 * layer + 1], a, pages_part(pages->ws), pages->freq, dtype,
                            G.num_sms, stream()));
     g_launches += 2;
     return 1;
@@ -295,9 +318,12 @@ int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, 
     a.cu = cu;
     a.n_req = n_seq; a.S = S;
     g_pages_ran = true;
-    CK(launch_pages_append(a, pages->freq, 1, stream()));
-    CK(launch_pages_attend(a, pages->freq, 1, stream()));
-    g_launches += 2;
+    const CUtensorMap *m = pages->maps + 5 * layer;
+    CUtensorMap gate;
+    if (!make_pages_gate_tmap(&gate, qg, S, H, H / KH)) return 0;
+    a.box_rows = pages->box_rows;
+    CK(launch_pages_prefill(m[2], m[3], m[4], gate, a, pages_part(pages->ws), pages->freq, G.num_sms, stream()));
+    g_launches += 3;
     return 1;
 }
 
@@ -317,7 +343,7 @@ int coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, con
                              int *table, int n_req, int max_pages)
 {
     if (!pages_handle(pages)) return 0;
-    if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 0x7fffffffLL)
+    if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 1 << 30)
         return fail("pages: bad table %d x %d", n_req, max_pages);
     if (n < 0 || n >= n_req) return fail("pages: %d forks among %d requests", n, n_req);
     if (n == 0) return 1;
@@ -335,7 +361,7 @@ int coli_cuda_pages_compact_dev(ColiCudaPages *pages, int n_req, const int *len,
                                 int *table_out, int *live)
 {
     if (!pages_handle(pages)) return 0;
-    if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 0x7fffffffLL)
+    if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 1 << 30)
         return fail("pages: bad table %d x %d", n_req, max_pages);
     if (!len || !table || !table_out || !live) return fail("pages: a null pointer among the arguments");
     PageCompactArgs c{};
