@@ -32,6 +32,23 @@ __device__ __forceinline__ void pages_rope_table(float *cs, float *sn, int pos, 
     }
 }
 
+// Scalars of these kernels. The IEEE division and square root are long
+// branchy sequences (a sigmoid with one took 150 cycles per element, a third of a
+// short call); these use the approximate instructions, relative error about
+// 2^-22, which neither bf16 nor the fp32 outputs' own sums resolve.
+__device__ __forceinline__ float rcp_approx(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float gate_of(float x) { return rcp_approx(1.f + ex2_approx(x * -1.4426950408889634f)); }   // sigmoid
+__device__ __forceinline__ float rms_factor(float s2, float eps)     // 1 / sqrt(s2 / hd + eps), one Newton step
+{
+    const float a = fmaf(s2, 1.f / GQA_HD, eps), r = rsqrtf(a);
+    return r * fmaf(-0.5f * a * r, r, 1.5f);
+}
+
 // First row of K/V of request r, KV head kh, position pos; -1 for a page id
 // outside the pool.
 __device__ __forceinline__ long long pages_row(const PageView &v, int r, int kh, int pos)
@@ -59,6 +76,113 @@ __device__ __forceinline__ int pages_rows_of(const GqaPagesArgs &p, int r, int &
     }
     if ((long long)pos0 + n > (long long)p.pv.max_pages * p.pv.page) { pages_error(PAGES_BAD_POS); return 0; }
     return n;
+}
+
+// One q or k row in the registers of a warp, lane = 8 dims: x raw in, normed
+// and roped out; sums in fp32. w1 is the lane's 1 + w, w the whole row's 1 + w and
+// `raw` the raw row (both read only where the rotation's half width is no
+// multiple of 8, so that a dim's partner is not one other lane's).
+template <typename TI>
+__device__ __forceinline__ void pages_norm_rope(float (&x)[8], const float (&w1)[8], float eps, int rot, const float *cs,
+                                                const float *sn, const TI *raw, const float *w, int lane)
+{
+    float s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s2 = fmaf(x[i], x[i], s2);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+    const float rs = rms_factor(s2, eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= rs * w1[i];
+    const int half = rot >> 1, d0 = lane * 8;
+    if ((half & 7) == 0) {                  // no branch inside: dims behind rot turn by angle 0
+        const int hl = half >> 3, from = lane < hl ? lane + hl : lane - hl, j = d0 < half ? d0 : d0 < rot ? d0 - half : 0;
+        const float sign = d0 < half ? -1.f : d0 < rot ? 1.f : 0.f;
+        float c[8], sv[8];
+        load8<float>(cs + j, c);
+        load8<float>(sn + j, sv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float z = __shfl_sync(0xffffffffu, x[i], from);
+            x[i] = x[i] * (d0 < rot ? c[i] : 1.f) + z * (sign * sv[i]);
+        }
+    } else {
+#pragma unroll 1
+        for (int d = d0; d < min(d0 + 8, rot); ++d) {
+            const bool lo = d < half;
+            const int j = lo ? d : d - half, o = lo ? d + half : j;
+            const float z = to_f32(raw[o]) * rs * w[o], v = to_f32(raw[d]) * rs * w[d];
+            const float t = lo ? v * cs[j] - z * sn[j] : v * cs[j] + z * sn[j];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (d - d0 == i) x[i] = t;
+        }
+    }
+}
+
+// Eight rows at once, four lanes (q = lane % 4) each: norm and partial RoPE of
+// rows in shared memory, in place. A row gives its 8-dim chunk c (load / store) and
+// single dims (load1 / store1); chunks go round the four lanes, and a rotated
+// pair of chunks is one lane's, so nothing is overwritten before it is read.
+// A quarter of the instructions of a row per warp, and two shuffles instead of 13.
+template <typename Row>
+__device__ __forceinline__ void pages_norm_rope_quad(const Row &row, int q, const float *w1, float eps, int rot, const float *cs,
+                                                     const float *sn, bool on)
+{
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        float x[8];
+        row.load(4 * k + q, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { s0 = fmaf(x[i], x[i], s0); s1 = fmaf(x[4 + i], x[4 + i], s1); }
+    }
+    s0 += s1;
+    s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
+    s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
+    const float rs = on ? rms_factor(s0, eps) : 0.f;
+    __syncwarp();
+    const int half = rot >> 1;
+    if ((half & 7) == 0) {
+        const int hc = half >> 3;
+#pragma unroll 1
+        for (int c = q; c < hc; c += 4) {
+            float a[8], b[8], wa[8], wb[8], co[8], si[8];
+            row.load(c, a);
+            row.load(c + hc, b);
+            load8<float>(w1 + 8 * c, wa);
+            load8<float>(w1 + 8 * (c + hc), wb);
+            load8<float>(cs + 8 * c, co);
+            load8<float>(sn + 8 * c, si);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = a[i] * wa[i] * rs, y = b[i] * wb[i] * rs;
+                a[i] = x * co[i] - y * si[i];
+                b[i] = y * co[i] + x * si[i];
+            }
+            row.store(c, a);
+            row.store(c + hc, b);
+        }
+#pragma unroll 3
+        for (int c = (rot >> 3) + q; c < GQA_HD / 8; c += 4) {
+            float a[8], wa[8];
+            row.load(c, a);
+            load8<float>(w1 + 8 * c, wa);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] *= wa[i] * rs;
+            row.store(c, a);
+        }
+    } else {
+#pragma unroll 1
+        for (int j = q; j < half; j += 4) {
+            const float x = row.load1(j) * w1[j] * rs, y = row.load1(j + half) * w1[j + half] * rs;
+            row.store1(j, x * cs[j] - y * sn[j]);
+            row.store1(j + half, y * cs[j] + x * sn[j]);
+        }
+#pragma unroll 1
+        for (int d = rot + q; d < GQA_HD; d += 4) row.store1(d, row.load1(d) * w1[d] * rs);
+    }
+    __syncwarp();
 }
 
 // ------------------------------------------------------------------ decode
@@ -96,18 +220,55 @@ constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_STAGES = 3, PD_STAGE 
 constexpr int PD_OROW = 132;                 // floats between heads of O: 8 banks apart for the writers' heads
 template <typename TI> struct PdEntry {      // layout of the q entry and of the gate entry in a stage
     static constexpr bool F32 = sizeof(TI) == 4;
+    static constexpr int PARTS = F32 ? 3 : 2;
     static constexpr int BYTES = GQA_HD * (int)sizeof(TI);    // a head's q (or gate), the new k, the new v
-    static constexpr int ROW = BYTES + 8 * (int)sizeof(TI);   // apart: no bank conflicts between a quad's and the next head's reads
+    // rows of the q entry: fp32, or bf16 with room for the second part; 4 banks (fp32: 8, for pairs of words) apart
+    static constexpr int ROW = 1024 + (F32 ? 32 : 16);
     static constexpr int KV = GQA_GRP * ROW;
-    // the roped dims times 1 + w, fp32, in rows of YROW: behind the raw rows, or in their place
-    static constexpr int Y = F32 ? 0 : (GQA_GRP + 2) * ROW, YROW = F32 ? ROW / 4 : 264;
-    static constexpr int O = GQA_GRP * ROW;                   // gate entry: half of O, fp32, behind the gate rows
-    static_assert((GQA_GRP + 2) * ROW <= PD_STAGE && Y + (GQA_GRP + 1) * YROW * 4 <= PD_STAGE && O + GQA_GRP * PD_OROW * 4 <= PD_STAGE && ROW % 16 == 0, "");
+    static constexpr int GROW = BYTES + 8 * (int)sizeof(TI);  // rows of the gate entry
+    static constexpr int O = GQA_GRP * GROW;                  // gate entry: half of O, fp32, behind the gate rows
+    static_assert((GQA_GRP + 2) * ROW <= PD_STAGE && O + GQA_GRP * PD_OROW * 4 <= PD_STAGE && GROW % 16 == 0, "");
+};
+// A head's row in the q entry, normed and roped in place: bf16 as its parts (hi, and lo 512 bytes behind), fp32 as it is.
+template <typename TI> struct PdRow;
+template <> struct PdRow<__nv_bfloat16> {
+    uint8_t *at;
+    __device__ __forceinline__ void load(int c, float (&x)[8]) const { load8<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16 *>(at) + 8 * c, x); }
+    __device__ __forceinline__ void store(int c, const float (&x)[8]) const
+    {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
+            lo[i] = pack_bf16(x[2 * i] - __uint_as_float(hi[i] << 16), x[2 * i + 1] - __uint_as_float(hi[i] & 0xffff0000u));
+        }
+        *reinterpret_cast<uint4 *>(at + 16 * c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(at + 512 + 16 * c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    __device__ __forceinline__ float load1(int d) const { return __bfloat162float(reinterpret_cast<__nv_bfloat16 *>(at)[d]); }
+    __device__ __forceinline__ void store1(int d, float x) const
+    {
+        const __nv_bfloat16 hi = __float2bfloat16_rn(x);
+        reinterpret_cast<__nv_bfloat16 *>(at)[d] = hi;
+        reinterpret_cast<__nv_bfloat16 *>(at + 512)[d] = __float2bfloat16_rn(x - __bfloat162float(hi));
+    }
+};
+template <> struct PdRow<float> {
+    uint8_t *at;
+    __device__ __forceinline__ void load(int c, float (&x)[8]) const { load8<float>(reinterpret_cast<float *>(at) + 8 * c, x); }
+    __device__ __forceinline__ void store(int c, const float (&x)[8]) const
+    {
+        float4 *to = reinterpret_cast<float4 *>(at + 32 * c);
+        to[0] = make_float4(x[0], x[1], x[2], x[3]);
+        to[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+    __device__ __forceinline__ float load1(int d) const { return reinterpret_cast<float *>(at)[d]; }
+    __device__ __forceinline__ void store1(int d, float x) const { reinterpret_cast<float *>(at)[d] = x; }
 };
 struct PdSmem {
     uint8_t ring[PD_WARPS][PD_STAGES][PD_STAGE];
-    float w1[2][GQA_HD];                    // 1 + q / k norm weights
-    float cs[PD_WARPS][GQA_HD / 2], sn[PD_WARPS][GQA_HD / 2];
+    alignas(16) float w1[2][GQA_HD];        // 1 + q / k norm weights
+    alignas(16) float cs[PD_WARPS][GQA_HD / 2], sn[PD_WARPS][GQA_HD / 2];
     unsigned long long turn[GQA_HD / 2];
     float2 ml[PD_WARPS][2][GQA_GRP];        // (max, sum) of a warp's continued / opened piece
     int4 cont[PD_WARPS], open[PD_WARPS];    // (there: 1, and ends here: 2; request; KV head; parked / last CTA)
@@ -149,20 +310,13 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&out)[PAR
     }
 }
 
-__device__ __forceinline__ float2 pair_of(const __nv_bfloat16 *p)
-{
-    const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-__device__ __forceinline__ float2 pair_of(const float *p) { return *reinterpret_cast<const float2 *>(p); }
-
 template <typename TI>
 __global__ void __launch_bounds__(PD_THREADS, 1)
 pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, GqaPagesArgs p,
                     PagesPart part, const __grid_constant__ RopeFreq f)
 {
     using E = PdEntry<TI>;
-    constexpr int PARTS = E::F32 ? 3 : 2;
+    constexpr int PARTS = E::PARTS;
     extern __shared__ uint8_t smem_raw[];
     PdSmem &sm = *reinterpret_cast<PdSmem *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
@@ -273,7 +427,7 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             const TI *from = static_cast<const TI *>(p.qg) + ((size_t)r * p.H + (u - r * KH) * G + lane) * 2 * GQA_HD + (is_q ? 0 : GQA_HD);
             if (lane == G) from = static_cast<const TI *>(p.k) + (size_t)u * GQA_HD;
             if (lane == G + 1) from = static_cast<const TI *>(p.v) + (size_t)u * GQA_HD;
-            if (lane < n) bulk_load(to + (lane < G ? lane * E::ROW : E::KV + (lane - G) * E::ROW), from, E::BYTES, bar);
+            if (lane < n) bulk_load(to + (!is_q ? lane * E::GROW : lane < G ? lane * E::ROW : E::KV + (lane - G) * E::ROW), from, E::BYTES, bar);
         }
     };
     // ---- entry by entry; each leaves its stage to the one PD_STAGES behind it
@@ -326,70 +480,38 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     pages_rope_table(cs, sn, pos, p.rot, sm.turn, lane, 32);
                 }
                 __syncwarp();
-                // rs: the norm's factor of a row, which the rotation commutes with; lanes 4h .. 4h + 3
-                // hold the quarters of head h's fragments, and all 32 lanes 8 dims each of the new k
-                const int h = lane >> 2, d0 = 2 * (lane & 3), half = p.rot >> 1;
-                const TI *x = reinterpret_cast<const TI *>(st + min(h, G - 1) * E::ROW);
-                const TI *xk = reinterpret_cast<const TI *>(st + E::KV);
-                float s0 = 0.f, s1 = 0.f, sk = 0.f, k[8], val[8];
-#pragma unroll
-                for (int kk = 0; kk < 16; ++kk) {
-                    const float2 a = pair_of(x + 16 * kk + d0), b = pair_of(x + 16 * kk + 8 + d0);
-                    s0 += a.x * a.x + a.y * a.y;
-                    s1 += b.x * b.x + b.y * b.y;
-                }
-                load8<TI>(xk + lane * 8, k);
+                float val[8];
                 load8<TI>(reinterpret_cast<const TI *>(st + E::KV + E::ROW) + lane * 8, val);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sk += k[e] * k[e];
-                s0 += s1;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    if (o < 4) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-                    sk += __shfl_xor_sync(0xffffffffu, sk, o);
+                new_vb = make_uint4(pack_bf16(val[0], val[1]), pack_bf16(val[2], val[3]), pack_bf16(val[4], val[5]), pack_bf16(val[6], val[7]));
+                if (ends) {                 // the row to append
+                    const TI *raw = reinterpret_cast<const TI *>(st + E::KV);
+                    float x[8], w1[8];
+                    load8<TI>(raw + lane * 8, x);
+                    load8<float>(sm.w1[1] + lane * 8, w1);
+                    pages_norm_rope(x, w1, p.eps, p.rot, cs, sn, raw, sm.w1[1], lane);
+                    new_k = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
                 }
-                const float rs = h < G ? 1.f / sqrtf(s0 / GQA_HD + p.eps) : 0.f;    // heads past the group's: q = 0
-                const float rk = 1.f / sqrtf(sk / GQA_HD + p.eps);
-                __syncwarp();               // (fp32: the roped dims take the place of what has been read)
-                float *y = reinterpret_cast<float *>(st + E::Y);
-                for (int j = lane; j < half; j += 32) {
-                    const float c = cs[j], sv = sn[j];
-#pragma unroll 3
-                    for (int row = 0; row < GQA_GRP + 1; ++row) {               // the heads, then k
-                        const TI *in = reinterpret_cast<const TI *>(st + row * E::ROW);
-                        const float *w = sm.w1[row == GQA_GRP];
-                        const float a = to_f32(in[j]) * w[j], b = to_f32(in[j + half]) * w[j + half];
-                        y[row * E::YROW + j] = a * c - b * sv;
-                        y[row * E::YROW + j + half] = b * c + a * sv;
-                    }
-                }
+                // heads past the group's: q = 0 (what lies there is finite or not: cleared, not scaled)
+                for (int j = G * (E::ROW / 16) + lane; j < GQA_GRP * (E::ROW / 16); j += 32)
+                    reinterpret_cast<uint4 *>(st)[j] = make_uint4(0, 0, 0, 0);
                 __syncwarp();
+                pages_norm_rope_quad(PdRow<TI>{st + (lane >> 2) * E::ROW}, lane & 3, sm.w1[0], p.eps, p.rot, cs, sn, true);
 #pragma unroll
                 for (int kk = 0; kk < 16; ++kk)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int d = 16 * kk + 8 * e + d0;
-                        float2 v;
-                        if (d < p.rot) {
-                            v = *reinterpret_cast<const float2 *>(y + h * E::YROW + d);
+                        const uint8_t *from = st + (lane >> 2) * E::ROW + (16 * kk + 8 * e + 2 * (lane & 3)) * (int)sizeof(TI);
+                        if constexpr (E::F32) {
+                            const float2 x = *reinterpret_cast<const float2 *>(from);
+                            uint32_t parts[PARTS];
+                            split_bf16<PARTS>(x.x, x.y, parts);
+#pragma unroll
+                            for (int q = 0; q < PARTS; ++q) qf[q][kk][e] = parts[q];
                         } else {
-                            const float2 w = *reinterpret_cast<const float2 *>(&sm.w1[0][d]);
-                            v = pair_of(x + d);
-                            v.x *= w.x;
-                            v.y *= w.y;
+                            qf[0][kk][e] = *reinterpret_cast<const uint32_t *>(from);
+                            qf[1][kk][e] = *reinterpret_cast<const uint32_t *>(from + 512);
                         }
-                        uint32_t parts[PARTS];
-                        split_bf16<PARTS>(h < G ? v.x * rs : 0.f, h < G ? v.y * rs : 0.f, parts);
-#pragma unroll
-                        for (int q = 0; q < PARTS; ++q) qf[q][kk][e] = parts[q];
                     }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = lane * 8 + e;
-                    k[e] = (d < p.rot ? y[GQA_GRP * E::YROW + d] : k[e] * sm.w1[1][d]) * rk;
-                }
-                new_k = make_uint4(pack_bf16(k[0], k[1]), pack_bf16(k[2], k[3]), pack_bf16(k[4], k[5]), pack_bf16(k[6], k[7]));
-                new_vb = make_uint4(pack_bf16(val[0], val[1]), pack_bf16(val[2], val[3]), pack_bf16(val[4], val[5]), pack_bf16(val[6], val[7]));
 #pragma unroll
                 for (int mt = 0; mt < 16; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
                 m0 = m1 = -INFINITY;
@@ -450,9 +572,9 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 }
                 const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
                 const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-                const float p0 = exp2f(x0 - b0), p1 = exp2f(x1 - b1), p2 = exp2f(x2 - b0), p3 = exp2f(x3 - b1);
+                const float p0 = ex2_approx(x0 - b0), p1 = ex2_approx(x1 - b1), p2 = ex2_approx(x2 - b0), p3 = ex2_approx(x3 - b1);
                 if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-                    const float al0 = exp2f(m0 - b0), al1 = exp2f(m1 - b1);
+                    const float al0 = ex2_approx(m0 - b0), al1 = ex2_approx(m1 - b1);
                     l0 *= al0;
                     l1 *= al1;
 #pragma unroll
@@ -522,10 +644,10 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll 4
                     for (int h = 0; h < GQA_GRP; ++h) {
                         float o[4], g[4];
-                        load4(reinterpret_cast<const TI *>(gate + h * E::ROW) + half * 128, g);
+                        load4(reinterpret_cast<const TI *>(gate + h * E::GROW) + half * 128, g);
                         load4(o_ + h * PD_OROW + 4 * lane, o);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] *= sigmoidf_(g[e]);
+                        for (int e = 0; e < 4; ++e) o[e] *= gate_of(g[e]);
                         if (h < G) store4(out + (size_t)h * GQA_HD + half * 128, o);
                     }
                     __syncwarp();
@@ -571,8 +693,8 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             f0[j] = f1[j] = 0.f;
             if (j >= n) continue;
             const float2 a = sm.ml[from + j][opened && j == 0][h0], b = sm.ml[from + j][opened && j == 0][h0 + 1];
-            f0[j] = a.x == -INFINITY ? 0.f : exp2f(a.x - M0);
-            f1[j] = b.x == -INFINITY ? 0.f : exp2f(b.x - M1);
+            f0[j] = a.x == -INFINITY ? 0.f : ex2_approx(a.x - M0);
+            f1[j] = b.x == -INFINITY ? 0.f : ex2_approx(b.x - M1);
             L0 += a.y * f0[j];
             L1 += b.y * f1[j];
         }
@@ -600,12 +722,12 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 TI *out = static_cast<TI *>(p.ctx) + row * GQA_HD + d;
                 const TI *g = static_cast<const TI *>(p.qg) + row * 2 * GQA_HD + GQA_HD + d;
                 if (h0 < G) {
-                    out[0] = from_f32<TI>(o.x * i0 * sigmoidf_(to_f32(g[0])));
-                    out[8] = from_f32<TI>(o.z * i0 * sigmoidf_(to_f32(g[8])));
+                    out[0] = from_f32<TI>(o.x * i0 * gate_of(to_f32(g[0])));
+                    out[8] = from_f32<TI>(o.z * i0 * gate_of(to_f32(g[8])));
                 }
                 if (h0 + 1 < G) {
-                    out[GQA_HD] = from_f32<TI>(o.y * i1 * sigmoidf_(to_f32(g[2 * GQA_HD])));
-                    out[GQA_HD + 8] = from_f32<TI>(o.w * i1 * sigmoidf_(to_f32(g[2 * GQA_HD + 8])));
+                    out[GQA_HD] = from_f32<TI>(o.y * i1 * gate_of(to_f32(g[2 * GQA_HD])));
+                    out[GQA_HD + 8] = from_f32<TI>(o.w * i1 * gate_of(to_f32(g[2 * GQA_HD + 8])));
                 }
             } else {
                 float *out = part.o + ((size_t)slot * GQA_GRP + h0) * GQA_HD + d;
@@ -658,7 +780,7 @@ pages_join_kernel(GqaPagesArgs p, PagesPart part)
         for (int u = 0; u < U; ++u) {
             if (ml[u].x == -INFINITY) continue;
             const float mn = fmaxf(m, ml[u].x);
-            const float fo = m == -INFINITY ? 0.f : exp2f(m - mn), fs = exp2f(ml[u].x - mn);
+            const float fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fs = ex2_approx(ml[u].x - mn);
             const float v[8] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x, y[u].y, y[u].z, y[u].w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = o[e] * fo + v[e] * fs;
@@ -675,11 +797,11 @@ pages_join_kernel(GqaPagesArgs p, PagesPart part)
     for (int w = 0; w < W; ++w) M = fmaxf(M, sm_ml[w][0]);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-        const float f = sm_ml[w][0] == -INFINITY ? 0.f : exp2f(sm_ml[w][0] - M);
+        const float f = sm_ml[w][0] == -INFINITY ? 0.f : ex2_approx(sm_ml[w][0] - M);
         O += sm_o[w][tid] * f;
         L += sm_ml[w][1] * f;
     }
-    static_cast<TI *>(p.ctx)[row * GQA_HD + tid] = from_f32<TI>(O / L * sigmoidf_(gate));
+    static_cast<TI *>(p.ctx)[row * GQA_HD + tid] = from_f32<TI>(O / L * gate_of(gate));
 }
 
 template <typename TI>
@@ -744,55 +866,14 @@ constexpr int PP_SETUP = 4;                 // a unit's start and end in tiles' 
 constexpr int PP_MIN = PP_SETUP + 2;        // least work of a CTA
 struct PpBars {
     uint64_t q_tmem, k_full[2], k_empty[2], v_full, v_empty, s_full, s_free, p_full, pv_done, g_full, epi_done;
+    unsigned long long turn[GQA_HD / 2];
+    alignas(16) float w1[GQA_HD];           // 1 + q norm weights
     uint32_t tmem_base;
     float lsum[PP_BM];
 };
 constexpr int PP_SMEM = 3 * PP_TILE + PP_P + (int)sizeof(PpBars);
+static_assert(offsetof(PpBars, w1) % 16 == 0 && (3 * PP_TILE + PP_P) % 16 == 0, "16-byte loads");
 static_assert(PP_SMEM <= 232448, "prefill shared memory exceeds the 227 KiB per-CTA limit");
-
-// k / q row in registers, lane = 8 dims: norm and partial RoPE, sums in fp32.
-// vw: 256 floats of this warp, for rotation widths whose half is no multiple of 8.
-__device__ __forceinline__ void pages_norm_rope(float (&y)[8], const float (&x)[8], const float *w, float eps, int rot,
-                                                const float *cs, const float *sn, float *vw, int lane)
-{
-    float s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s2 = fmaf(x[i], x[i], s2);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-    const float rs = 1.f / sqrtf(s2 / GQA_HD + eps);
-    float wv[8];
-    load8<float>(w + lane * 8, wv);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i] * rs * (1.f + wv[i]);
-    const int half = rot >> 1, d0 = lane * 8;
-    if ((half & 7) == 0) {                  // the partner dims are one other lane's
-        const int hl = half >> 3, src = lane < hl ? lane + hl : lane - hl, j = d0 < half ? d0 : d0 - half;
-        float z[8], c[8], sv[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = __shfl_sync(0xffffffffu, y[i], src);
-        if (d0 < rot) {
-            load8<float>(cs + j, c);
-            load8<float>(sn + j, sv);
-            const float sign = d0 < half ? -1.f : 1.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = y[i] * c[i] + sign * z[i] * sv[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vw[d0 + i] = y[i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = d0 + i;
-            if (d < rot) {
-                const int j = d < half ? d : d - half;
-                y[i] = d < half ? y[i] * cs[j] - vw[d + half] * sn[j] : y[i] * cs[j] + vw[j] * sn[j];
-            }
-        }
-        __syncwarp();
-    }
-}
 
 // Tiles of query tile qt of a chunk of n rows at position b.
 __device__ __forceinline__ int pp_tiles(int n, int b, int qt, int tokens)
@@ -800,13 +881,16 @@ __device__ __forceinline__ int pp_tiles(int n, int b, int qt, int tokens)
     return (b + min(n, (qt + 1) * tokens) - 1) / PP_BN + 1;
 }
 // Work of its query tiles before qt (all of them whole): sum over j < qt of
-// floor((a + j) / group) + 1 + PP_SETUP with a = floor((b - 1 + tokens) / tokens).
-__device__ __forceinline__ long long pp_work(int b, int qt, int tokens, int group)
+// floor((a + j) / group) + 1 + PP_SETUP with a = floor((b - 1 + tokens) / tokens),
+// group = 1 << gs, tokens = 128 >> gs.
+__device__ __forceinline__ long long pp_work(int b, int qt, int gs)
 {
-    const long long a = (b - 1 + tokens) / tokens, e = a + qt;
-    const long long ka = a / group, ke = e / group;
-    const long long pa = group * ka * (ka - 1) / 2 + ka * (a - ka * group), pe = group * ke * (ke - 1) / 2 + ke * (e - ke * group);
-    return pe - pa + (long long)qt * (1 + PP_SETUP);
+    auto below = [&](long long m) {         // sum over i < m of floor(i / group)
+        const long long k = m >> gs;
+        return ((k * (k - 1) / 2) << gs) + k * (m - (k << gs));
+    };
+    const long long a = (b - 1 + (PP_BM >> gs)) >> (7 - gs);
+    return below(a + qt) - below(a) + (long long)qt * (1 + PP_SETUP);
 }
 
 constexpr int PL_THREADS = 256;
@@ -834,19 +918,19 @@ template <int NT> __device__ __forceinline__ long long scan64(long long x, long 
 __global__ void __launch_bounds__(PL_THREADS)
 pages_plan_kernel(GqaPagesArgs p, PagesPart part, int ctas, const __grid_constant__ RopeFreq f)
 {
-    __shared__ union {
-        struct { float cs[PL_THREADS / 32][GQA_HD / 2], sn[PL_THREADS / 32][GQA_HD / 2], vw[PL_THREADS / 32][GQA_HD]; } a;
+    __shared__ __align__(16) union {
+        struct { float cs[PL_THREADS / 32][GQA_HD / 2], sn[PL_THREADS / 32][GQA_HD / 2], w1[GQA_HD]; } a;
         long long pre[1024 + 1];
     } sm;
     griddep_launch();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, KH = p.pv.KH, group = p.H / KH, tokens = PP_BM / group;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, KH = p.pv.KH, gs = __ffs(p.H / KH) - 1, tokens = PP_BM >> gs;
     if (blockIdx.x == 0) {
         auto work = [&](int r) {            // of one KV head
             int row0, b;
             const int n = pages_rows_of(p, r, row0, b);
             if (n == 0) return 0ll;
-            const int last = (n - 1) / tokens;
-            return pp_work(b, last, tokens, group) + pp_tiles(n, b, last, tokens) + PP_SETUP;
+            const int last = (n - 1) >> (7 - gs);
+            return pp_work(b, last, gs) + pp_tiles(n, b, last, tokens) + PP_SETUP;
         };
         const int each = (p.n_req + PL_THREADS - 1) / PL_THREADS, r0 = min(p.n_req, tid * each), r1 = min(p.n_req, r0 + each);
         long long mine = 0, total;
@@ -872,19 +956,21 @@ pages_plan_kernel(GqaPagesArgs p, PagesPart part, int ctas, const __grid_constan
                 rel -= u.y * head;
                 int row0, b, q0 = 0;
                 const int n = pages_rows_of(p, lo, row0, b);
-                int q1 = (n - 1) / tokens;
+                int q1 = (n - 1) >> (7 - gs);
                 while (q0 < q1) {           // the last query tile that starts at or before rel
                     const int mid = (q0 + q1 + 1) >> 1;
-                    if (pp_work(b, mid, tokens, group) <= rel) q0 = mid; else q1 = mid - 1;
+                    if (pp_work(b, mid, gs) <= rel) q0 = mid; else q1 = mid - 1;
                 }
                 u.z = q0;
-                u.w = max(0, (int)(rel - pp_work(b, q0, tokens, group)) - PP_SETUP);
+                u.w = max(0, (int)(rel - pp_work(b, q0, gs)) - PP_SETUP);
             }
             part.plan[c] = u;
         }
         return;
     }
-    const int item = (blockIdx.x - 1) * (PL_THREADS / 32) + warp, row = item / KH, kh = item - row * KH;
+    sm.a.w1[tid] = 1.f + p.knw[tid];
+    __syncthreads();
+    const int item = (blockIdx.x - 1) * (PL_THREADS / 32) + warp, row = p.pv.heads_div(item), kh = item - row * KH;
     if (row >= p.S) return;
     int lo = 0, hi = p.n_req - 1, row0, b;
     while (lo < hi) {                       // the last request that starts at or before the row
@@ -894,15 +980,17 @@ pages_plan_kernel(GqaPagesArgs p, PagesPart part, int ctas, const __grid_constan
     if (row < p.cu[lo] || row >= p.cu[lo + 1] || pages_rows_of(p, lo, row0, b) == 0) return;
     const int pos = b + row - row0;
     const size_t in = (size_t)item * GQA_HD + lane * 8;
-    float x[8], y[8], v[8];
-    load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.k) + in, x);
+    float x[8], v[8], w1[8];
+    const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (size_t)item * GQA_HD;
+    load8<float>(sm.a.w1 + lane * 8, w1);
+    load8<__nv_bfloat16>(k + lane * 8, x);
     load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.v) + in, v);
     const long long at = pages_row(p.pv, lo, kh, pos);
     pages_rope_table(sm.a.cs[warp], sm.a.sn[warp], pos, p.rot, f.turn, lane, 32);
     __syncwarp();
-    pages_norm_rope(y, x, p.knw, p.eps, p.rot, sm.a.cs[warp], sm.a.sn[warp], sm.a.vw[warp], lane);
+    pages_norm_rope(x, w1, p.eps, p.rot, sm.a.cs[warp], sm.a.sn[warp], k, sm.a.w1, lane);
     if (at < 0) return;
-    store8(p.pv.k + at * GQA_HD + lane * 8, y);
+    store8(p.pv.k + at * GQA_HD + lane * 8, x);
     store8(p.pv.v + at * GQA_HD + lane * 8, v);
 }
 
@@ -945,6 +1033,21 @@ __device__ __forceinline__ uint64_t pp_desc_k(uint32_t addr)
     return (tc::desc_k_sw128(addr) & ~((uint64_t)0x3FFF << 32)) | (uint64_t)(4096 >> 4) << 32;
 }
 
+// A q row in the V buffer: 16-byte chunk c of row r in 64-column block c / 8, at chunk (c % 8) ^ (r % 8).
+struct PpRow {
+    uint8_t *at;
+    int swz;
+    bool on;                                // off: this pass leaves the row alone
+    __device__ __forceinline__ __nv_bfloat16 *chunk(int c) const
+    {
+        return reinterpret_cast<__nv_bfloat16 *>(at + (c >> 3) * (PP_BM * 128) + (((c & 7) ^ swz) << 4));
+    }
+    __device__ __forceinline__ void load(int c, float (&x)[8]) const { load8<__nv_bfloat16>(chunk(c), x); }
+    __device__ __forceinline__ void store(int c, const float (&x)[8]) const { if (on) store8(chunk(c), x); }
+    __device__ __forceinline__ float load1(int d) const { return __bfloat162float(chunk(d >> 3)[d & 7]); }
+    __device__ __forceinline__ void store1(int d, float x) const { if (on) chunk(d >> 3)[d & 7] = __float2bfloat16_rn(x); }
+};
+
 __global__ void __launch_bounds__(PP_THREADS, 1)
 pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ CUtensorMap tmV8, const __grid_constant__ CUtensorMap tmG, GqaPagesArgs p,
@@ -971,6 +1074,8 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         mbar_init(&bars.g_full, 1); mbar_init(&bars.epi_done, PP_SOFTMAX);
         fence_mbar_init();
     }
+    if (threadIdx.x < p.rot / 2) bars.turn[threadIdx.x] = f.turn[threadIdx.x];
+    if (threadIdx.x < GQA_HD) bars.w1[threadIdx.x] = 1.f + p.qnw[threadIdx.x];
     if (warp == 2) tc::alloc(&bars.tmem_base, 512);
     tc::fence_before();
     __syncthreads();
@@ -987,7 +1092,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         fence_proxy_async_global();         // rows appended by the kernel before, read through the async proxy here
         const int box = p.box_rows, boxes = PP_BN / box, beyond = (int)((long long)p.pv.n_pages * KH * p.pv.page >> 3);
         bool ok = true;
-        int gate_of[2] = {-1, -1}, wholes = 0, pc = 0;
+        int gate_in[2] = {-1, -1}, wholes = 0, pc = 0;
         for (; ok && w.piece(tokens); w.next(p, tokens), ++pc) {
             const int end = w.base + w.n;   // the request's rows
             if (warp == 1) ok = mbar_wait(&bars.q_tmem, pc & 1);   // Q has left the V buffer
@@ -1003,7 +1108,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 }
                 if (warp == 0) {
                     if (jj >= 2) ok = mbar_wait(&bars.k_empty[s], ((jj >> 1) - 1) & 1);
-                    if (ok && gate_of[s] >= 0) { ok = mbar_wait(&bars.epi_done, gate_of[s] & 1); gate_of[s] = -1; }
+                    if (ok && gate_in[s] >= 0) { ok = mbar_wait(&bars.epi_done, gate_in[s] & 1); gate_in[s] = -1; }
                 } else if (jj >= 1) {
                     ok = mbar_wait(&bars.v_empty, (jj - 1) & 1);
                 }
@@ -1026,7 +1131,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         tma_load_3d(sK + s * PP_TILE + c * (PP_BM * 128), &tmG, GQA_HD + 64 * c, w.at.y * group,
                                     w.row0 + w.at.z * tokens, &bars.g_full);
                 }
-                gate_of[s] = wholes++;
+                gate_in[s] = wholes++;
             }
         }
     } else if (warp == 2) {
@@ -1087,33 +1192,36 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         int wholes = 0;
         for (int pc = 0; w.piece(tokens); w.next(p, tokens), ++pc) {
             const int tok0 = w.at.z * tokens, end = w.base + w.n;
-            {   // ---- q: a warp norms and ropes 16 rows (row = token * group + head), through
-                // the V buffer (128B-swizzled 64-column blocks) into TMEM as bf16 pairs
-                float *cs = reinterpret_cast<float *>(sP + sw * 4096), *sn = cs + GQA_HD / 2, *vw = sn + GQA_HD / 2;
-                int known = -1;
-#pragma unroll 1
-                for (int r4 = 0; r4 < 16; r4 += 4) {
-                    Raw8<__nv_bfloat16> raw[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 16 * sw + r4 + i, t = min(tok0 + (r >> gs), w.n - 1);
-                        raw[i].load(qg + ((size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1))) * 2 * GQA_HD + lane * 8);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 16 * sw + r4 + i, t = min(tok0 + (r >> gs), w.n - 1);
-                        if (t != known) {
-                            __syncwarp();
-                            pages_rope_table(cs, sn, w.base + t, p.rot, f.turn, lane, 32);
-                            __syncwarp();
-                            known = t;
-                        }
-                        float x[8], y[8];
-                        raw[i].unpack(x);
-                        pages_norm_rope(y, x, p.qnw, p.eps, p.rot, cs, sn, vw, lane);
-                        store8(reinterpret_cast<__nv_bfloat16 *>(sV + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), y);
-                    }
+            {   // ---- q: a warp copies its 16 rows (row = token * group + head) into the V buffer, in
+                // 128B-swizzled 64-column blocks, norms and ropes them there, and they go to TMEM as
+                // bf16 pairs. Rolled loops: unrolled, fetching the instructions took longer.
+#pragma unroll 4
+                for (int r = 16 * sw; r < 16 * sw + 16; ++r) {
+                    const int t = min(tok0 + (r >> gs), w.n - 1);
+                    copy16_async(sV + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4),
+                                 qg + ((size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1))) * 2 * GQA_HD + lane * 8);
                 }
+                copies_wait();
+                // 8 rows at a time; the angles of their 8 / group (at least one) tokens in the P buffer, of
+                // half of them where all do not fit (8 tokens, rot > 128)
+                const int half = p.rot >> 1, many = max(1, 8 >> gs), fit = many * p.rot > 1024 ? many / 2 : many;
+                float *cs = reinterpret_cast<float *>(sP + sw * 4096), *sn = cs + fit * half;
+                const int rl = ((lane >> 2) & 1) * 4 + (lane >> 3);      // of the 8: lanes of a phase read both halves of the banks
+#pragma unroll 1
+                for (int r8 = 16 * sw; r8 < 16 * sw + 16; r8 += 8)
+#pragma unroll 1
+                    for (int t0 = 0; t0 < many; t0 += fit) {
+                        const int first = (r8 >> gs) + t0;
+                        __syncwarp();
+#pragma unroll 1
+                        for (int i = 0; i < fit; ++i)
+                            pages_rope_table(cs + i * half, sn + i * half, w.base + tok0 + first + i, p.rot, bars.turn, lane, 32);
+                        __syncwarp();
+                        const int r = r8 + rl, mine = (r >> gs) - first;
+                        PpRow row{sV + r * 128, r & 7, mine >= 0 && mine < fit};
+                        const int at = row.on ? mine * half : 0;
+                        pages_norm_rope_quad(row, lane & 3, bars.w1, p.eps, p.rot, cs + at, sn + at, true);
+                    }
                 asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
                 const int row = 32 * quarter + lane;
 #pragma unroll
@@ -1181,7 +1289,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     if (__any_sync(0xffffffffu, need0 || need1)) {
                         mbar_wait(&bars.pv_done, (jj - 1) & 1);        // O complete up to the tile before
                         tc::fence_after();
-                        const float a0 = need0 ? exp2f(m0 - mn0) : 1.f, a1 = need1 ? exp2f(m1 - mn1) : 1.f;
+                        const float a0 = need0 ? ex2_approx(m0 - mn0) : 1.f, a1 = need1 ? ex2_approx(m1 - mn1) : 1.f;
 #pragma unroll 1
                         for (int c = 0; c < GQA_HD / 64; ++c) {
                             float o[32];
@@ -1265,7 +1373,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         float gv[8], y[8];
                         load8v(reinterpret_cast<const __nv_bfloat16 *>(gt + off), gv);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = o[8 * k + e] * inv_l * sigmoidf_(gv[e]);
+                        for (int e = 0; e < 8; ++e) y[e] = o[8 * k + e] * inv_l * gate_of(gv[e]);
                         store8v(reinterpret_cast<__nv_bfloat16 *>(sV + off), y);
                     }
                 }
@@ -1328,7 +1436,7 @@ pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
         const float2 ml = part.ml[slot * PP_BM + row];
         const float4 x = reinterpret_cast<const float4 *>(part.o)[slot * (PP_BM * GQA_HD / 4) + (8 * block + j) * PP_BM + row];
         if (ml.x == -INFINITY) continue;
-        const float mn = fmaxf(m, ml.x), fo = m == -INFINITY ? 0.f : exp2f(m - mn), fs = exp2f(ml.x - mn);
+        const float mn = fmaxf(m, ml.x), fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fs = ex2_approx(ml.x - mn);
         o.x = o.x * fo + x.x * fs; o.y = o.y * fo + x.y * fs; o.z = o.z * fo + x.z * fs; o.w = o.w * fo + x.w * fs;
         l = l * fo + ml.y * fs;
         m = mn;
@@ -1346,7 +1454,7 @@ pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
     float g[4], y[4];
     load4(static_cast<const __nv_bfloat16 *>(p.qg) + at * 2 * GQA_HD + GQA_HD + block * 32 + c, g);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = turned[r][c + e] * sigmoidf_(g[e]);
+    for (int e = 0; e < 4; ++e) y[e] = turned[r][c + e] * gate_of(g[e]);
     store4(static_cast<__nv_bfloat16 *>(p.ctx) + at * GQA_HD + block * 32 + c, y);
 }
 
