@@ -17,6 +17,20 @@ __device__ __forceinline__ uint4 *page_at(const PageMoveArgs &m, int plane, int 
     return reinterpret_cast<uint4 *>(m.base + ((size_t)plane * m.n_pages + id) * m.page_bytes);
 }
 
+// `words` 16-byte words by the CTA's threads, four loads in flight each.
+__device__ __forceinline__ void copy_words(uint4 *to, const uint4 *from, int words)
+{
+    int j = threadIdx.x;
+    for (; j + 3 * MV_THREADS < words; j += 4 * MV_THREADS) {
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __ldcs(from + j + i * MV_THREADS);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) __stcs(to + j + i * MV_THREADS, x[i]);
+    }
+    for (; j < words; j += MV_THREADS) to[j] = from[j];
+}
+
 // ------------------------------------------------------------------ copy
 // One CTA per (pair, plane). A pair is left out when its destination is
 // named by another pair too, or when its source is another pair's
@@ -37,9 +51,7 @@ pages_copy_kernel(PageMoveArgs m, int n, const int *src, const int *dst)
         return;
     }
     if (s == d) return;
-    const uint4 *from = page_at(m, blockIdx.y, s);
-    uint4 *to = page_at(m, blockIdx.y, d);
-    for (int j = threadIdx.x; j < (int)(m.page_bytes / 16); j += MV_THREADS) to[j] = from[j];
+    copy_words(page_at(m, blockIdx.y, d), page_at(m, blockIdx.y, s), (int)(m.page_bytes / 16));
 }
 
 cudaError_t launch_pages_copy(const PageMoveArgs &m, int n, const int *src, const int *dst, cudaStream_t st)
@@ -90,13 +102,11 @@ pages_fork_kernel(PageMoveArgs m, PageForkArgs f)
             f.len[c] = len;
         }
     }
-    const int per = m.page * 32;         // 16-byte words of one head's rows in a page
-    const uint4 *from = tail ? page_at(m, blockIdx.y, from_id) : nullptr;
-    uint4 *to = tail ? page_at(m, blockIdx.y, to_id) : nullptr;
-    for (int j = threadIdx.x; j < m.KH * tail * 32; j += MV_THREADS) {
-        const int kh = j / (tail * 32), at = kh * per + j - kh * tail * 32;
-        to[at] = from[at];
-    }
+    if (tail == 0) return;
+    const size_t per = (size_t)m.page * 32;      // 16-byte words of one head's rows in a page
+    const uint4 *from = page_at(m, blockIdx.y, from_id);
+    uint4 *to = page_at(m, blockIdx.y, to_id);
+    for (int kh = 0; kh < m.KH; ++kh) copy_words(to + kh * per, from + kh * per, tail * 32);
 }
 
 cudaError_t launch_pages_fork(const PageMoveArgs &m, const PageForkArgs &f, cudaStream_t st)
@@ -106,7 +116,7 @@ cudaError_t launch_pages_fork(const PageMoveArgs &m, const PageForkArgs &f, cuda
 }
 
 // ------------------------------------------------------------------ compact
-constexpr int CP_THREADS = 1024;
+constexpr int CP_THREADS = 1024, CP_PIECE = 8 * MV_THREADS, CP_CTAS = 148 * 32;
 
 // Exclusive prefix sum over the CTA's threads; `total` is every thread's sum.
 __device__ __forceinline__ int block_scan(int x, int &total)
@@ -149,6 +159,7 @@ __global__ void __launch_bounds__(CP_THREADS, 1)
 pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
 {
     extern __shared__ uint32_t bits[];
+    griddep_launch();
     const int words = (m.n_pages + 31) / 32, tid = threadIdx.x;
     for (int w = tid; w < words; w += CP_THREADS) bits[w] = 0;
     __syncthreads();
@@ -165,21 +176,19 @@ pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
     int mine = 0, live, holes, movers;
     for (int w = w0; w < w1; ++w) mine += __popc(bits[w]);
     block_scan(mine, live);
+    // of word w: the dead pages before `live`, and the live ones from there on
+    auto low = [&](int w) { return w * 32 + 32 <= live ? ~0u : w * 32 >= live ? 0u : (1u << (live - w * 32)) - 1; };
     int nh = 0, nm = 0;
-    for (int w = w0; w < w1; ++w)
-        for (int b = 0; b < 32 && w * 32 + b < m.n_pages; ++b) {
-            const bool on = bits[w] >> b & 1u, low = w * 32 + b < live;
-            nh += !on && low;
-            nm += on && !low;
-        }
+    for (int w = w0; w < w1; ++w) { nh += __popc(~bits[w] & low(w)); nm += __popc(bits[w] & ~low(w)); }
     int h = block_scan(nh, holes), v = block_scan(nm, movers);
-    for (int w = w0; w < w1; ++w)
-        for (int b = 0; b < 32 && w * 32 + b < m.n_pages; ++b) {
-            const int id = w * 32 + b;
-            const bool on = bits[w] >> b & 1u, low = id < live;
-            if (!on && low) c.dst[h++] = id;
-            if (on && !low) { c.remap[id] = v; c.src[v++] = id; }
+    for (int w = w0; w < w1; ++w) {
+        for (uint32_t x = ~bits[w] & low(w); x; x &= x - 1) c.dst[h++] = w * 32 + __ffs(x) - 1;
+        for (uint32_t x = bits[w] & ~low(w); x; x &= x - 1) {
+            const int id = w * 32 + __ffs(x) - 1;
+            c.remap[id] = v;
+            c.src[v++] = id;
         }
+    }
     if (tid == 0) { *c.count = movers; *c.live = live; }
 }
 
@@ -188,15 +197,21 @@ pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
 __global__ void __launch_bounds__(MV_THREADS)
 pages_compact_move_kernel(PageMoveArgs m, PageCompactArgs c)
 {
-    const int movers = *c.count, live = *c.live, planes = 2 * m.layers;
-    for (int i = blockIdx.x; i < movers * planes; i += gridDim.x) {
-        const int plane = i / movers, k = i - plane * movers;
-        const uint4 *from = page_at(m, plane, c.src[k]);
-        uint4 *to = page_at(m, plane, c.dst[k]);
-        for (int j = threadIdx.x; j < (int)(m.page_bytes / 16); j += MV_THREADS) to[j] = from[j];
+    griddep_wait();                         // a programmatic dependent of the plan
+    const int movers = *c.count, live = *c.live, words = (int)(m.page_bytes / 16);
+    // blockIdx.y: a plane and a piece of the page; blockIdx.x and on: the movers, the next one's ids ahead
+    const int pieces = (words + CP_PIECE - 1) / CP_PIECE, plane = blockIdx.y / pieces, at = (blockIdx.y - plane * pieces) * CP_PIECE;
+    int k = blockIdx.x, from = k < movers ? c.src[k] : 0, to = k < movers ? c.dst[k] : 0;
+    while (k < movers) {
+        k += gridDim.x;
+        const int next_from = k < movers ? c.src[k] : 0, next_to = k < movers ? c.dst[k] : 0;
+        copy_words(page_at(m, plane, to) + at, page_at(m, plane, from) + at, min(CP_PIECE, words - at));
+        from = next_from;
+        to = next_to;
     }
     const long long cells = (long long)c.n_req * c.max_pages;
-    for (long long i = blockIdx.x * (long long)MV_THREADS + threadIdx.x; i < cells; i += (long long)gridDim.x * MV_THREADS) {
+    const long long first = (blockIdx.y * (long long)gridDim.x + blockIdx.x) * MV_THREADS + threadIdx.x;
+    for (long long i = first; i < cells; i += (long long)gridDim.x * gridDim.y * MV_THREADS) {
         const int r = (int)(i / c.max_pages), j = (int)(i - (long long)r * c.max_pages);
         int id = c.table[i];
         if (j < pages_held(m, c, r) && id >= live && id < m.n_pages) id = c.dst[c.remap[id]];
@@ -212,8 +227,13 @@ cudaError_t launch_pages_compact(const PageMoveArgs &m, const PageCompactArgs &c
     pages_compact_plan_kernel<<<1, CP_THREADS, smem, st>>>(m, c);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    pages_compact_move_kernel<<<148 * 8, MV_THREADS, 0, st>>>(m, c);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    const int words = (int)(m.page_bytes / 16), rows = 2 * m.layers * ((words + CP_PIECE - 1) / CP_PIECE);
+    cfg.gridDim = dim3(std::max(1, std::min(m.n_pages, (CP_CTAS + rows - 1) / rows)), rows); cfg.blockDim = dim3(MV_THREADS); cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, pages_compact_move_kernel, m, c);
 }
 
 }  // namespace coli
