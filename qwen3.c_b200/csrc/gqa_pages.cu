@@ -838,9 +838,11 @@ cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, co
 // long context are spread over the GPU. A piece of a unit leaves its O, max and sum in the
 // workspace, and pages_prefill_join_kernel merges them (two at most per CTA).
 //
-//   pages_plan_kernel     block 0 lays the ranges out; the others norm, rope and
-//                         append k (and v), a warp per (row, KV head)
-//   pages_prefill_kernel  tcgen05, 352 threads:
+//   pages_append_kernel   k normed, roped and appended with v, a warp per (row, KV
+//                         head); the next kernel starts beside it, and its loads of
+//                         tiles that hold new rows wait for it
+//   pages_prefill_kernel  each CTA lays out its range from the chunks' sizes; tcgen05,
+//                         352 threads:
 //     warp 0      K tiles into a 2-stage ring, up to 8 TMA boxes of whole pages
 //                 each (a lane per box, its page id looked up there), and the gate
 //                 tile into the stage that the piece's last K tile leaves
@@ -862,12 +864,13 @@ cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, co
 constexpr int PP_BM = 128, PP_BN = 128;
 constexpr int PP_TILE = PP_BN * GQA_HD * 2, PP_P = PP_BM * PP_BN * 2;
 constexpr int PP_SOFTMAX = 256, PP_THREADS = 96 + PP_SOFTMAX;
-constexpr int PP_SETUP = 4;                 // a unit's start and end in tiles' time
-constexpr int PP_MIN = PP_SETUP + 2;        // least work of a CTA
+constexpr int PP_SETUP = 7;                 // a unit's start and end in tiles' time (4: 5-15 % slower, 9 and 12: 1-4 %)
+constexpr int PP_MIN = 4;                   // least work of a CTA
 struct PpBars {
     uint64_t q_tmem, k_full[2], k_empty[2], v_full, v_empty, s_full, s_free, p_full, pv_done, g_full, epi_done;
     unsigned long long turn[GQA_HD / 2];
     alignas(16) float w1[GQA_HD];           // 1 + q norm weights
+    int4 range[2];
     uint32_t tmem_base;
     float lsum[PP_BM];
 };
@@ -893,85 +896,85 @@ __device__ __forceinline__ long long pp_work(int b, int qt, int gs)
     return below(a + qt) - below(a) + (long long)qt * (1 + PP_SETUP);
 }
 
-constexpr int PL_THREADS = 256;
-template <int NT> __device__ __forceinline__ long long scan64(long long x, long long &total)   // exclusive, over the CTA
+// Work of request r's chunk for one KV head.
+__device__ __forceinline__ long long pp_chunk_work(const GqaPagesArgs &p, int r, int gs)
 {
-    __shared__ long long part[NT / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long inc = x;
+    int row0, b;
+    const int n = pages_rows_of(p, r, row0, b);
+    if (n == 0) return 0;
+    const int last = (n - 1) >> (7 - gs);
+    return pp_work(b, last, gs) + pp_tiles(n, b, last, PP_BM >> gs) + PP_SETUP;
+}
+
+// Where the ranges of CTAs cta and cta + 1 start, (request, KV head, query
+// tile, key tile), into range[0] and range[1]; `scratch` 8 KiB + 256 of shared
+// memory, all threads of the CTA.
+__device__ __forceinline__ void pp_plan(const GqaPagesArgs &p, int cta, int ctas, int gs, void *scratch, int4 *range)
+{
+    long long *pre = static_cast<long long *>(scratch), *sums = pre + 1024 + 8;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, KH = p.pv.KH;
+    const int each = (p.n_req + PP_THREADS - 1) / PP_THREADS, r0 = min(p.n_req, tid * each), r1 = min(p.n_req, r0 + each);
+    long long mine = 0;
+#pragma unroll 1
+    for (int r = r0; r < r1; ++r) mine += pp_chunk_work(p, r, gs);
+    long long inc = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, inc, d);
         if (lane >= d) inc += y;
     }
-    if (lane == 31) part[warp] = inc;
+    if (lane == 31) sums[warp] = inc;
     __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) before += part[w];
-        all += part[w];
+    long long at = inc - mine;
+    for (int w = 0; w < warp; ++w) at += sums[w];
+#pragma unroll 1
+    for (int r = r0; r < r1; ++r) { pre[r] = at; at += pp_chunk_work(p, r, gs); }
+    if (tid == PP_THREADS - 1) pre[p.n_req] = at;
+    __syncthreads();
+    if (tid < 2) {
+        const long long all = pre[p.n_req] * KH, per = max((long long)PP_MIN, (all + ctas - 1) / ctas), v = (cta + tid) * per;
+        int4 u = make_int4(p.n_req, 0, 0, 0);
+        if (v < all) {
+            int lo = 0, hi = p.n_req - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (pre[mid] * KH <= v) lo = mid; else hi = mid - 1;
+            }
+            const long long head = pre[lo + 1] - pre[lo];
+            long long rel = v - pre[lo] * KH;
+            u.x = lo;
+            u.y = (int)(rel / head);
+            rel -= u.y * head;
+            int row0, b, q0 = 0;
+            const int n = pages_rows_of(p, lo, row0, b);
+            int q1 = (n - 1) >> (7 - gs);
+            while (q0 < q1) {               // the last query tile that starts at or before rel
+                const int mid = (q0 + q1 + 1) >> 1;
+                if (pp_work(b, mid, gs) <= rel) q0 = mid; else q1 = mid - 1;
+            }
+            u.z = q0;
+            u.w = max(0, (int)(rel - pp_work(b, q0, gs)) - PP_SETUP);
+        }
+        range[tid] = u;
     }
-    total = all;
-    return before + inc - x;
+    __syncthreads();
 }
 
-__global__ void __launch_bounds__(PL_THREADS)
-pages_plan_kernel(GqaPagesArgs p, PagesPart part, int ctas, const __grid_constant__ RopeFreq f)
+constexpr int PA_WARPS = 8;
+__global__ void __launch_bounds__(PA_WARPS * 32)
+pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
 {
-    __shared__ __align__(16) union {
-        struct { float cs[PL_THREADS / 32][GQA_HD / 2], sn[PL_THREADS / 32][GQA_HD / 2], w1[GQA_HD]; } a;
-        long long pre[1024 + 1];
-    } sm;
-    griddep_launch();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, KH = p.pv.KH, gs = __ffs(p.H / KH) - 1, tokens = PP_BM >> gs;
-    if (blockIdx.x == 0) {
-        auto work = [&](int r) {            // of one KV head
-            int row0, b;
-            const int n = pages_rows_of(p, r, row0, b);
-            if (n == 0) return 0ll;
-            const int last = (n - 1) >> (7 - gs);
-            return pp_work(b, last, gs) + pp_tiles(n, b, last, tokens) + PP_SETUP;
-        };
-        const int each = (p.n_req + PL_THREADS - 1) / PL_THREADS, r0 = min(p.n_req, tid * each), r1 = min(p.n_req, r0 + each);
-        long long mine = 0, total;
-        for (int r = r0; r < r1; ++r) mine += work(r);
-        long long at = scan64<PL_THREADS>(mine, total);
-        for (int r = r0; r < r1; ++r) { sm.pre[r] = at; at += work(r); }
-        if (tid == 0) sm.pre[p.n_req] = total;
-        __syncthreads();
-        const long long all = total * KH, per = max((long long)PP_MIN, (all + ctas - 1) / ctas);
-        for (int c = tid; c <= ctas; c += PL_THREADS) {
-            const long long v = c * per;
-            int4 u = make_int4(p.n_req, 0, 0, 0);               // (request, KV head, query tile, key tile)
-            if (v < all) {
-                int lo = 0, hi = p.n_req - 1;
-                while (lo < hi) {
-                    const int mid = (lo + hi + 1) >> 1;
-                    if (sm.pre[mid] * KH <= v) lo = mid; else hi = mid - 1;
-                }
-                const long long head = sm.pre[lo + 1] - sm.pre[lo];
-                long long rel = v - sm.pre[lo] * KH;
-                u.x = lo;
-                u.y = (int)(rel / head);
-                rel -= u.y * head;
-                int row0, b, q0 = 0;
-                const int n = pages_rows_of(p, lo, row0, b);
-                int q1 = (n - 1) >> (7 - gs);
-                while (q0 < q1) {           // the last query tile that starts at or before rel
-                    const int mid = (q0 + q1 + 1) >> 1;
-                    if (pp_work(b, mid, gs) <= rel) q0 = mid; else q1 = mid - 1;
-                }
-                u.z = q0;
-                u.w = max(0, (int)(rel - pp_work(b, q0, gs)) - PP_SETUP);
-            }
-            part.plan[c] = u;
-        }
-        return;
-    }
-    sm.a.w1[tid] = 1.f + p.knw[tid];
+    __shared__ __align__(16) float cs[PA_WARPS][GQA_HD / 2], sn[PA_WARPS][GQA_HD / 2], w1s[GQA_HD];
+    griddep_launch();                       // the attention starts now; what reads appended rows waits
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, KH = p.pv.KH;
+    w1s[tid] = 1.f + p.knw[tid];
     __syncthreads();
-    const int item = (blockIdx.x - 1) * (PL_THREADS / 32) + warp, row = p.pv.heads_div(item), kh = item - row * KH;
+    const int item = blockIdx.x * PA_WARPS + warp, row = p.pv.heads_div(item), kh = item - row * KH;
     if (row >= p.S) return;
+    const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (size_t)item * GQA_HD;
+    float x[8], v[8], w1[8];
+    load8<__nv_bfloat16>(k + lane * 8, x);
+    load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.v) + (size_t)item * GQA_HD + lane * 8, v);
     int lo = 0, hi = p.n_req - 1, row0, b;
     while (lo < hi) {                       // the last request that starts at or before the row
         const int mid = (lo + hi + 1) >> 1;
@@ -979,16 +982,11 @@ pages_plan_kernel(GqaPagesArgs p, PagesPart part, int ctas, const __grid_constan
     }
     if (row < p.cu[lo] || row >= p.cu[lo + 1] || pages_rows_of(p, lo, row0, b) == 0) return;
     const int pos = b + row - row0;
-    const size_t in = (size_t)item * GQA_HD + lane * 8;
-    float x[8], v[8], w1[8];
-    const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (size_t)item * GQA_HD;
-    load8<float>(sm.a.w1 + lane * 8, w1);
-    load8<__nv_bfloat16>(k + lane * 8, x);
-    load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.v) + in, v);
     const long long at = pages_row(p.pv, lo, kh, pos);
-    pages_rope_table(sm.a.cs[warp], sm.a.sn[warp], pos, p.rot, f.turn, lane, 32);
+    pages_rope_table(cs[warp], sn[warp], pos, p.rot, f.turn, lane, 32);
     __syncwarp();
-    pages_norm_rope(x, w1, p.eps, p.rot, sm.a.cs[warp], sm.a.sn[warp], k, sm.a.w1, lane);
+    load8<float>(w1s + lane * 8, w1);
+    pages_norm_rope(x, w1, p.eps, p.rot, cs[warp], sn[warp], k, w1s, lane);
     if (at < 0) return;
     store8(p.pv.k + at * GQA_HD + lane * 8, x);
     store8(p.pv.v + at * GQA_HD + lane * 8, v);
@@ -999,10 +997,10 @@ struct PpWalk {
     int4 at, stop;
     int n, row0, base, nt, t1;              // of the piece in work: rows, first row, first position, tiles, end tile
     bool ends;
-    __device__ __forceinline__ PpWalk(const GqaPagesArgs &p, const PagesPart &part, int cta)
+    __device__ __forceinline__ PpWalk(const GqaPagesArgs &p, const int4 *range)
     {
-        at = part.plan[cta];
-        stop = part.plan[cta + 1];
+        at = range[0];
+        stop = range[1];
         n = at.x < p.n_req ? pages_rows_of(p, at.x, row0, base) : 0;
     }
     __device__ __forceinline__ bool piece(int tokens)
@@ -1077,21 +1075,22 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     if (threadIdx.x < p.rot / 2) bars.turn[threadIdx.x] = f.turn[threadIdx.x];
     if (threadIdx.x < GQA_HD) bars.w1[threadIdx.x] = 1.f + p.qnw[threadIdx.x];
     if (warp == 2) tc::alloc(&bars.tmem_base, 512);
+    pp_plan(p, cta, gridDim.x, gs, sP, bars.range);   // (its barriers order the set-up above, too)
+    if (threadIdx.x < 2) part.plan[cta + threadIdx.x] = bars.range[threadIdx.x];   // for the join
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tbase = bars.tmem_base;
     const uint32_t tS = tbase, tO = tbase + 128, tQ = tbase + 384;
-    griddep_wait();                         // the plan and the appended rows
-    PpWalk w(p, part, cta);
+    PpWalk w(p, bars.range);
     int jj = 0;                             // key tiles of this CTA so far
 
     if (warp < 2) {
         // ------------------------------------------------ TMA producers (a lane per box)
         if (lane == 0) { tma_prefetch_desc(warp ? &tmV : &tmK); tma_prefetch_desc(warp ? &tmV8 : &tmG); }
-        fence_proxy_async_global();         // rows appended by the kernel before, read through the async proxy here
         const int box = p.box_rows, boxes = PP_BN / box, beyond = (int)((long long)p.pv.n_pages * KH * p.pv.page >> 3);
         bool ok = true;
+        bool appended = false;              // .. the rows that the kernel before appends are visible
         int gate_in[2] = {-1, -1}, wholes = 0, pc = 0;
         for (; ok && w.piece(tokens); w.next(p, tokens), ++pc) {
             const int end = w.base + w.n;   // the request's rows
@@ -1099,6 +1098,11 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             for (int j = w.at.w; ok && j < w.t1; ++j, ++jj) {
                 const int s = jj & 1;
                 // a lane's box: `rows` of them from key `key`; 8-row boxes where V ends inside the tile
+                if (!appended && (j + 1) * PP_BN > w.base) {
+                    griddep_wait();
+                    fence_proxy_async_global();     // written by plain stores, read through the async proxy
+                    appended = true;
+                }
                 const bool tail = warp == 1 && (j + 1) * PP_BN > end;
                 const int rows = tail ? 8 : box, key = j * PP_BN + lane * rows, n_box = tail ? PP_BN / 8 : boxes;
                 int at = beyond;
@@ -1411,6 +1415,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         tc::fence_after();
         tc::dealloc(tbase, 512);
     }
+    griddep_wait();                         // this grid ends after the one before, also where no tile waited for it
 }
 
 // One CTA per (first CTA of a split unit, 32 rows, 32 dims): adds the pieces
@@ -1463,8 +1468,7 @@ cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, c
 {
     cudaError_t e = cudaFuncSetAttribute(pages_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PP_SMEM);
     if (e != cudaSuccess) return e;
-    const int rows_per = PL_THREADS / 32;
-    pages_plan_kernel<<<1 + (int)(((long long)a.S * a.pv.KH + rows_per - 1) / rows_per), PL_THREADS, 0, st>>>(a, part, ctas, f);
+    pages_append_kernel<<<(int)(((long long)a.S * a.pv.KH + PA_WARPS - 1) / PA_WARPS), PA_WARPS * 32, 0, st>>>(a, f);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
