@@ -23,13 +23,15 @@ __device__ __forceinline__ void pages_error(int code) { atomicCAS(&g_pages_error
 
 // Angle table of position pos, entries [0, rot / 2): the angle in turns is the
 // fraction of an exact 64-bit product, so far positions lose nothing.
+__device__ __forceinline__ void pages_rope_entry(float *cs, float *sn, int pos, unsigned long long turn)
+{
+    const int top = (int)(((unsigned long long)pos * turn) >> 32);             // 2^-32 turns, [-1/2, 1/2)
+    sincospif((float)top * 4.656612873077393e-10f, sn, cs);                    // 2^-31: in half turns
+}
 __device__ __forceinline__ void pages_rope_table(float *cs, float *sn, int pos, int rot, const unsigned long long *turn,
                                                  int tid0, int nthr)
 {
-    for (int j = tid0; j < (rot >> 1); j += nthr) {
-        const int top = (int)(((unsigned long long)pos * turn[j]) >> 32);      // 2^-32 turns, [-1/2, 1/2)
-        sincospif((float)top * 4.656612873077393e-10f, &sn[j], &cs[j]);        // 2^-31: in half turns
-    }
+    for (int j = tid0; j < (rot >> 1); j += nthr) pages_rope_entry(cs + j, sn + j, pos, turn[j]);
 }
 
 // Scalars of these kernels. The IEEE division and square root are long
@@ -120,33 +122,34 @@ __device__ __forceinline__ void pages_norm_rope(float (&x)[8], const float (&w1)
     }
 }
 
-// Eight rows at once, four lanes (q = lane % 4) each: norm and partial RoPE of
-// rows in shared memory, in place. A row gives its 8-dim chunk c (load / store) and
-// single dims (load1 / store1); chunks go round the four lanes, and a rotated
-// pair of chunks is one lane's, so nothing is overwritten before it is read.
-// A quarter of the instructions of a row per warp, and two shuffles instead of 13.
-template <typename Row>
-__device__ __forceinline__ void pages_norm_rope_quad(const Row &row, int q, const float *w1, float eps, int rot, const float *cs,
-                                                     const float *sn, bool on)
+// 32 / LANES rows at once, LANES lanes (q = lane % LANES) each: norm and partial
+// RoPE of rows in shared memory, in place. A row gives its 8-dim chunk c (load /
+// store) and single dims (load1 / store1); chunks go round the row's lanes, and a
+// rotated pair of chunks is one lane's, so nothing is overwritten before it is
+// read. A row on all 32 lanes takes 13 shuffles in a chain, 850 cycles; eight rows
+// on four lanes each take about 2000 together.
+template <int LANES, typename Row>
+__device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, const float *w1, float eps, int rot, const float *cs,
+                                                     const float *sn)
 {
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < GQA_HD / 8 / LANES; ++k) {
         float x[8];
-        row.load(4 * k + q, x);
+        row.load(LANES * k + q, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { s0 = fmaf(x[i], x[i], s0); s1 = fmaf(x[4 + i], x[4 + i], s1); }
     }
     s0 += s1;
-    s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
-    s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
-    const float rs = on ? rms_factor(s0, eps) : 0.f;
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    const float rs = rms_factor(s0, eps);
     __syncwarp();
     const int half = rot >> 1;
     if ((half & 7) == 0) {
         const int hc = half >> 3;
 #pragma unroll 1
-        for (int c = q; c < hc; c += 4) {
+        for (int c = q; c < hc; c += LANES) {
             float a[8], b[8], wa[8], wb[8], co[8], si[8];
             row.load(c, a);
             row.load(c + hc, b);
@@ -164,7 +167,7 @@ __device__ __forceinline__ void pages_norm_rope_quad(const Row &row, int q, cons
             row.store(c + hc, b);
         }
 #pragma unroll 3
-        for (int c = (rot >> 3) + q; c < GQA_HD / 8; c += 4) {
+        for (int c = (rot >> 3) + q; c < GQA_HD / 8; c += LANES) {
             float a[8], wa[8];
             row.load(c, a);
             load8<float>(w1 + 8 * c, wa);
@@ -174,13 +177,13 @@ __device__ __forceinline__ void pages_norm_rope_quad(const Row &row, int q, cons
         }
     } else {
 #pragma unroll 1
-        for (int j = q; j < half; j += 4) {
+        for (int j = q; j < half; j += LANES) {
             const float x = row.load1(j) * w1[j] * rs, y = row.load1(j + half) * w1[j + half] * rs;
             row.store1(j, x * cs[j] - y * sn[j]);
             row.store1(j + half, y * cs[j] + x * sn[j]);
         }
 #pragma unroll 1
-        for (int d = rot + q; d < GQA_HD; d += 4) row.store1(d, row.load1(d) * w1[d] * rs);
+        for (int d = rot + q; d < GQA_HD; d += LANES) row.store1(d, row.load1(d) * w1[d] * rs);
     }
     __syncwarp();
 }
@@ -495,7 +498,7 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 for (int j = G * (E::ROW / 16) + lane; j < GQA_GRP * (E::ROW / 16); j += 32)
                     reinterpret_cast<uint4 *>(st)[j] = make_uint4(0, 0, 0, 0);
                 __syncwarp();
-                pages_norm_rope_quad(PdRow<TI>{st + (lane >> 2) * E::ROW}, lane & 3, sm.w1[0], p.eps, p.rot, cs, sn, true);
+                pages_norm_rope_rows<4>(PdRow<TI>{st + (lane >> 2) * E::ROW}, lane & 3, sm.w1[0], p.eps, p.rot, cs, sn);
 #pragma unroll
                 for (int kk = 0; kk < 16; ++kk)
 #pragma unroll
@@ -1194,58 +1197,61 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const float sl2 = p.scale_log2;
         const __nv_bfloat16 *qg = static_cast<const __nv_bfloat16 *>(p.qg);
         int wholes = 0;
-        for (int pc = 0; w.piece(tokens); w.next(p, tokens), ++pc) {
-            const int tok0 = w.at.z * tokens, end = w.base + w.n;
-            {   // ---- q: a warp copies its 16 rows (row = token * group + head) into the V buffer, in
-                // 128B-swizzled 64-column blocks, norms and ropes them there, and they go to TMEM as
-                // bf16 pairs. Rolled loops: unrolled, fetching the instructions took longer.
+        // ---- q of piece x: a warp copies its 16 rows (row = token * group + head) into the V buffer, in
+        // 128B-swizzled 64-column blocks, norms and ropes them there, and they go to TMEM as bf16
+        // pairs. The V buffer and Q's columns are free: the piece before has done its last product.
+        auto load_q = [&](const PpWalk &x) {
+            const int t_first = x.at.z * tokens;
 #pragma unroll 4
-                for (int r = 16 * sw; r < 16 * sw + 16; ++r) {
-                    const int t = min(tok0 + (r >> gs), w.n - 1);
-                    copy16_async(sV + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4),
-                                 qg + ((size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1))) * 2 * GQA_HD + lane * 8);
-                }
-                copies_wait();
-                // 8 rows at a time; the angles of their 8 / group (at least one) tokens in the P buffer, of
-                // half of them where all do not fit (8 tokens, rot > 128)
-                const int half = p.rot >> 1, many = max(1, 8 >> gs), fit = many * p.rot > 1024 ? many / 2 : many;
-                float *cs = reinterpret_cast<float *>(sP + sw * 4096), *sn = cs + fit * half;
-                const int rl = ((lane >> 2) & 1) * 4 + (lane >> 3);      // of the 8: lanes of a phase read both halves of the banks
-#pragma unroll 1
-                for (int r8 = 16 * sw; r8 < 16 * sw + 16; r8 += 8)
-#pragma unroll 1
-                    for (int t0 = 0; t0 < many; t0 += fit) {
-                        const int first = (r8 >> gs) + t0;
-                        __syncwarp();
-#pragma unroll 1
-                        for (int i = 0; i < fit; ++i)
-                            pages_rope_table(cs + i * half, sn + i * half, w.base + tok0 + first + i, p.rot, bars.turn, lane, 32);
-                        __syncwarp();
-                        const int r = r8 + rl, mine = (r >> gs) - first;
-                        PpRow row{sV + r * 128, r & 7, mine >= 0 && mine < fit};
-                        const int at = row.on ? mine * half : 0;
-                        pages_norm_rope_quad(row, lane & 3, bars.w1, p.eps, p.rot, cs + at, sn + at, true);
-                    }
-                asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
-                const int row = 32 * quarter + lane;
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                    float v[32];
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const int d = 128 * u + 64 * hh + 8 * c;
-                        const uint4 x = *reinterpret_cast<const uint4 *>(
-                            sV + (d >> 6) * (PP_BM * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4));
-                        v[4 * c] = __uint_as_float(x.x); v[4 * c + 1] = __uint_as_float(x.y);
-                        v[4 * c + 2] = __uint_as_float(x.z); v[4 * c + 3] = __uint_as_float(x.w);
-                    }
-                    tc::st32(tQ + 64 * u + 32 * hh + ((uint32_t)(32 * quarter) << 16), v);
-                }
-                tc::wait_st();
-                tc::fence_before();
-                fence_proxy_async();        // what was written and read here before V tiles land in its place
-                mbar_arrive(&bars.q_tmem);
+            for (int r = 16 * sw; r < 16 * sw + 16; ++r) {
+                const int t = min(t_first + (r >> gs), x.n - 1);
+                copy16_async(sV + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4),
+                             qg + ((size_t)(x.row0 + t) * p.H + x.at.y * group + (r & (group - 1))) * 2 * GQA_HD + lane * 8);
             }
+            // the angles of the warp's 16 / group (at least one) tokens in the P buffer, `fit` tokens at a time
+            const int half = p.rot >> 1, many = max(1, 16 >> gs), fit = min(many, 1024 / p.rot);
+            float *cs = reinterpret_cast<float *>(sP + sw * 4096), *sn = cs + fit * half;
+            const int r = 16 * sw + (lane >> 4) * 8 + ((lane >> 3) & 1) + 2 * ((lane >> 1) & 3);   // lanes of a phase: all banks
+#pragma unroll 1
+            for (int t0 = 0; t0 < many; t0 += fit) {
+                const int first = t_first + ((16 * sw) >> gs) + t0;
+                __syncwarp();
+#pragma unroll 1
+                for (int i = lane; i < fit * half; i += 32) {
+                    const int t = i / half;
+                    pages_rope_entry(cs + i, sn + i, x.base + first + t, bars.turn[i - t * half]);
+                }
+                if (t0 == 0) copies_wait();
+                __syncwarp();
+                const int mine = t_first + (r >> gs) - first;
+                PpRow row{sV + r * 128, r & 7, mine >= 0 && mine < fit};
+                const int at = row.on ? mine * half : 0;
+                pages_norm_rope_rows<2>(row, lane & 1, bars.w1, p.eps, p.rot, cs + at, sn + at);
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
+            const int tr = 32 * quarter + lane;
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const int d = 128 * u + 64 * hh + 8 * c;
+                    const uint4 y = *reinterpret_cast<const uint4 *>(
+                        sV + (d >> 6) * (PP_BM * 128) + tr * 128 + ((((d & 63) >> 3) ^ (tr & 7)) << 4));
+                    v[4 * c] = __uint_as_float(y.x); v[4 * c + 1] = __uint_as_float(y.y);
+                    v[4 * c + 2] = __uint_as_float(y.z); v[4 * c + 3] = __uint_as_float(y.w);
+                }
+                tc::st32(tQ + 64 * u + 32 * hh + ((uint32_t)(32 * quarter) << 16), v);
+            }
+            tc::wait_st();
+            tc::fence_before();
+            fence_proxy_async();            // what was written and read here before V tiles land in its place
+            mbar_arrive(&bars.q_tmem);
+        };
+        bool more = w.piece(tokens);
+        if (more) load_q(w);
+        while (more) {
+            const int tok0 = w.at.z * tokens, end = w.base + w.n;
             const int qpos0 = w.base + tok0 + (row0 >> gs), qpos1 = w.base + tok0 + (row1 >> gs);
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
             for (int i = w.at.w; i < w.t1; ++i, ++jj) {
@@ -1356,13 +1362,18 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
             mbar_wait(&bars.pv_done, (jj - 1) & 1);
             tc::fence_after();
+            // the next piece's q first: its S runs during this epilogue
+            PpWalk nx = w;
+            nx.next(p, tokens);
+            more = nx.piece(tokens);
+            if (more) load_q(nx);
             const int row = 32 * quarter + lane;
             const uint32_t qoff = (uint32_t)(32 * quarter) << 16;
             if (whole) {
-                // thread = tile row, O columns 128 u ..; gate and staged ctx share the
-                // layout of 128B-swizzled 64 x 128 boxes; then a warp per row to memory
+                // thread = tile row, O columns 128 u ..; ctx takes the gate's place in its
+                // 128B-swizzled 64 x 128 boxes; then a warp per row to memory
                 const float inv_l = 1.f / bars.lsum[row];
-                const uint8_t *gt = sK + ((jj - 1) & 1) * PP_TILE;
+                uint8_t *gt = sK + ((jj - 1) & 1) * PP_TILE;
                 mbar_wait(&bars.g_full, wholes++ & 1);
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -1378,20 +1389,20 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         load8v(reinterpret_cast<const __nv_bfloat16 *>(gt + off), gv);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[e] = o[8 * k + e] * inv_l * gate_of(gv[e]);
-                        store8v(reinterpret_cast<__nv_bfloat16 *>(sV + off), y);
+                        store8v(reinterpret_cast<__nv_bfloat16 *>(gt + off), y);
                     }
                 }
-                fence_proxy_async();        // the gate has been read: its stage takes K tiles again
-                mbar_arrive(&bars.epi_done);
                 asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
 #pragma unroll 4
                 for (int i = 0; i < 16; ++i) {
                     const int r = 16 * sw + i, t = tok0 + (r >> gs);
                     if (t >= w.n) break;
-                    const uint4 x = *reinterpret_cast<const uint4 *>(sV + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                    const uint4 x = *reinterpret_cast<const uint4 *>(gt + (lane >> 3) * (PP_BM * 128) + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
                     *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.ctx) +
                                                ((size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1))) * GQA_HD + lane * 8) = x;
                 }
+                fence_proxy_async();        // read out: the stage takes K tiles again
+                mbar_arrive(&bars.epi_done);
             } else {
                 // O as it is, [16-byte column chunk][row]: a warp writes 512 bytes at a time
                 float4 *out = reinterpret_cast<float4 *>(part.o) + slot * (PP_BM * GQA_HD / 4) + quarter * 32 + lane;
@@ -1405,8 +1416,8 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         out[(32 * u + 8 * c + j) * PP_BM] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                 }
             }
-            tc::fence_before();             // O read: the next piece's products overwrite it
-            asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
+            tc::fence_before();             // O read: the next piece's products overwrite it (behind p_full)
+            w = nx;
         }
     }
     tc::fence_before();
