@@ -197,8 +197,8 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
 //
 // A warp works on its own. Everything it reads comes through its own 3-stage
 // ring of 16 KiB (mbarrier completion), which runs on across units, so that no
-// unit waits for its own loads: tiles as one TMA box of K and one of V, q and
-// gate rows as bulk copies. 32 entries are looked up at once by the 32 lanes, a
+// unit waits for its own loads: a tile's K and V as one TMA box, q and gate rows
+// as bulk copies. 32 entries are looked up at once by the 32 lanes, a
 // batch ahead of their use. The warp norms and ropes q, and writes the ctx of
 // a unit that it holds whole. What warps of one CTA share of a unit is merged
 // in shared memory when the ranges are done; what CTAs share goes through the
@@ -315,8 +315,7 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&out)[PAR
 
 template <typename TI>
 __global__ void __launch_bounds__(PD_THREADS, 1)
-pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, GqaPagesArgs p,
-                    PagesPart part, const __grid_constant__ RopeFreq f)
+pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ RopeFreq f)
 {
     using E = PdEntry<TI>;
     constexpr int PARTS = E::PARTS;
@@ -325,39 +324,43 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
     const int KH = p.pv.KH, G = p.H / KH, page = p.pv.page;
     griddep_launch();                       // the join may be scheduled; it waits for this grid
-    if (lane == 0) {
-        for (int s = 0; s < PD_STAGES; ++s) mbar_init(&sm.full[warp][s], 1);
-        fence_mbar_init();
-        sm.cont[warp] = sm.open[warp] = make_int4(0, 0, 0, 0);
-    }
-    if (tid == 0) { tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); }
-
-    // entries before each request: its tiles, a q and a gate entry
+    // entries before each request: its tiles, a q and a gate entry. Up to 32
+    // requests every warp counts for itself (all write the same), with no barrier.
+    auto entries = [&](int r) {
+        int row0, pos0;
+        return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 3 : 0;
+    };
     {
-        const int each = (p.n_req + PD_THREADS - 1) / PD_THREADS, r0 = min(p.n_req, tid * each), r1 = min(p.n_req, r0 + each);
-        auto entries = [&](int r) {
-            int row0, pos0;
-            return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 3 : 0;
-        };
+        const int each = (p.n_req + PD_THREADS - 1) / PD_THREADS, small = p.n_req <= 32;
+        const int r0 = min(p.n_req, small ? lane : tid * each), r1 = min(p.n_req, small ? lane + 1 : r0 + each);
         int mine = 0;
 #pragma unroll 1
         for (int r = r0; r < r1; ++r) mine += entries(r);
-        if (tid < p.rot / 2) sm.turn[tid] = f.turn[tid];
-        for (int j = tid; j < 2 * GQA_HD; j += PD_THREADS) sm.w1[0][j] = 1.f + p.qnw[j];   // knw follows qnw
+        if (lane == 0) {
+            for (int s = 0; s < PD_STAGES; ++s) mbar_init(&sm.full[warp][s], 1);
+            fence_mbar_init();
+            sm.cont[warp] = sm.open[warp] = make_int4(0, 0, 0, 0);
+        }
         int inc = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, inc, d);
             if (lane >= d) inc += y;
         }
-        if (lane == 31) sm.part[warp] = inc;
-        __syncthreads();
         int at = inc - mine;
-        for (int w = 0; w < warp; ++w) at += sm.part[w];
+        if (small) {
+            if (lane < p.n_req) sm.pre[lane] = at;
+            if (lane == 31) sm.pre[p.n_req] = inc;
+            __syncwarp();
+        } else {
+            if (lane == 31) sm.part[warp] = inc;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) at += sm.part[w];
 #pragma unroll 1
-        for (int r = r0; r < r1; ++r) { sm.pre[r] = at; at += entries(r); }
-        if (tid == PD_THREADS - 1) sm.pre[p.n_req] = at;
-        __syncthreads();
+            for (int r = r0; r < r1; ++r) { sm.pre[r] = at; at += entries(r); }
+            if (tid == PD_THREADS - 1) sm.pre[p.n_req] = at;
+            __syncthreads();
+        }
     }
     const int total = sm.pre[p.n_req] * KH, workers = gridDim.x * PD_WARPS;
     const int per = max(1, (total + workers - 1) / workers);
@@ -420,8 +423,7 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (e >= 0) {
             if (lane == 0) {
                 mbar_expect_tx(bar, PD_STAGE);
-                tma_load_4d(to, &tmK, 0, 0, 0, e, bar);
-                tma_load_4d(to + GQA_TILE_BYTES, &tmV, 0, 0, 0, e, bar);
+                tma_load_5d(to, &tmKV, 0, 0, 0, e, 0, bar);
             }
         } else {                            // rows of unit `u`, a bulk copy per lane
             const int u = (-1 - e) >> 1, is_q = (-1 - e) & 1, r = p.pv.heads_div(u), n = is_q ? G + 2 : G;
@@ -451,6 +453,14 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     enum { AT_Q, AT_TILE, AT_GATE } at = AT_Q;
 #pragma unroll 1
     for (int i = -PD_STAGES;; ++i) {
+        if (i == -1) {                      // behind the first loads: every warp writes the same
+            for (int j = lane; j < 2 * GQA_HD / 4; j += 32) {
+                const float4 w = reinterpret_cast<const float4 *>(p.qnw)[j];       // knw follows qnw
+                reinterpret_cast<float4 *>(sm.w1[0])[j] = make_float4(1.f + w.x, 1.f + w.y, 1.f + w.z, 1.f + w.w);
+            }
+            for (int j = lane; j < p.rot / 2; j += 32) sm.turn[j] = f.turn[j];
+            __syncwarp();
+        }
         if (i >= 0) {
             if (at == AT_Q) {
                 // ---- the next unit with tiles in the range
@@ -684,59 +694,53 @@ pages_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             whole = opened;
         }
         // pieces: warps from .. from + n - 1, none of those between empty
-        float f0[PD_WARPS], f1[PD_WARPS], M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
-#pragma unroll
-        for (int j = 0; j < PD_WARPS; ++j) {
-            if (j >= n) continue;
-            M0 = fmaxf(M0, sm.ml[from + j][opened && j == 0][h0].x);
-            M1 = fmaxf(M1, sm.ml[from + j][opened && j == 0][h0 + 1].x);
+        float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f, o[4][4] = {};
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+            const float2 *ml = sm.ml[from + j][opened && j == 0];
+            M0 = fmaxf(M0, ml[h0].x);
+            M1 = fmaxf(M1, ml[h0 + 1].x);
         }
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+            const bool open = opened && j == 0;
+            const float2 a = sm.ml[from + j][open][h0], b = sm.ml[from + j][open][h0 + 1];
+            const float f0 = a.x == -INFINITY ? 0.f : ex2_approx(a.x - M0), f1 = b.x == -INFINITY ? 0.f : ex2_approx(b.x - M1);
+            L0 += a.y * f0;
+            L1 += b.y * f1;
+            const float4 *src = (!open && sm.cont[from + j].w ? part.park + (size_t)(cta * PD_WARPS + from + j) * 512
+                                                              : reinterpret_cast<const float4 *>(sm.ring[from + j][0])) + lane;
 #pragma unroll
-        for (int j = 0; j < PD_WARPS; ++j) {
-            f0[j] = f1[j] = 0.f;
-            if (j >= n) continue;
-            const float2 a = sm.ml[from + j][opened && j == 0][h0], b = sm.ml[from + j][opened && j == 0][h0 + 1];
-            f0[j] = a.x == -INFINITY ? 0.f : ex2_approx(a.x - M0);
-            f1[j] = b.x == -INFINITY ? 0.f : ex2_approx(b.x - M1);
-            L0 += a.y * f0[j];
-            L1 += b.y * f1[j];
+            for (int u = 0; u < 4; ++u) {
+                const float4 x = src[(warp + PD_WARPS * u) * 32];
+                o[u][0] += x.x * f0; o[u][1] += x.y * f1; o[u][2] += x.z * f0; o[u][3] += x.w * f1;
+            }
         }
         const int slot = 2 * cta + (opened ? 1 : 0);
-        const float i0 = 1.f / L0, i1 = 1.f / L1;
-        if (!whole && warp == 0 && lane < 4) {
-            float2 *ml = part.ml + (size_t)slot * GQA_GRP + h0;
-            ml[0] = make_float2(M0, L0);
-            ml[1] = make_float2(M1, L1);
-        }
+        if (whole) {
+            const float i0 = rcp_approx(L0), i1 = rcp_approx(L1);
+            const size_t row = (size_t)unit.y * p.H + unit.z * G + h0;
+            TI *out = static_cast<TI *>(p.ctx) + row * GQA_HD + warp * 16 + dr;
+            const TI *g = static_cast<const TI *>(p.qg) + row * 2 * GQA_HD + GQA_HD + warp * 16 + dr;
 #pragma unroll
-        for (int u = 0; u < 16 / PD_WARPS; ++u) {
-            const int mt = warp + PD_WARPS * u, d = mt * 16 + dr;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int j = 0; j < PD_WARPS; ++j) {
-                if (j >= n) continue;
-                const bool parked = !(opened && j == 0) && sm.cont[from + j].w;
-                const float4 a = parked ? part.park[(size_t)(cta * PD_WARPS + from + j) * 512 + mt * 32 + lane]
-                                        : reinterpret_cast<const float4 *>(sm.ring[from + j][0])[mt * 32 + lane];
-                o.x += a.x * f0[j]; o.y += a.y * f1[j]; o.z += a.z * f0[j]; o.w += a.w * f1[j];
+                for (int e = 0; e < 4; ++e)     // (head h0 + e % 2, dim + 8 (e / 2))
+                    if (h0 + (e & 1) < G) {
+                        const int d = 16 * PD_WARPS * u + 8 * (e >> 1);
+                        out[(e & 1) * GQA_HD + d] = from_f32<TI>(o[u][e] * (e & 1 ? i1 : i0) * gate_of(to_f32(g[(e & 1) * 2 * GQA_HD + d])));
+                    }
+        } else {
+            if (warp == 0 && lane < 4) {
+                float2 *ml = part.ml + (size_t)slot * GQA_GRP + h0;
+                ml[0] = make_float2(M0, L0);
+                ml[1] = make_float2(M1, L1);
             }
-            if (whole) {
-                const size_t row = (size_t)unit.y * p.H + unit.z * G + h0;
-                TI *out = static_cast<TI *>(p.ctx) + row * GQA_HD + d;
-                const TI *g = static_cast<const TI *>(p.qg) + row * 2 * GQA_HD + GQA_HD + d;
-                if (h0 < G) {
-                    out[0] = from_f32<TI>(o.x * i0 * gate_of(to_f32(g[0])));
-                    out[8] = from_f32<TI>(o.z * i0 * gate_of(to_f32(g[8])));
-                }
-                if (h0 + 1 < G) {
-                    out[GQA_HD] = from_f32<TI>(o.y * i1 * gate_of(to_f32(g[2 * GQA_HD])));
-                    out[GQA_HD + 8] = from_f32<TI>(o.w * i1 * gate_of(to_f32(g[2 * GQA_HD + 8])));
-                }
-            } else {
-                float *out = part.o + ((size_t)slot * GQA_GRP + h0) * GQA_HD + d;
-                out[0] = o.x; out[8] = o.z;
-                out[GQA_HD] = o.y; out[GQA_HD + 8] = o.w;
-            }
+            float *out = part.o + ((size_t)slot * GQA_GRP + h0) * GQA_HD + warp * 16 + dr;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[(e & 1) * GQA_HD + 16 * PD_WARPS * u + 8 * (e >> 1)] = o[u][e];
         }
         if (step == 2 * PD_WARPS) break;
         n = 0;
@@ -808,13 +812,13 @@ pages_join_kernel(GqaPagesArgs p, PagesPart part)
 }
 
 template <typename TI>
-static cudaError_t pages_decode_run(const CUtensorMap &tk, const CUtensorMap &tv, const GqaPagesArgs &a, const PagesPart &part,
+static cudaError_t pages_decode_run(const CUtensorMap &tkv, const GqaPagesArgs &a, const PagesPart &part,
                                     const RopeFreq &f, int ctas, cudaStream_t st)
 {
     const int smem = (int)sizeof(PdSmem) + 1024;
     cudaError_t e = cudaFuncSetAttribute(pages_decode_kernel<TI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    pages_decode_kernel<TI><<<ctas, PD_THREADS, smem, st>>>(tk, tv, a, part, f);
+    pages_decode_kernel<TI><<<ctas, PD_THREADS, smem, st>>>(a, part, tkv, f);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, a.H / a.pv.KH); cfg.blockDim = dim3(GQA_HD); cfg.stream = st;
@@ -825,11 +829,11 @@ static cudaError_t pages_decode_run(const CUtensorMap &tk, const CUtensorMap &tv
     return cudaLaunchKernelEx(&cfg, pages_join_kernel<TI>, a, part);
 }
 
-cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, const GqaPagesArgs &a, const PagesPart &part,
+cudaError_t launch_pages_decode(const CUtensorMap &tkv, const GqaPagesArgs &a, const PagesPart &part,
                                 const RopeFreq &f, int in_bf16, int ctas, cudaStream_t st)
 {
-    return in_bf16 ? pages_decode_run<__nv_bfloat16>(tk, tv, a, part, f, ctas, st)
-                   : pages_decode_run<float>(tk, tv, a, part, f, ctas, st);
+    return in_bf16 ? pages_decode_run<__nv_bfloat16>(tkv, a, part, f, ctas, st)
+                   : pages_decode_run<float>(tkv, a, part, f, ctas, st);
 }
 
 // ------------------------------------------------------------------ prefill

@@ -222,7 +222,7 @@ struct PagesPart {
     int4 *plan;           // prefill: [ctas + 1] where each CTA's range starts (request, KV head, query tile, key tile)
     int4 *units;          // decode: [ctas] unit that begins in CTA c and goes on: (last CTA or -1, request, KV head, ..)
 };
-cudaError_t launch_pages_decode(const CUtensorMap &tk, const CUtensorMap &tv, const GqaPagesArgs &a, const PagesPart &part,
+cudaError_t launch_pages_decode(const CUtensorMap &tkv, const GqaPagesArgs &a, const PagesPart &part,
                                 const RopeFreq &f, int in_bf16, int ctas, cudaStream_t st);
 cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tv8, const CUtensorMap &tg,
                                  const GqaPagesArgs &a, const PagesPart &part, const RopeFreq &f, int ctas, cudaStream_t st);

@@ -18,7 +18,7 @@ struct ColiCudaPages {
     float *norm_w;            // [layers][2][256]
     unsigned char *norm_set;  // [layers] (host)
     uint8_t *ws, *own_ws;
-    CUtensorMap *maps;        // [layers][K, V] in boxes of 16 rows, K and V of box_rows, V of 8
+    CUtensorMap *maps;        // [layers][4] K and V in one box of 16 rows each; K, V in boxes of box_rows, V of 8
     int box_rows;
     int rot;                  // rotary frequencies as last used
     float theta;
@@ -53,16 +53,16 @@ PagesPart pages_part(uint8_t *ws)
     return t;
 }
 
-// Rows of 256 bf16 as (64 columns, 8 rows, 4 column blocks, groups of 8 rows):
-// one box is a run of whole row groups, [group][block][8 rows][128 B] in shared
-// memory, 128B-swizzled.
-int make_pages_tmap(CUtensorMap *m, void *base, long long rows, int box_rows)
+// Rows of 256 bf16 as (64 columns, 8 rows, 4 column blocks, groups of 8 rows), and
+// `planes` such arrays `plane` bytes apart: one box is a run of whole row groups of
+// every plane, [plane][group][block][8 rows][128 B] in shared memory, 128B-swizzled.
+int make_pages_tmap(CUtensorMap *m, void *base, long long rows, int box_rows, int planes, size_t plane)
 {
-    cuuint64_t dims[4] = {64, 8, 4, (cuuint64_t)(rows / 8)};
-    cuuint64_t strides[3] = {GQA_HD * 2, 128, 8 * GQA_HD * 2};
-    cuuint32_t box[4] = {64, 8, 4, (cuuint32_t)(box_rows / 8)};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    CUresult r = G.encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, estr,
+    cuuint64_t dims[5] = {64, 8, 4, (cuuint64_t)(rows / 8), (cuuint64_t)planes};
+    cuuint64_t strides[4] = {GQA_HD * 2, 128, 8 * GQA_HD * 2, (cuuint64_t)plane};
+    cuuint32_t box[5] = {64, 8, 4, (cuuint32_t)(box_rows / 8), (cuuint32_t)planes};
+    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    CUresult r = G.encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes > 1 ? 5 : 4, base, dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled (pages) failed (%d)", (int)r);
@@ -209,7 +209,7 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
     p->layers = layers; p->n_pages = n_pages; p->page = page; p->KH = KH;
     p->base = (uint8_t *)kv_dev;
     p->norm_set = new (std::nothrow) unsigned char[layers]();
-    p->maps = new (std::nothrow) CUtensorMap[5 * layers];
+    p->maps = new (std::nothrow) CUtensorMap[4 * layers];
     const size_t bytes = (size_t)layers * 2 * n_pages * pages_page_bytes(KH, page);
     int ok = p->norm_set && p->maps;
     if (!ok) fail("pages: out of host memory");
@@ -224,10 +224,9 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
     for (int i = 0; ok && i < layers; ++i) {
         uint8_t *k = p->base + (size_t)i * (bytes / layers), *v = k + bytes / layers / 2;
         const long long rows = (long long)n_pages * KH * page;
-        CUtensorMap *m = p->maps + 5 * i;
-        ok = make_pages_tmap(m, k, rows, GQA_TILE) && make_pages_tmap(m + 1, v, rows, GQA_TILE) &&
-             make_pages_tmap(m + 2, k, rows, p->box_rows) && make_pages_tmap(m + 3, v, rows, p->box_rows) &&
-             make_pages_tmap(m + 4, v, rows, 8);
+        CUtensorMap *m = p->maps + 4 * i;
+        ok = make_pages_tmap(m, k, rows, GQA_TILE, 2, v - k) && make_pages_tmap(m + 1, k, rows, p->box_rows, 1, 0) &&
+             make_pages_tmap(m + 2, v, rows, p->box_rows, 1, 0) && make_pages_tmap(m + 3, v, rows, 8, 1, 0);
     }
     if (!ok) { pages_release(p); return 0; }
     g_pages[slot] = p;
@@ -297,7 +296,7 @@ int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const
         return fail("pages: a table of %d x %d pages passes 2^31 tiles", B, max_pages);
     a.n_req = a.S = B;
     g_pages_ran = true;
-    CK(launch_pages_decode(pages->maps[5 * layer], pages->maps[5 * layer + 1], a, pages_part(pages->ws), pages->freq, dtype,
+    CK(launch_pages_decode(pages->maps[4 * layer], a, pages_part(pages->ws), pages->freq, dtype,
                            G.num_sms, stream()));
     g_launches += 2;
     return 1;
@@ -318,11 +317,11 @@ int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, 
     a.cu = cu;
     a.n_req = n_seq; a.S = S;
     g_pages_ran = true;
-    const CUtensorMap *m = pages->maps + 5 * layer;
+    const CUtensorMap *m = pages->maps + 4 * layer;
     CUtensorMap gate;
     if (!make_pages_gate_tmap(&gate, qg, S, H, H / KH)) return 0;
     a.box_rows = pages->box_rows;
-    CK(launch_pages_prefill(m[2], m[3], m[4], gate, a, pages_part(pages->ws), pages->freq, G.num_sms, stream()));
+    CK(launch_pages_prefill(m[1], m[2], m[3], gate, a, pages_part(pages->ws), pages->freq, G.num_sms, stream()));
     g_launches += 3;
     return 1;
 }
