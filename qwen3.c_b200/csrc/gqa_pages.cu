@@ -330,6 +330,11 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
         int row0, pos0;
         return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 3 : 0;
     };
+    // the norm weights and rotary frequencies: loads in flight until the first
+    // tiles are, then every warp writes the same
+    float4 w_in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w_in[j] = reinterpret_cast<const float4 *>(p.qnw)[lane + 32 * j];   // knw follows qnw
     {
         const int each = (p.n_req + PD_THREADS - 1) / PD_THREADS, small = p.n_req <= 32;
         const int r0 = min(p.n_req, small ? lane : tid * each), r1 = min(p.n_req, small ? lane + 1 : r0 + each);
@@ -453,11 +458,11 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
     enum { AT_Q, AT_TILE, AT_GATE } at = AT_Q;
 #pragma unroll 1
     for (int i = -PD_STAGES;; ++i) {
-        if (i == -1) {                      // behind the first loads: every warp writes the same
-            for (int j = lane; j < 2 * GQA_HD / 4; j += 32) {
-                const float4 w = reinterpret_cast<const float4 *>(p.qnw)[j];       // knw follows qnw
-                reinterpret_cast<float4 *>(sm.w1[0])[j] = make_float4(1.f + w.x, 1.f + w.y, 1.f + w.z, 1.f + w.w);
-            }
+        if (i == -1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                reinterpret_cast<float4 *>(sm.w1[0])[lane + 32 * j] =
+                    make_float4(1.f + w_in[j].x, 1.f + w_in[j].y, 1.f + w_in[j].z, 1.f + w_in[j].w);
             for (int j = lane; j < p.rot / 2; j += 32) sm.turn[j] = f.turn[j];
             __syncwarp();
         }
@@ -708,13 +713,16 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
             const float f0 = a.x == -INFINITY ? 0.f : ex2_approx(a.x - M0), f1 = b.x == -INFINITY ? 0.f : ex2_approx(b.x - M1);
             L0 += a.y * f0;
             L1 += b.y * f1;
-            const float4 *src = (!open && sm.cont[from + j].w ? part.park + (size_t)(cta * PD_WARPS + from + j) * 512
-                                                              : reinterpret_cast<const float4 *>(sm.ring[from + j][0])) + lane;
+            float4 x[4];
+            if (!open && sm.cont[from + j].w) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float4 x = src[(warp + PD_WARPS * u) * 32];
-                o[u][0] += x.x * f0; o[u][1] += x.y * f1; o[u][2] += x.z * f0; o[u][3] += x.w * f1;
+                for (int u = 0; u < 4; ++u) x[u] = part.park[(size_t)(cta * PD_WARPS + from + j) * 512 + (warp + PD_WARPS * u) * 32 + lane];
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = reinterpret_cast<const float4 *>(sm.ring[from + j][0])[(warp + PD_WARPS * u) * 32 + lane];
             }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { o[u][0] += x[u].x * f0; o[u][1] += x[u].y * f1; o[u][2] += x[u].z * f0; o[u][3] += x[u].w * f1; }
         }
         const int slot = 2 * cta + (opened ? 1 : 0);
         if (whole) {
@@ -750,31 +758,36 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
     if (tid == 0) part.units[cta] = make_int4(n > 0 && opened ? unit.w : -1, unit.y, unit.z, 0);
 }
 
-// One CTA per (first CTA of a split unit, query head): merges the unit's
-// pieces. Warp w takes pieces w, w + 8, .. with a running maximum, lane = 8
-// dims; then thread d merges the warps' results of dim d.
+// One CTA of four warps per (CTA of the kernel before, query head): merges the
+// pieces of the unit that begins there and goes on. Warp w takes pieces w, w + 4,
+// .. with a running maximum, lane = 8 dims; then thread d merges the four results
+// of dims d and d + 128. Small enough that all of them, most with nothing to do,
+// are resident at once; one CTA for all heads of a unit had one SM read all pieces
+// of a long single request (5 us of 20).
+constexpr int PJ_WARPS = 4;
 template <typename TI>
-__global__ void __launch_bounds__(GQA_HD)
+__global__ void __launch_bounds__(PJ_WARPS * 32)
 pages_join_kernel(GqaPagesArgs p, PagesPart part)
 {
-    constexpr int W = GQA_HD / 32;
-    __shared__ float sm_ml[W][2];
-    __shared__ __align__(16) float sm_o[W][GQA_HD];
+    __shared__ float sm_ml[PJ_WARPS][2];
+    __shared__ __align__(16) float sm_o[PJ_WARPS][GQA_HD];
     const int a = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_wait();                         // a programmatic dependent of the decode kernel
     const int4 unit = part.units[a];
     if (unit.x < 0) return;
-    const int n = unit.x - a + 1, G = p.H / p.pv.KH, head = unit.z * G + h;
-    const size_t row = (size_t)unit.y * p.H + head;
-    const float gate = to_f32(static_cast<const TI *>(p.qg)[row * 2 * GQA_HD + GQA_HD + tid]);
+    const int n = unit.x - a + 1;
+    const size_t row = (size_t)unit.y * p.H + unit.z * (p.H / p.pv.KH) + h;
+    float gate[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) gate[e] = to_f32(static_cast<const TI *>(p.qg)[row * 2 * GQA_HD + GQA_HD + tid + 128 * e]);
     float m = -INFINITY, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     constexpr int U = 4;                    // pieces whose loads a warp issues together
-    for (int s0 = warp; s0 < n; s0 += U * W) {
+    for (int s0 = warp; s0 < n; s0 += U * PJ_WARPS) {
         float2 ml[U];
         float4 x[U], y[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = s0 + u * W;
+            const int s = s0 + u * PJ_WARPS;
             ml[u] = make_float2(-INFINITY, 0.f);
             if (s < n) {
                 const size_t at = (size_t)(s ? 2 * (a + s) : 2 * a + 1) * GQA_GRP + h;
@@ -799,16 +812,20 @@ pages_join_kernel(GqaPagesArgs p, PagesPart part)
     *reinterpret_cast<float4 *>(&sm_o[warp][8 * lane]) = make_float4(o[0], o[1], o[2], o[3]);
     *reinterpret_cast<float4 *>(&sm_o[warp][8 * lane + 4]) = make_float4(o[4], o[5], o[6], o[7]);
     __syncthreads();
-    float M = -INFINITY, O = 0.f, L = 0.f;
+    float M = -INFINITY, O[2] = {0.f, 0.f}, L = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, sm_ml[w][0]);
+    for (int w = 0; w < PJ_WARPS; ++w) M = fmaxf(M, sm_ml[w][0]);
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < PJ_WARPS; ++w) {
         const float f = sm_ml[w][0] == -INFINITY ? 0.f : ex2_approx(sm_ml[w][0] - M);
-        O += sm_o[w][tid] * f;
+        O[0] += sm_o[w][tid] * f;
+        O[1] += sm_o[w][tid + 128] * f;
         L += sm_ml[w][1] * f;
     }
-    static_cast<TI *>(p.ctx)[row * GQA_HD + tid] = from_f32<TI>(O / L * gate_of(gate));
+    const float inv = rcp_approx(L);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        static_cast<TI *>(p.ctx)[row * GQA_HD + tid + 128 * e] = from_f32<TI>(O[e] * inv * gate_of(gate[e]));
 }
 
 template <typename TI>
@@ -821,7 +838,7 @@ static cudaError_t pages_decode_run(const CUtensorMap &tkv, const GqaPagesArgs &
     pages_decode_kernel<TI><<<ctas, PD_THREADS, smem, st>>>(a, part, tkv, f);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, a.H / a.pv.KH); cfg.blockDim = dim3(GQA_HD); cfg.stream = st;
+    cfg.gridDim = dim3(ctas, a.H / a.pv.KH); cfg.blockDim = dim3(PJ_WARPS * 32); cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
