@@ -45,6 +45,24 @@ __device__ __forceinline__ float rcp_approx(float x)
     return y;
 }
 __device__ __forceinline__ float gate_of(float x) { return rcp_approx(1.f + ex2_approx(x * -1.4426950408889634f)); }   // sigmoid
+// o *= sigmoid(g) for four elements, e^g / (1 + e^g) with one reciprocal of the
+// product of the four 1 + e^g: 5 special-function instructions instead of 8, which
+// bound the epilogues. Above 20 a sigmoid is 1 in fp32; held there, the product
+// stays below 6e34.
+__device__ __forceinline__ void gate4(float *o, const float *g)
+{
+    float e[4], d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        e[i] = ex2_approx((g[i] > 20.f ? 20.f : g[i]) * 1.4426950408889634f);
+        d[i] = 1.f + e[i];
+    }
+    const float d01 = d[0] * d[1], d23 = d[2] * d[3], r = rcp_approx(d01 * d23), r01 = r * d23, r23 = r * d01;
+    o[0] *= e[0] * d[1] * r01;
+    o[1] *= e[1] * d[0] * r01;
+    o[2] *= e[2] * d[3] * r23;
+    o[3] *= e[3] * d[2] * r23;
+}
 __device__ __forceinline__ float rms_factor(float s2, float eps)     // 1 / sqrt(s2 / hd + eps), one Newton step
 {
     const float a = fmaf(s2, 1.f / GQA_HD, eps), r = rsqrtf(a);
@@ -220,6 +238,9 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
 // Short calls are bound by latency, instruction fetch a large part of it: what
 // runs once per unit is kept in rolled loops over heads.
 constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_STAGES = 3, PD_STAGE = 2 * GQA_TILE_BYTES;
+// Entries that a unit counts more than it has when the list is cut: its q and
+// gate take a warp about as long as PD_EXTRA + 2 tiles.
+constexpr int PD_EXTRA = 2;
 constexpr int PD_OROW = 132;                 // floats between heads of O: 8 banks apart for the writers' heads
 template <typename TI> struct PdEntry {      // layout of the q entry and of the gate entry in a stage
     static constexpr bool F32 = sizeof(TI) == 4;
@@ -328,7 +349,7 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
     // requests every warp counts for itself (all write the same), with no barrier.
     auto entries = [&](int r) {
         int row0, pos0;
-        return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 3 : 0;
+        return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 3 + PD_EXTRA : 0;
     };
     // the norm weights and rotary frequencies: loads in flight until the first
     // tiles are, then every warp writes the same
@@ -394,12 +415,12 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
         int kh = (int)__fdividef((float)rel0, (float)n);        // at most KH <= 64: off by one at most
         kh -= kh * n > rel0;
         kh += (kh + 1) * n <= rel0;
-        const int rel = rel0 - kh * n, nt = n - 2;
+        const int rel = rel0 - kh * n - PD_EXTRA, nt = n - 2 - PD_EXTRA;       // 0: q, 1 ..: tiles, nt + 1: gate
         const bool begins = at - rel + 1 >= v0;                 // the unit's first tile is in the range
         if (v < v0) ahead = rel >= 1 && rel <= nt ? 1 : -1;
         else if (v == v1) ahead = rel == nt && begins ? 2 : -1;
         else if (rel == 0) ahead = v + 1 < v1 ? 1 : -1;
-        else if (rel <= nt) ahead = 0;
+        else if (rel <= nt) ahead = rel < 0 ? -1 : 0;
         else ahead = begins ? 2 : -1;
         ahead_row = r * KH + kh;
         if (ahead == 0) {
@@ -473,10 +494,10 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                     if (next_v >= v1) break;
                     r = next_r; kh = next_kh;
                     const int n = sm.pre[r + 1] - sm.pre[r];
-                    nt = n - 2;
+                    nt = n - 2 - PD_EXTRA;
                     u0 = sm.pre[r] * KH + kh * n;
-                    tile = max(next_v - u0 - 1, 0);
-                    end_tile = min(v1 - u0 - 1, nt);
+                    tile = max(next_v - u0 - 1 - PD_EXTRA, 0);
+                    end_tile = min(v1 - u0 - 1 - PD_EXTRA, nt);
                     next_v = min(v1, u0 + n);
                     if (++next_kh == KH) {
                         next_kh = 0;
@@ -633,7 +654,7 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                         const int kind = begins ? 1 : 0;
                         const bool last = next_v >= v1;
                         if (lane == 0) {
-                            if (begins) sm.open[warp] = make_int4(1, r, kh, (u0 + nt) / per / PD_WARPS);
+                            if (begins) sm.open[warp] = make_int4(1, r, kh, (u0 + PD_EXTRA + nt) / per / PD_WARPS);
                             else sm.cont[warp] = make_int4(ends ? 3 : 1, r, kh, last ? 0 : 1);
                         }
                         if (lane < 4) { sm.ml[warp][kind][h0] = make_float2(m0, l0); sm.ml[warp][kind][h0 + 1] = make_float2(m1, l1); }
@@ -664,8 +685,7 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                         float o[4], g[4];
                         load4(reinterpret_cast<const TI *>(gate + h * E::GROW) + half * 128, g);
                         load4(o_ + h * PD_OROW + 4 * lane, o);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] *= gate_of(g[e]);
+                        gate4(o, g);
                         if (h < G) store4(out + (size_t)h * GQA_HD + half * 128, o);
                     }
                     __syncwarp();
@@ -1409,7 +1429,9 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                         float gv[8], y[8];
                         load8v(reinterpret_cast<const __nv_bfloat16 *>(gt + off), gv);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = o[8 * k + e] * inv_l * gate_of(gv[e]);
+                        for (int e = 0; e < 8; ++e) y[e] = o[8 * k + e] * inv_l;
+                        gate4(y, gv);
+                        gate4(y + 4, gv + 4);
                         store8v(reinterpret_cast<__nv_bfloat16 *>(gt + off), y);
                     }
                 }
@@ -1491,7 +1513,8 @@ pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
     float g[4], y[4];
     load4(static_cast<const __nv_bfloat16 *>(p.qg) + at * 2 * GQA_HD + GQA_HD + block * 32 + c, g);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = turned[r][c + e] * gate_of(g[e]);
+    for (int e = 0; e < 4; ++e) y[e] = turned[r][c + e];
+    gate4(y, g);
     store4(static_cast<__nv_bfloat16 *>(p.ctx) + at * GQA_HD + block * 32 + c, y);
 }
 
