@@ -975,31 +975,27 @@ __device__ __forceinline__ void pp_plan(const GqaPagesArgs &p, int cta, int ctas
     for (int r = r0; r < r1; ++r) { pre[r] = at; at += pp_chunk_work(p, r, gs); }
     if (tid == PP_THREADS - 1) pre[p.n_req] = at;
     __syncthreads();
-    if (tid < 2) {
-        const long long all = pre[p.n_req] * KH, per = max((long long)PP_MIN, (all + ctas - 1) / ctas), v = (cta + tid) * per;
+    if (warp < 2) {                         // a warp per range, 32 places looked at at a time
+        const long long all = pre[p.n_req] * KH, per = max((long long)PP_MIN, (all + ctas - 1) / ctas), v = (cta + warp) * per;
         int4 u = make_int4(p.n_req, 0, 0, 0);
         if (v < all) {
-            int lo = 0, hi = p.n_req - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (pre[mid] * KH <= v) lo = mid; else hi = mid - 1;
-            }
+            int lo = -1;                    // the last request that starts at or before v
+            for (int r = lane; r - lane < p.n_req; r += 32) lo += __popc(__ballot_sync(0xffffffffu, r < p.n_req && pre[r] * KH <= v));
             const long long head = pre[lo + 1] - pre[lo];
             long long rel = v - pre[lo] * KH;
             u.x = lo;
-            u.y = (int)(rel / head);
-            rel -= u.y * head;
+            while (rel >= head) { rel -= head; ++u.y; }
             int row0, b, q0 = 0;
             const int n = pages_rows_of(p, lo, row0, b);
-            int q1 = (n - 1) >> (7 - gs);
-            while (q0 < q1) {               // the last query tile that starts at or before rel
-                const int mid = (q0 + q1 + 1) >> 1;
-                if (pp_work(b, mid, gs) <= rel) q0 = mid; else q1 = mid - 1;
+            for (int left = ((n - 1) >> (7 - gs)) + 1; left > 1;) {           // .. and query tile, of the `left` from q0 on
+                const int step = (left + 31) / 32, k = __popc(__ballot_sync(0xffffffffu, lane * step < left && pp_work(b, q0 + lane * step, gs) <= rel)) - 1;
+                q0 += k * step;
+                left = min(step, left - k * step);
             }
             u.z = q0;
             u.w = max(0, (int)(rel - pp_work(b, q0, gs)) - PP_SETUP);
         }
-        range[tid] = u;
+        if (lane == 0) range[warp] = u;
     }
     __syncthreads();
 }
@@ -1019,12 +1015,9 @@ pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
     float x[8], v[8], w1[8];
     load8<__nv_bfloat16>(k + lane * 8, x);
     load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.v) + (size_t)item * GQA_HD + lane * 8, v);
-    int lo = 0, hi = p.n_req - 1, row0, b;
-    while (lo < hi) {                       // the last request that starts at or before the row
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.cu[mid] <= row) lo = mid; else hi = mid - 1;
-    }
-    if (row < p.cu[lo] || row >= p.cu[lo + 1] || pages_rows_of(p, lo, row0, b) == 0) return;
+    int lo = -1, row0, b;                   // the last request that starts at or before the row
+    for (int r = lane; r - lane < p.n_req; r += 32) lo += __popc(__ballot_sync(0xffffffffu, r < p.n_req && p.cu[r] <= row));
+    if (lo < 0 || row < p.cu[lo] || row >= p.cu[lo + 1] || pages_rows_of(p, lo, row0, b) == 0) return;
     const int pos = b + row - row0;
     const long long at = pages_row(p.pv, lo, kh, pos);
     pages_rope_table(cs[warp], sn[warp], pos, p.rot, f.turn, lane, 32);
@@ -1472,50 +1465,132 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     griddep_wait();                         // this grid ends after the one before, also where no tile waited for it
 }
 
-// One CTA per (first CTA of a split unit, 32 rows, 32 dims): adds the pieces
-// up, lane = row, warp = 4 dims, then turns the block to write 64-byte runs.
-constexpr int PJ_THREADS = 256;
+// The unit that begins in CTA a and goes on, and the number of its pieces; false
+// where there is none. A whole CTA of at least `ctas` threads.
+__device__ __forceinline__ bool pp_split_unit(const PagesPart &part, int a, int ctas, int4 &unit, int &n)
+{
+    const int4 first = part.plan[a];
+    unit = part.plan[a + 1];
+    const int4 u = unit;
+    auto same = [&](const int4 &x) { return x.x == u.x && x.y == u.y && x.z == u.z && x.w > 0; };
+    if (u.w == 0 || same(first)) return false;
+    const int at = a + 1 + (int)threadIdx.x;
+    n = 1 + __syncthreads_count(at <= ctas && same(part.plan[at]));
+    return true;
+}
+
+// Two joins. Many units on the GPU: few pieces each, and one CTA per (unit, 32
+// rows, 128 dims) adds them up, lane = row, a warp 4 x 4 dims whose loads go out
+// together, then turns the block to write 256-byte runs. Few units (a quarter of
+// the CTAs or less): many pieces each, and one CTA per (unit, 32 rows, 32 dims) has
+// its warps take every eighth of them. 16 rows at 28k: 62 us with
+// the second, 93 with the first.
+constexpr int PJ_THREADS = 256, PJ_DIMS = 128;
 __global__ void __launch_bounds__(PJ_THREADS)
 pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
 {
-    __shared__ float turned[32][33];
+    __shared__ __align__(16) float turned[32][PJ_DIMS + 4];
     const int a = blockIdx.x, quarter = blockIdx.y & 3, block = blockIdx.y >> 2, tid = threadIdx.x, j = tid >> 5, lane = tid & 31;
     griddep_wait();
-    const int4 unit = part.plan[a + 1], first = part.plan[a];
-    if (unit.w == 0) return;                // no unit is cut between CTA a and the next
-    auto same = [&](const int4 &x) { return x.x == unit.x && x.y == unit.y && x.z == unit.z && x.w > 0; };
-    if (same(first)) return;                // .. or its first piece is an earlier CTA's
-    const int n = 1 + __syncthreads_count(a + 1 + tid <= (int)gridDim.x && same(part.plan[a + 1 + tid]));
+    int4 unit;
+    int n;
+    if (!pp_split_unit(part, a, gridDim.x, unit, n)) return;
     const int row = quarter * 32 + lane;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+    float m = -INFINITY, l = 0.f, o[4][4] = {};
+#pragma unroll 2
     for (int s = 0; s < n; ++s) {
         const size_t slot = s ? 2 * (a + s) : 2 * a + 1;
         const float2 ml = part.ml[slot * PP_BM + row];
-        const float4 x = reinterpret_cast<const float4 *>(part.o)[slot * (PP_BM * GQA_HD / 4) + (8 * block + j) * PP_BM + row];
+        float4 x[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            x[c] = reinterpret_cast<const float4 *>(part.o)[slot * (PP_BM * GQA_HD / 4) + (block * (PJ_DIMS / 4) + 8 * c + j) * PP_BM + row];
         if (ml.x == -INFINITY) continue;
         const float mn = fmaxf(m, ml.x), fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fs = ex2_approx(ml.x - mn);
-        o.x = o.x * fo + x.x * fs; o.y = o.y * fo + x.y * fs; o.z = o.z * fo + x.z * fs; o.w = o.w * fo + x.w * fs;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            o[c][0] = o[c][0] * fo + x[c].x * fs; o[c][1] = o[c][1] * fo + x[c].y * fs;
+            o[c][2] = o[c][2] * fo + x[c].z * fs; o[c][3] = o[c][3] * fo + x[c].w * fs;
+        }
         l = l * fo + ml.y * fs;
         m = mn;
     }
     const float inv = 1.f / l;
-    turned[lane][4 * j] = o.x * inv; turned[lane][4 * j + 1] = o.y * inv;
-    turned[lane][4 * j + 2] = o.z * inv; turned[lane][4 * j + 3] = o.w * inv;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<float4 *>(&turned[lane][32 * c + 4 * j]) = make_float4(o[c][0] * inv, o[c][1] * inv, o[c][2] * inv, o[c][3] * inv);
     __syncthreads();
     int row0, base;
     const int rows = pages_rows_of(p, unit.x, row0, base);
-    const int group = p.H / p.pv.KH, tokens = PP_BM / group, r = tid >> 3, c = (tid & 7) * 4;
-    const int tile_row = quarter * 32 + r, t = unit.z * tokens + tile_row / group;
-    if (t >= rows) return;
-    const size_t at = (size_t)(row0 + t) * p.H + unit.y * group + tile_row % group;
-    float g[4], y[4];
-    load4(static_cast<const __nv_bfloat16 *>(p.qg) + at * 2 * GQA_HD + GQA_HD + block * 32 + c, g);
+    const int group = p.H / p.pv.KH, gs = __ffs(group) - 1;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = turned[r][c + e];
+    for (int i = 0; i < 4; ++i) {           // a warp per row, 4 dims to a lane
+        const int r = 8 * i + j, tile_row = quarter * 32 + r, t = (unit.z * PP_BM + tile_row) >> gs;
+        if (t >= rows) continue;
+        const size_t at = (size_t)(row0 + t) * p.H + unit.y * group + (tile_row & (group - 1));
+        float g[4], y[4];
+        load4(static_cast<const __nv_bfloat16 *>(p.qg) + at * 2 * GQA_HD + GQA_HD + block * PJ_DIMS + 4 * lane, g);
+        load4(&turned[r][4 * lane], y);
+        gate4(y, g);
+        store4(static_cast<__nv_bfloat16 *>(p.ctx) + at * GQA_HD + block * PJ_DIMS + 4 * lane, y);
+    }
+}
+
+constexpr int PJ_DEEP = 32;
+__global__ void __launch_bounds__(PJ_THREADS)
+pages_prefill_join_deep_kernel(GqaPagesArgs p, PagesPart part)
+{
+    __shared__ __align__(16) float acc[PJ_THREADS / 32][32][PJ_DEEP + 4];
+    __shared__ float2 mls[PJ_THREADS / 32][32];
+    const int a = blockIdx.x, quarter = blockIdx.y & 3, block = blockIdx.y >> 2, tid = threadIdx.x, j = tid >> 5, lane = tid & 31;
+    griddep_wait();
+    int4 unit;
+    int n;
+    if (!pp_split_unit(part, a, gridDim.x, unit, n)) return;
+    const int row = quarter * 32 + lane;
+    float m = -INFINITY, l = 0.f, o[8][4] = {};
+    for (int s = j; s < n; s += PJ_THREADS / 32) {
+        const size_t slot = s ? 2 * (a + s) : 2 * a + 1;
+        const float2 ml = part.ml[slot * PP_BM + row];
+        float4 x[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            x[c] = reinterpret_cast<const float4 *>(part.o)[slot * (PP_BM * GQA_HD / 4) + (block * (PJ_DEEP / 4) + c) * PP_BM + row];
+        if (ml.x == -INFINITY) continue;
+        const float mn = fmaxf(m, ml.x), fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fs = ex2_approx(ml.x - mn);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            o[c][0] = o[c][0] * fo + x[c].x * fs; o[c][1] = o[c][1] * fo + x[c].y * fs;
+            o[c][2] = o[c][2] * fo + x[c].z * fs; o[c][3] = o[c][3] * fo + x[c].w * fs;
+        }
+        l = l * fo + ml.y * fs;
+        m = mn;
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *reinterpret_cast<float4 *>(&acc[j][lane][4 * c]) = make_float4(o[c][0], o[c][1], o[c][2], o[c][3]);
+    mls[j][lane] = make_float2(m, l);
+    __syncthreads();
+    int row0, base;
+    const int rows = pages_rows_of(p, unit.x, row0, base);
+    const int group = p.H / p.pv.KH, gs = __ffs(group) - 1, r = tid >> 3, c = (tid & 7) * 4;
+    const int tile_row = quarter * 32 + r, t = (unit.z * PP_BM + tile_row) >> gs;
+    if (t >= rows) return;
+    const size_t at = (size_t)(row0 + t) * p.H + unit.y * group + (tile_row & (group - 1));
+    float g[4], y[4] = {}, M = -INFINITY, L = 0.f;
+    load4(static_cast<const __nv_bfloat16 *>(p.qg) + at * 2 * GQA_HD + GQA_HD + block * PJ_DEEP + c, g);
+#pragma unroll
+    for (int w = 0; w < PJ_THREADS / 32; ++w) M = fmaxf(M, mls[w][r].x);
+#pragma unroll
+    for (int w = 0; w < PJ_THREADS / 32; ++w) {
+        const float f = mls[w][r].x == -INFINITY ? 0.f : ex2_approx(mls[w][r].x - M);
+        L += mls[w][r].y * f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] += acc[w][r][c + e] * f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] *= 1.f / L;
     gate4(y, g);
-    store4(static_cast<__nv_bfloat16 *>(p.ctx) + at * GQA_HD + block * 32 + c, y);
+    store4(static_cast<__nv_bfloat16 *>(p.ctx) + at * GQA_HD + block * PJ_DEEP + c, y);
 }
 
 cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &tv8, const CUtensorMap &tg,
@@ -1523,6 +1598,11 @@ cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, c
 {
     cudaError_t e = cudaFuncSetAttribute(pages_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PP_SMEM);
     if (e != cudaSuccess) return e;
+    // at most that many units, and CTAs with work; the join looks at those only
+    const int tokens = PP_BM / (a.H / a.pv.KH);
+    const long long units = (long long)a.pv.KH * ((a.S + tokens - 1) / tokens + a.n_req);
+    const long long work = units * (((long long)a.pv.max_pages * a.pv.page + PP_BN - 1) / PP_BN + PP_SETUP);
+    const int used = (int)std::min<long long>(ctas, (work + PP_MIN - 1) / PP_MIN);
     pages_append_kernel<<<(int)(((long long)a.S * a.pv.KH + PA_WARPS - 1) / PA_WARPS), PA_WARPS * 32, 0, st>>>(a, f);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -1530,10 +1610,11 @@ cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, c
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
-    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(PP_THREADS); cfg.dynamicSmemBytes = PP_SMEM;
+    cfg.gridDim = dim3(used); cfg.blockDim = dim3(PP_THREADS); cfg.dynamicSmemBytes = PP_SMEM;
     if ((e = cudaLaunchKernelEx(&cfg, pages_prefill_kernel, tk, tv, tv8, tg, a, part, f)) != cudaSuccess) return e;
-    cfg.gridDim = dim3(ctas, 32); cfg.blockDim = dim3(PJ_THREADS); cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, pages_prefill_join_kernel, a, part);
+    const bool deep = 4 * units <= ctas;
+    cfg.gridDim = dim3(used, 4 * GQA_HD / (deep ? PJ_DEEP : PJ_DIMS)); cfg.blockDim = dim3(PJ_THREADS); cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, deep ? pages_prefill_join_deep_kernel : pages_prefill_join_kernel, a, part);
 }
 
 }  // namespace coli
