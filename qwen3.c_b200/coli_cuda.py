@@ -437,12 +437,20 @@ class PagedCache:
     kv: device address of the caller's memory for the pool, bf16
     [layers][2][n_pages][KH][page][hd] (None: the cache's own, zeroed). All
     *_dev calls take device addresses, run on the backend stream and neither
-    allocate nor wait; table is int32 [requests][max_pages]."""
+    allocate nor wait; table is int32 [requests][max_pages]. The pool is
+    released by free(), or with the object."""
 
     def __init__(self, be, layers, n_pages, page=64, KH=2, hd=256, kv=None):
         self.be, self.layers, self.n_pages, self.page, self.KH, self.hd = be, layers, n_pages, page, KH, hd
-        self.h = _vp()
-        be._ok(be.lib.coli_cuda_pages_create(ctypes.byref(self.h), layers, n_pages, page, KH, hd, kv), "pages_create")
+        self.h = None
+        h = _vp()
+        be._ok(be.lib.coli_cuda_pages_create(ctypes.byref(h), layers, n_pages, page, KH, hd, kv), "pages_create")
+        self.h, lib = h.value, be.lib
+        # bound once: a short call's time on the host is mostly this class's
+        self._free, self._decode, self._prefill = (lib.coli_cuda_pages_free, lib.coli_cuda_gqa_decode_pages_dev,
+                                                   lib.coli_cuda_gqa_prefill_pages_dev)
+        self._copy, self._fork, self._compact = (lib.coli_cuda_pages_copy_dev, lib.coli_cuda_pages_fork_dev,
+                                                 lib.coli_cuda_pages_compact_dev)
 
     @staticmethod
     def nbytes_for(be, layers, n_pages, page=64, KH=2, hd=256):
@@ -451,11 +459,13 @@ class PagedCache:
         return n
 
     def free(self):
-        if self.h:
-            self.be.lib.coli_cuda_pages_free(self.h)
-            self.h = _vp()
+        h, self.h = self.h, None
+        if h:
+            self._free(h)
 
-    __del__ = free
+    def __del__(self):
+        if getattr(self, "h", None):
+            self.free()
 
     def device_ptr(self, layer):
         k, v = _vp(), _vp()
@@ -477,26 +487,27 @@ class PagedCache:
         self.be._ok(self.be.lib.coli_cuda_pages_set_workspace(self.h, ws, nbytes), "pages_set_workspace")
 
     def decode_dev(self, layer, B, qg, k, v, pos, table, max_pages, ctx, H=16, rot=64, eps=1e-6, theta=1e7, dtype=1):
-        self.be._ok(self.be.lib.coli_cuda_gqa_decode_pages_dev(self.h, layer, B, qg, k, v, pos, table, max_pages, ctx, H,
-                                                               self.KH, self.hd, rot, eps, theta, dtype),
-                    "gqa_decode_pages_dev")
+        if self._decode(self.h, layer, B, qg, k, v, pos, table, max_pages, ctx, H, self.KH, self.hd, rot, eps, theta,
+                        dtype) != 1:
+            self.be._ok(0, "gqa_decode_pages_dev")
 
     def prefill_dev(self, layer, n_seq, S, cu, pos_base, qg, k, v, table, max_pages, ctx, H=16, rot=64, eps=1e-6,
                     theta=1e7, dtype=1):
-        self.be._ok(self.be.lib.coli_cuda_gqa_prefill_pages_dev(self.h, layer, n_seq, S, cu, pos_base, qg, k, v, table,
-                                                                max_pages, ctx, H, self.KH, self.hd, rot, eps, theta,
-                                                                dtype), "gqa_prefill_pages_dev")
+        if self._prefill(self.h, layer, n_seq, S, cu, pos_base, qg, k, v, table, max_pages, ctx, H, self.KH, self.hd,
+                         rot, eps, theta, dtype) != 1:
+            self.be._ok(0, "gqa_prefill_pages_dev")
 
     def copy_dev(self, n, src, dst):
-        self.be._ok(self.be.lib.coli_cuda_pages_copy_dev(self.h, n, src, dst), "pages_copy_dev")
+        if self._copy(self.h, n, src, dst) != 1:
+            self.be._ok(0, "pages_copy_dev")
 
     def fork_dev(self, n, parent, child, fresh, length, table, n_req, max_pages):
-        self.be._ok(self.be.lib.coli_cuda_pages_fork_dev(self.h, n, parent, child, fresh, length, table, n_req,
-                                                         max_pages), "pages_fork_dev")
+        if self._fork(self.h, n, parent, child, fresh, length, table, n_req, max_pages) != 1:
+            self.be._ok(0, "pages_fork_dev")
 
     def compact_dev(self, n_req, length, table, max_pages, table_out, live):
-        self.be._ok(self.be.lib.coli_cuda_pages_compact_dev(self.h, n_req, length, table, max_pages, table_out, live),
-                    "pages_compact_dev")
+        if self._compact(self.h, n_req, length, table, max_pages, table_out, live) != 1:
+            self.be._ok(0, "pages_compact_dev")
 
 
 def _block_methods():

@@ -145,13 +145,14 @@ __device__ __forceinline__ void pages_norm_rope(float (&x)[8], const float (&w1)
 // store) and single dims (load1 / store1); chunks go round the row's lanes, and a
 // rotated pair of chunks is one lane's, so nothing is overwritten before it is
 // read. A row on all 32 lanes takes 13 shuffles in a chain, 850 cycles; eight rows
-// on four lanes each take about 2000 together.
+// on four lanes each take about 2000 together. Rolled loops: code that runs once is
+// bound by instruction fetch.
 template <int LANES, typename Row>
 __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, const float *w1, float eps, int rot, const float *cs,
                                                      const float *sn)
 {
     float s0 = 0.f, s1 = 0.f;
-#pragma unroll
+#pragma unroll 2
     for (int k = 0; k < GQA_HD / 8 / LANES; ++k) {
         float x[8];
         row.load(LANES * k + q, x);
@@ -184,7 +185,7 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
             row.store(c, a);
             row.store(c + hc, b);
         }
-#pragma unroll 3
+#pragma unroll 1
         for (int c = (rot >> 3) + q; c < GQA_HD / 8; c += LANES) {
             float a[8], wa[8];
             row.load(c, a);
