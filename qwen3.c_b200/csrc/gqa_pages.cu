@@ -295,6 +295,7 @@ struct PdSmem {
     alignas(16) float w1[2][GQA_HD];        // 1 + q / k norm weights
     alignas(16) float cs[PD_WARPS][GQA_HD / 2], sn[PD_WARPS][GQA_HD / 2];
     unsigned long long turn[GQA_HD / 2];
+    double2 turned[PD_WARPS][GQA_HD / 2];   // (cos, sin) of the row to append (fp32 activations)
     float2 ml[PD_WARPS][2][GQA_GRP];        // (max, sum) of a warp's continued / opened piece
     int4 cont[PD_WARPS], open[PD_WARPS];    // (there: 1, and ends here: 2; request; KV head; parked / last CTA)
     int pre[1024 + 4];                      // entries (of one KV head) before each request
@@ -527,8 +528,40 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                     const TI *raw = reinterpret_cast<const TI *>(st + E::KV);
                     float x[8], w1[8];
                     load8<TI>(raw + lane * 8, x);
-                    load8<float>(sm.w1[1] + lane * 8, w1);
-                    pages_norm_rope(x, w1, p.eps, p.rot, cs, sn, raw, sm.w1[1], lane);
+                    if constexpr (E::F32) {
+                        // in double up to its rounding: fp32 outputs show it where an element of
+                        // the cached row falls to the other side of a bf16 border
+                        double s2 = 0.0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s2 += (double)x[e] * x[e];
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+                        const double a = s2 * (1.0 / GQA_HD) + p.eps, r0 = rsqrtf((float)a), r = r0 * (1.5 - 0.5 * a * r0 * r0);
+                        const int half = p.rot >> 1;
+#pragma unroll 1
+                        for (int j = lane; j < half; j += 32) {
+                            double2 t;
+                            sincospi((double)(long long)((unsigned long long)pos * sm.turn[j]) * 0x1p-63, &t.y, &t.x);
+                            sm.turned[warp][j] = t;
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int d = lane * 8 + e;
+                            double y = x[e] * r * (1.0 + p.knw[d]);
+                            if (d < p.rot) {
+                                const bool low = d < half;
+                                const int o = low ? d + half : d - half;
+                                const double2 t = sm.turned[warp][low ? d : o];
+                                const double z = raw[o] * r * (1.0 + p.knw[o]);
+                                y = low ? y * t.x - z * t.y : y * t.x + z * t.y;
+                            }
+                            x[e] = (float)y;
+                        }
+                    } else {
+                        load8<float>(sm.w1[1] + lane * 8, w1);
+                        pages_norm_rope(x, w1, p.eps, p.rot, cs, sn, raw, sm.w1[1], lane);
+                    }
                     new_k = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
                 }
                 // heads past the group's: q = 0 (what lies there is finite or not: cleared, not scaled)
