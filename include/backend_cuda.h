@@ -370,12 +370,13 @@ int  coli_cuda_gdn_full_route(int layer, const float *x_in, const float *resid, 
  * device. page is a multiple of 16 up to 1024, hd = 256, H / KH is 1, 2, 4
  * or 8, n_pages <= 2^20, KH * page * n_pages < 2^31.
  *
- * Every call below takes device pointers and runs asynchronously on the
- * backend stream; none allocates, frees or synchronises, so each can be
- * captured into a graph. They use the handle's one workspace: calls on one
- * handle that may overlap on the GPU (two streams, two graphs in flight) need
- * a workspace of their own (set_workspace before the call or its capture),
- * beside touching different pages.
+ * The operators (gqa_*_pages_dev, pages_copy / fork / compact_dev) take
+ * device pointers and run asynchronously on the backend stream; none
+ * allocates, frees or synchronises, so each can be captured into a graph.
+ * They use the handle's one workspace: calls on one handle that may overlap
+ * on the GPU (two streams, two graphs in flight) need a workspace of their
+ * own (pages_set_workspace before the call or its capture), beside touching
+ * different pages. The other calls belong outside captures.
  * Page ids, positions, lengths and row offsets are checked on the device:
  * what is out of range is left out (its outputs are undefined, no memory
  * outside the arguments is touched), and the next coli_cuda_sync returns 0
@@ -404,11 +405,14 @@ int    coli_cuda_pages_set_workspace(ColiCudaPages *pages, void *ws, size_t byte
  * each request b < B <= 1024 at its own position pos[b]: q/k norm, RoPE, K/V
  * append, attention over rows 0..pos[b], sigmoid gate), for requests whose
  * rows are in pages. pos[b] < 0 names an idle slot: nothing is appended and
- * its ctx row is left as it was. The page of position pos[b] has to be the
- * request's alone (fork before). dtype 1: bf16 activations; q and the
- * probabilities enter the tensor cores as bf16. dtype 0: fp32 activations; both
- * enter as two bf16 parts, so ctx is good to about 2^-17. RoPE angles are
- * formed in double. qg, k, v, ctx 16-byte aligned. */
+ * its ctx row is left as it was. Each live slot is a request of its own, and
+ * the page of position pos[b] that request's alone (fork before). q and the
+ * probabilities enter the tensor cores as two bf16 parts each with bf16
+ * activations (dtype 1) and as three with fp32 ones (dtype 0), so ctx is good
+ * to about 2^-17 and 2^-21 before its own rounding; the cache is bf16. RoPE
+ * angles are exact products, reduced before the sine (the contiguous calls
+ * form them in fp32, 2e-3 off at position 32768). qg, k, v, ctx 16-byte
+ * aligned. */
 int  coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const void *qg, const void *k,
                                     const void *v, const int *pos_dev, const int *table, int max_pages, void *ctx,
                                     int H, int KH, int hd, int rot, float eps, float theta, int dtype);
@@ -419,7 +423,10 @@ int  coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, cons
  * pos_base[r] ..; they are appended to its pages and attend to rows
  * 0..their own position. A chunk may be empty or a single token (a request
  * that decodes beside others that prefill); rows outside all chunks are left
- * as they were. bf16 activations (dtype 1) only. S <= 2^24. */
+ * as they were. A request has one chunk in a call, and the pages that it is
+ * appended to are that request's alone. q and the probabilities enter the
+ * tensor cores as bf16. bf16 activations (dtype 1) only. S <= 2^24,
+ * max_pages * page <= 2^30 (decode too). */
 int  coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, int S, const int *cu,
                                      const int *pos_base, const void *qg, const void *k, const void *v,
                                      const int *table, int max_pages, void *ctx, int H, int KH, int hd, int rot,

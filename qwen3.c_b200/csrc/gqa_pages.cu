@@ -48,20 +48,19 @@ __device__ __forceinline__ float gate_of(float x) { return rcp_approx(1.f + ex2_
 // o *= sigmoid(g) for four elements, e^g / (1 + e^g) with one reciprocal of the
 // product of the four 1 + e^g: 5 special-function instructions instead of 8, which
 // bound the epilogues. Above 20 a sigmoid is 1 in fp32; held there, the product
-// stays below 6e34.
+// stays below 6e34. A NaN gate is kept out of it, so that it is its own element's only.
 __device__ __forceinline__ void gate4(float *o, const float *g)
 {
     float e[4], d[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        e[i] = ex2_approx((g[i] > 20.f ? 20.f : g[i]) * 1.4426950408889634f);
+        e[i] = ex2_approx(fminf(g[i], 20.f) * 1.4426950408889634f);       // fminf(NaN, 20) = 20
         d[i] = 1.f + e[i];
     }
     const float d01 = d[0] * d[1], d23 = d[2] * d[3], r = rcp_approx(d01 * d23), r01 = r * d23, r23 = r * d01;
-    o[0] *= e[0] * d[1] * r01;
-    o[1] *= e[1] * d[0] * r01;
-    o[2] *= e[2] * d[3] * r23;
-    o[3] *= e[3] * d[2] * r23;
+    const float s[4] = {e[0] * d[1] * r01, e[1] * d[0] * r01, e[2] * d[3] * r23, e[3] * d[2] * r23};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= g[i] == g[i] ? s[i] : g[i];
 }
 __device__ __forceinline__ float rms_factor(float s2, float eps)     // 1 / sqrt(s2 / hd + eps), one Newton step
 {

@@ -195,17 +195,17 @@ pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
 // Moves the pages and writes the new table: every entry, those behind a
 // request's length as they are.
 __global__ void __launch_bounds__(MV_THREADS)
-pages_compact_move_kernel(PageMoveArgs m, PageCompactArgs c)
+pages_compact_move_kernel(PageMoveArgs m, PageCompactArgs c, int piece)
 {
     griddep_wait();                         // a programmatic dependent of the plan
     const int movers = *c.count, live = *c.live, words = (int)(m.page_bytes / 16);
     // blockIdx.y: a plane and a piece of the page; blockIdx.x and on: the movers, the next one's ids ahead
-    const int pieces = (words + CP_PIECE - 1) / CP_PIECE, plane = blockIdx.y / pieces, at = (blockIdx.y - plane * pieces) * CP_PIECE;
+    const int pieces = (words + piece - 1) / piece, plane = blockIdx.y / pieces, at = (blockIdx.y - plane * pieces) * piece;
     int k = blockIdx.x, from = k < movers ? c.src[k] : 0, to = k < movers ? c.dst[k] : 0;
     while (k < movers) {
         k += gridDim.x;
         const int next_from = k < movers ? c.src[k] : 0, next_to = k < movers ? c.dst[k] : 0;
-        copy_words(page_at(m, plane, to) + at, page_at(m, plane, from) + at, min(CP_PIECE, words - at));
+        copy_words(page_at(m, plane, to) + at, page_at(m, plane, from) + at, min(piece, words - at));
         from = next_from;
         to = next_to;
     }
@@ -231,9 +231,11 @@ cudaError_t launch_pages_compact(const PageMoveArgs &m, const PageCompactArgs &c
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    const int words = (int)(m.page_bytes / 16), rows = 2 * m.layers * ((words + CP_PIECE - 1) / CP_PIECE);
+    // pieces of a page: small enough that few pages fill the GPU, few enough for the grid's y
+    const int words = (int)(m.page_bytes / 16), most = 65535 / (2 * m.layers), piece = std::max(CP_PIECE, (words + most - 1) / most);
+    const int rows = 2 * m.layers * ((words + piece - 1) / piece);
     cfg.gridDim = dim3(std::max(1, std::min(m.n_pages, (CP_CTAS + rows - 1) / rows)), rows); cfg.blockDim = dim3(MV_THREADS); cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, pages_compact_move_kernel, m, c);
+    return cudaLaunchKernelEx(&cfg, pages_compact_move_kernel, m, c, piece);
 }
 
 }  // namespace coli

@@ -101,8 +101,27 @@ void pages_release(ColiCudaPages *p)
     delete p;
 }
 
+// Handles freed while the backend stream was capturing: freeing memory there
+// would end the capture, so it waits for the next call that may.
+ColiCudaPages *g_pages_freed[PAGES_MAX_HANDLES] = {};
+bool pages_capturing()
+{
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(stream(), &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+void pages_release_freed()
+{
+    for (int i = 0; i < PAGES_MAX_HANDLES; ++i) {
+        if (!g_pages_freed[i]) continue;
+        cudaStreamSynchronize(stream());   // queued calls may still use the pool and the workspace
+        pages_release(g_pages_freed[i]);
+        g_pages_freed[i] = nullptr;
+    }
+}
+
 void pages_shutdown()
 {
+    pages_release_freed();
     for (int i = 0; i < PAGES_MAX_HANDLES; ++i) {
         if (g_pages[i]) pages_release(g_pages[i]);
         g_pages[i] = nullptr;
@@ -151,6 +170,7 @@ int pages_attend_args(GqaPagesArgs &a, ColiCudaPages *p, int layer, const void *
     if (!qg || !k || !v || !base || !table || !ctx) return fail("pages: a null pointer among the arguments");
     if (((uintptr_t)qg | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ctx) & 15)
         return fail("pages: qg, k, v and ctx must be 16-byte aligned");
+    if (((uintptr_t)base | (uintptr_t)table) & 3) return fail("pages: index arrays must be 4-byte aligned");
     if (p->rot != rot || p->theta != theta) {
         for (int j = 0; j < rot / 2; ++j) {
             const double t = std::pow((double)theta, -2.0 * j / rot) / 6.283185307179586476925286766559;
@@ -201,6 +221,8 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
     if (!pages) return fail("pages: null handle");
     if (!pages_geometry(layers, n_pages, page, KH, hd)) return 0;
     if ((uintptr_t)kv_dev & 127) return fail("pages: kv_dev must be 128-byte aligned");
+    if (pages_capturing()) return fail("pages: a pool cannot be made while the backend stream is capturing");
+    pages_release_freed();
     int slot = 0;
     while (slot < PAGES_MAX_HANDLES && g_pages[slot]) ++slot;
     if (slot == PAGES_MAX_HANDLES) return fail("pages: %d handles are alive already", PAGES_MAX_HANDLES);
@@ -239,9 +261,11 @@ void coli_cuda_pages_free(ColiCudaPages *pages)
     if (!pages) return;
     for (int i = 0; i < PAGES_MAX_HANDLES; ++i) {
         if (g_pages[i] != pages) continue;
-        cudaStreamSynchronize(stream());   // queued calls may still use the pool and the workspace
-        pages_release(pages);
+        if (g_pages_freed[i]) return;      // as many are waiting for a capture to end as there can be handles
         g_pages[i] = nullptr;
+        g_pages_freed[i] = pages;
+        if (!pages_capturing()) pages_release_freed();
+        return;
     }
 }
 
@@ -260,6 +284,7 @@ int coli_cuda_pages_norm_weight(ColiCudaPages *pages, int layer, const float *qn
     if (!pages_handle(pages)) return 0;
     if (layer < 0 || layer >= pages->layers) return fail("pages: layer %d out of range", layer);
     if (hd != GQA_HD || !qnw || !knw) return fail("pages: bad norm weights (hd=%d)", hd);
+    if (pages_capturing()) return fail("pages: norm weights cannot be set while the backend stream is capturing");
     float *d = pages->norm_w + (size_t)layer * 2 * GQA_HD;
     CK(cudaMemcpyAsync(d, qnw, GQA_HD * 4, cudaMemcpyHostToDevice, stream()));
     CK(cudaMemcpyAsync(d + GQA_HD, knw, GQA_HD * 4, cudaMemcpyHostToDevice, stream()));
@@ -292,8 +317,8 @@ int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const
     if (B == 0) return 1;
     GqaPagesArgs a{};
     if (!pages_attend_args(a, pages, layer, qg, k, v, pos_dev, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
-    if ((long long)B * pages->KH * max_pages * (pages->page / 16) > 0x7fffffffLL)
-        return fail("pages: a table of %d x %d pages passes 2^31 tiles", B, max_pages);
+    if (((long long)max_pages * (pages->page / GQA_TILE) + PD_EXTRA + 3) * B * pages->KH > 1 << 30)
+        return fail("pages: a table of %d x %d pages passes 2^30 tiles", B, max_pages);
     a.n_req = a.S = B;
     g_pages_ran = true;
     CK(launch_pages_decode(pages->maps[4 * layer], a, pages_part(pages->ws), pages->freq, dtype,
@@ -312,6 +337,7 @@ int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, 
     if (S < 0 || S > 1 << 24) return fail("pages: %d rows out of 0..2^24", S);
     if (n_seq == 0 || S == 0) return 1;
     if (!cu) return fail("pages: a null pointer among the arguments");
+    if ((uintptr_t)cu & 3) return fail("pages: index arrays must be 4-byte aligned");
     GqaPagesArgs a{};
     if (!pages_attend_args(a, pages, layer, qg, k, v, pos_base, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
     a.cu = cu;
@@ -332,6 +358,7 @@ int coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const 
     if (n < 0 || n > pages->n_pages) return fail("pages: %d pairs for %d pages", n, pages->n_pages);
     if (n == 0) return 1;
     if (!src || !dst) return fail("pages: a null pointer among the arguments");
+    if (((uintptr_t)src | (uintptr_t)dst) & 3) return fail("pages: index arrays must be 4-byte aligned");
     g_pages_ran = true;
     CK(launch_pages_copy(pages_move_args(pages), n, src, dst, stream()));
     g_launches += 1;
@@ -347,6 +374,8 @@ int coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, con
     if (n < 0 || n >= n_req) return fail("pages: %d forks among %d requests", n, n_req);
     if (n == 0) return 1;
     if (!parent || !child || !fresh || !len || !table) return fail("pages: a null pointer among the arguments");
+    if (((uintptr_t)parent | (uintptr_t)child | (uintptr_t)fresh | (uintptr_t)len | (uintptr_t)table) & 3)
+        return fail("pages: index arrays must be 4-byte aligned");
     PageForkArgs f{};
     f.parent = parent; f.child = child; f.fresh = fresh; f.len = len; f.table = table;
     f.n = n; f.n_req = n_req; f.max_pages = max_pages;
@@ -363,6 +392,8 @@ int coli_cuda_pages_compact_dev(ColiCudaPages *pages, int n_req, const int *len,
     if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 1 << 30)
         return fail("pages: bad table %d x %d", n_req, max_pages);
     if (!len || !table || !table_out || !live) return fail("pages: a null pointer among the arguments");
+    if (((uintptr_t)len | (uintptr_t)table | (uintptr_t)table_out | (uintptr_t)live) & 3)
+        return fail("pages: index arrays must be 4-byte aligned");
     PageCompactArgs c{};
     const size_t list = pages_list_bytes(pages->n_pages);
     c.len = len; c.table = table; c.table_out = table_out; c.live = live;

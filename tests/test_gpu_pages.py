@@ -492,3 +492,309 @@ def test_serving_run_matches_contiguous_cache(be):
     np.testing.assert_array_equal(td.cpu().numpy(), want_table)
     steps(3)
     be.kv_reset()
+
+
+def test_compact_twice_is_the_identity(be):
+    """A compacted pool has nothing to move: the table stays, no page changes."""
+    P = Pool(be, 120, 16, 1, 3, seed=7)
+    lens = [100, 0, 333, 16, 5]
+    table = pages_for(lens, 16, 120, seed=2)
+    table[table == 1 << 30] = -1
+    ld, td, lv = ints(lens), ints(table), ints([0])
+    for _ in range(2):
+        P.cache.compact_dev(5, ld.data_ptr(), td.data_ptr(), table.shape[1], td.data_ptr(), lv.data_ptr())
+    be.sync()
+    want, live, _ = ref.compact(table, lens, 16, 120)
+    np.testing.assert_array_equal(td.cpu().numpy(), want)
+    again, live2, moves = ref.compact(want, lens, 16, 120)
+    assert lv.item() == live == live2 and not moves and np.array_equal(again, want)
+
+
+# the most requests of a call, some idle, and more of them than a warp counts alone
+@pytest.mark.parametrize("B,KH,group,dtype", [(1024, 1, 2, 1), (33, 2, 8, 0), (200, 3, 4, 1)])
+def test_decode_many_requests(be, B, KH, group, dtype):
+    rng = np.random.default_rng(B)
+    lens = [int(n) for n in rng.integers(0, 70, size=B)]
+    page = 16
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    P = Pool(be, n_pages, page, KH, seed=B)
+    table = pages_for(lens, page, n_pages, seed=B)
+    poison(P, table, lens)
+    before = P.host()
+    qg, k, v, ctx = P.inputs(B, KH * group, dtype)
+    pos, td = ints([n - 1 for n in lens]), ints(table)
+    P.cache.decode_dev(0, B, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), table.shape[1],
+                       ctx.data_ptr(), H=KH * group, rot=ROT, eps=EPS, theta=THETA, dtype=dtype)
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, table, [(r, r, n - 1) for r, n in enumerate(lens) if n], group, dtype)
+    for r, n in enumerate(lens):
+        if not n:
+            assert (ctx[r] == 7).all()
+
+
+def test_all_slots_idle(be):
+    P = Pool(be, 4, 16, 2, seed=1)
+    before = P.kv.clone()
+    qg, k, v, ctx = P.inputs(3, 16, 1)
+    pos, td = ints([-1, -1, -7]), ints([[0], [1], [2]])
+    P.cache.decode_dev(0, 3, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), 1, ctx.data_ptr())
+    cu, base = ints([0, 0, 0, 0]), ints([5, -1, 0])
+    P.cache.prefill_dev(0, 3, 3, cu.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(), td.data_ptr(), 1,
+                        ctx.data_ptr())
+    be.sync()
+    assert (ctx == 7).all() and P.torch.equal(P.kv, before)
+
+
+def test_prefill_many_chunks(be):
+    """The most chunks of a call, most of them empty or a token long."""
+    rng = np.random.default_rng(3)
+    chunks = [(int(n), int(c)) for n, c in zip(rng.integers(0, 3, size=1024), rng.integers(0, 40, size=1024))]
+    page, KH, group = 16, 1, 8
+    total = [n + c if n else 0 for n, c in chunks]
+    n_pages = sum(-(-n // page) for n in total) + 1
+    P = Pool(be, n_pages, page, KH, seed=4)
+    table = pages_for(total, page, n_pages, seed=4)
+    poison(P, table, total)
+    before = P.host()
+    cu = np.concatenate([[0], np.cumsum([n for n, _ in chunks])])
+    qg, k, v, ctx = P.inputs(int(cu[-1]), KH * group, 1)
+    cu_d, base, td = ints(cu), ints([c for _, c in chunks]), ints(table)
+    P.cache.prefill_dev(0, 1024, int(cu[-1]), cu_d.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(),
+                        td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group)
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, table, [(int(cu[r]) + i, r, c + i) for r, (n, c) in enumerate(chunks) for i in range(n)],
+               group, 1)
+
+
+@pytest.mark.parametrize("rot,group", [(256, 1), (256, 8), (36, 2), (2, 4)])
+def test_prefill_rotary_widths(be, rot, group):
+    page, KH = 32, 2
+    chunks = [(150, 10), (9, 77)]
+    total = [n + c for n, c in chunks]
+    P = Pool(be, 12, page, KH, seed=rot + group)
+    table = pages_for(total, page, 12, seed=1)
+    before = P.host()
+    qg, k, v, ctx = P.inputs(159, KH * group, 1)
+    cu, base, td = ints([0, 150, 159]), ints([10, 77]), ints(table)
+    P.cache.prefill_dev(0, 2, 159, cu.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(), td.data_ptr(),
+                        table.shape[1], ctx.data_ptr(), H=KH * group, rot=rot, theta=5e5)
+    be.sync()
+    placed = [(i, 0, 10 + i) for i in range(150)] + [(150 + i, 1, 77 + i) for i in range(9)]
+    check_rows(P, before, qg, k, v, ctx, table, placed, group, 1, rot, 5e5)
+
+
+def test_gate_extremes(be):
+    """Gates of +-infinity, the type's lowest and highest values, NaN: 0, 1, 0, 1 and NaN times the attention."""
+    import torch
+    P = Pool(be, 8, 16, 1, seed=3)
+    edge = [float("-inf"), float("inf"), -3.38e38, 3.38e38, -100.0, 100.0, 20.5, float("nan")]
+    for dtype in (0, 1):
+        qg, k, v, ctx = P.inputs(2, 8, dtype)
+        qg[:, :, HD:HD + 8] = torch.tensor(edge, device="cuda").to(qg.dtype)
+        table, td = np.array([[0, 1, 2], [3, 4, 5]], np.int32), ints([[0, 1, 2], [3, 4, 5]])
+        pos = ints([0, 40])
+        P.cache.decode_dev(0, 2, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), 3, ctx.data_ptr(),
+                           H=8, dtype=dtype)
+        be.sync()
+        got = ctx[0, :, :8].double().cpu().numpy()       # one key: the attention is its v row
+        want = v[0, 0, :8].bfloat16().double().cpu().numpy()
+        assert np.isnan(got[:, 7]).all()
+        np.testing.assert_array_equal(got[:, [0, 2]], 0)
+        np.testing.assert_allclose(got[:, [1, 3, 5, 6]], np.tile(want[[1, 3, 5, 6]], (8, 1)), rtol=2.0 ** -8 + 1e-6)
+        assert (np.abs(got[:, 4]) < 1e-37).all()
+
+
+def test_offsets_beyond_32_bits(be):
+    """Pages whose elements lie past 2^31 and whose bytes lie past 2^32: decode, prefill, copy, fork and compaction there."""
+    import torch
+    page, KH, n_pages = 64, 2, 70000                     # 2.3e9 elements, 4.6 GB, to a plane
+    kv = torch.empty(1, 2, n_pages, KH, page, HD, dtype=torch.bfloat16, device="cuda")
+    far = list(range(n_pages - 12, n_pages))
+    kv[:, :, far] = torch.randn(1, 2, 12, KH, page, HD, device="cuda").bfloat16()
+    kv[:, :, :4] = 0
+    cache = load_pkg().PagedCache(be, 1, n_pages, page, KH, kv=kv.data_ptr())
+    zero = np.zeros(HD, np.float32)
+    cache.norm_weight(0, zero, zero)
+
+    class View:                                          # what check_rows looks at: the far pages as pages 0 .. 11
+        knw = qnw = zero
+
+        def host(self):
+            return kv[0][:, far].float().cpu().numpy().astype(np.float64)
+
+    View.page = page
+    P = View()
+    near = np.array([[0, 1, 2], [3, 4, 5]], np.int32)
+    td = ints(near + n_pages - 12)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda").bfloat16()   # noqa: E731
+    qg, k, v, ctx = rnd(2, 16, 2 * HD), rnd(2, KH, HD), rnd(2, KH, HD), torch.zeros(2, 16, HD, dtype=torch.bfloat16, device="cuda")
+    before = P.host()
+    pos = ints([190, 100])
+    cache.decode_dev(0, 2, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), 3, ctx.data_ptr())
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, near, [(0, 0, 190), (1, 1, 100)], 8, 1)
+    qg, k, v, ctx = rnd(40, 16, 2 * HD), rnd(40, KH, HD), rnd(40, KH, HD), torch.zeros(40, 16, HD, dtype=torch.bfloat16, device="cuda")
+    before = P.host()
+    cu, base = ints([0, 30, 40]), ints([150, 101])
+    cache.prefill_dev(0, 2, 40, cu.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(), td.data_ptr(), 3, ctx.data_ptr())
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, near, [(i, 0, 150 + i) for i in range(30)] + [(30 + i, 1, 101 + i) for i in range(10)], 8, 1)
+    src, dst = ints([n_pages - 12]), ints([n_pages - 1])
+    cache.copy_dev(1, src.data_ptr(), dst.data_ptr())
+    table, ln = ints([[n_pages - 12, n_pages - 11], [0, 0]]), ints([100, 0])
+    par, chi, fre = ints([0]), ints([1]), ints([n_pages - 2])
+    cache.fork_dev(1, par.data_ptr(), chi.data_ptr(), fre.data_ptr(), ln.data_ptr(), table.data_ptr(), 2, 2)
+    be.sync()
+    assert torch.equal(kv[:, :, n_pages - 1], kv[:, :, n_pages - 12])
+    assert table.tolist() == [[n_pages - 12, n_pages - 11], [n_pages - 12, n_pages - 2]] and ln.tolist() == [100, 100]
+    assert torch.equal(kv[:, :, n_pages - 2, :, :36], kv[:, :, n_pages - 11, :, :36])
+    live = ints([0])
+    want = [kv[:, :, i].clone() for i in (n_pages - 12, n_pages - 11, n_pages - 2)]
+    cache.compact_dev(2, ln.data_ptr(), table.data_ptr(), 2, table.data_ptr(), live.data_ptr())
+    be.sync()
+    assert live.item() == 3 and table.tolist() == [[0, 1], [0, 2]]
+    for i, w in enumerate(want):
+        assert torch.equal(kv[:, :, i], w)
+    cache.free()
+
+
+def test_two_graphs_in_flight_with_their_own_workspaces(be):
+    """Two captured steps of one handle on two streams, split units in both, replayed together many times."""
+    import torch
+    P = Pool(be, 1100, 16, 2, 2, seed=8)
+    R = 4
+    lens = [[4000, 33, 700, 3000], [2500, 4000, 1, 90]]
+    ids = np.random.default_rng(4).permutation(1100)
+    tables, at = [], 0
+    for group_lens in lens:
+        t = np.full((R, 256), 1 << 30, np.int32)
+        for r, n in enumerate(group_lens):
+            c = -(-n // 16)
+            t[r, :c] = ids[at:at + c]
+            at += c
+        tables.append(ints(t))
+    pos = [ints([n - 1 for n in group_lens]) for group_lens in lens]
+    x = [P.inputs(R, 16, 1) for _ in lens]
+    chunk = [P.inputs(20, 16, 1) for _ in lens]
+    cu, base = ints([0, 20]), [ints([lens[i][1] - 1]) for i in (0, 1)]
+    ws = [None, torch.empty(P.cache.workspace_bytes(), dtype=torch.uint8, device="cuda")]
+    streams, graphs = [torch.cuda.Stream() for _ in lens], []
+
+    def step(i):
+        qg, k, v, ctx = (t.data_ptr() for t in x[i])
+        P.cache.decode_dev(i, R, qg, k, v, pos[i].data_ptr(), tables[i].data_ptr(), 256, ctx)
+        qg, k, v, ctx = (t.data_ptr() for t in chunk[i])
+        # the second request goes on with 20 rows
+        P.cache.prefill_dev(i, 1, 20, cu.data_ptr(), base[i].data_ptr(), qg, k, v, tables[i][1].data_ptr(), 256, ctx)
+
+    # room for the 20 rows
+    for i in (0, 1):
+        c = -(-lens[i][1] // 16)
+        extra = min(256, c + 2) - c
+        tables[i][1, c:c + extra] = ints(ids[at:at + extra])
+        at += extra
+        base[i].clamp_(max=256 * 16 - 20)
+    want = []
+    for i in (0, 1):
+        step(i)
+        be.sync()
+        want.append((x[i][3].clone(), chunk[i][3].clone()))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        if ws[i] is not None:
+            P.cache.set_workspace(ws[i].data_ptr(), ws[i].numel())
+        be.set_stream(streams[i].cuda_stream)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i], capture_error_mode="thread_local"):
+            step(i)
+        graphs.append(g)
+    P.cache.set_workspace()
+    be.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    for i in (0, 1):
+        x[i][3].zero_()
+        chunk[i][3].zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    be.sync()
+    for i in (0, 1):
+        assert torch.equal(x[i][3], want[i][0]) and torch.equal(chunk[i][3], want[i][1])
+
+
+def test_moves_replay_from_a_graph(be):
+    """Copy, fork and compaction captured once and replayed on new contents."""
+    import torch
+    P = Pool(be, 40, 16, 2, 2, seed=6)
+    table = np.full((4, 4), -1, np.int32)
+    table[0, :3], table[1, :1] = [30, 7, 21], [12]
+    td0, ln0 = ints(table), ints([40, 9, 0, 0])
+    td, ln, lv = td0.clone(), ln0.clone(), ints([0])
+    src, dst = ints([30]), ints([33])
+    par, chi, fre = ints([0, 1]), ints([2, 3]), ints([25, 26])
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    be.set_stream(st.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+        P.cache.copy_dev(1, src.data_ptr(), dst.data_ptr())
+        P.cache.fork_dev(2, par.data_ptr(), chi.data_ptr(), fre.data_ptr(), ln.data_ptr(), td.data_ptr(), 4, 4)
+        P.cache.compact_dev(4, ln.data_ptr(), td.data_ptr(), 4, td.data_ptr(), lv.data_ptr())
+    be.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    for _ in range(3):
+        P.kv.copy_(P.randn(*P.kv.shape).bfloat16())
+        td.copy_(td0)
+        ln.copy_(ln0)
+        kv = P.kv.clone()
+        kv[:, :, 33] = kv[:, :, 30]
+        Q = type("Q", (), dict(kv=kv, page=16))
+        kv, t1, l1 = fork_want(Q, table, [40, 9, 0, 0], [0, 1], [2, 3], [25, 26])
+        want, live, moves = ref.compact(t1, l1, 16, 40)
+        s, d = (list(z) for z in zip(*moves))
+        after = kv.clone()
+        after[:, :, d] = kv[:, :, s]
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        be.sync()
+        np.testing.assert_array_equal(td.cpu().numpy(), want)
+        assert lv.item() == live and ln.tolist() == l1
+        assert torch.equal(P.kv.view(torch.int16), after.view(torch.int16))
+
+
+def test_a_pool_of_its_own_and_handles_that_end(be):
+    """Library-owned memory: zeroed, counted, given back; the most handles; a handle freed while its stream captures."""
+    import torch
+    pkg = load_pkg()
+    before = be.mem_info()
+    c = pkg.PagedCache(be, 2, 8, 16, 1)
+    assert pkg.PagedCache.nbytes_for(be, 2, 8, 16, 1) == 2 * 2 * 8 * 16 * 512
+    k0, v0 = c.device_ptr(0)
+    k1, _ = c.device_ptr(1)
+    assert v0 - k0 == 8 * 16 * 512 and k1 - k0 == 2 * 8 * 16 * 512
+    be.sync()
+    c.free()
+    assert be.mem_info() == before
+    many = [pkg.PagedCache(be, 1, 1, 16, 1) for _ in range(8)]
+    st = torch.cuda.Stream()
+    x = ints([0])
+    y = ints([0])
+    torch.cuda.synchronize()
+    be.set_stream(st.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st, capture_error_mode="thread_local"):
+        many[0].copy_dev(1, x.data_ptr(), y.data_ptr())
+        many[1].free()
+        with pytest.raises(pkg.BackendError, match="capturing"):
+            pkg.PagedCache(be, 1, 1, 16, 1)
+    be.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    g.replay()
+    torch.cuda.synchronize()
+    del g
+    for m in many:
+        m.free()
+    be.sync()
+    assert be.mem_info() == before
