@@ -1005,7 +1005,7 @@ __device__ __forceinline__ void pp_plan(const GqaPagesArgs &p, int cta, int ctas
     long long at = inc - mine;
     for (int w = 0; w < warp; ++w) at += sums[w];
 #pragma unroll 1
-    for (int r = r0; r < r1; ++r) { pre[r] = at; at += pp_chunk_work(p, r, gs); }
+    for (int r = r0; r < r1; ++r) { pre[r] = at; at += r + 1 < r1 || r > r0 ? pp_chunk_work(p, r, gs) : mine; }
     if (tid == PP_THREADS - 1) pre[p.n_req] = at;
     __syncthreads();
     if (warp < 2) {                         // a warp per range, 32 places looked at at a time

@@ -118,27 +118,33 @@ cudaError_t launch_pages_fork(const PageMoveArgs &m, const PageForkArgs &f, cuda
 // ------------------------------------------------------------------ compact
 constexpr int CP_THREADS = 1024, CP_PIECE = 8 * MV_THREADS, CP_CTAS = 148 * 32;
 
-// Exclusive prefix sum over the CTA's threads; `total` is every thread's sum.
-__device__ __forceinline__ int block_scan(int x, int &total)
+// Exclusive prefix sums over the CTA's threads of two counts at once (low and
+// high half); `total` is every thread's sums.
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long x, unsigned long long &total)
 {
-    __shared__ int part[CP_THREADS / 32];
+    __shared__ unsigned long long part[CP_THREADS / 32 + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc = x;
+    auto scan = [&](unsigned long long v) {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += y;
-    }
+        for (int d = 1; d < 32; d <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= d) v += y;
+        }
+        return v;
+    };
+    const unsigned long long inc = scan(x);
     if (lane == 31) part[warp] = inc;
     __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < CP_THREADS / 32; ++w) {
-        if (w < warp) before += part[w];
-        all += part[w];
+    if (warp == 0) {                        // CP_THREADS / 32 = 32 warps
+        const unsigned long long mine = part[lane], all = scan(mine);
+        __syncwarp();
+        part[lane] = all - mine;
+        if (lane == 31) part[32] = all;
     }
     __syncthreads();
-    total = all;
+    total = part[32];
+    const unsigned long long before = part[warp];
+    __syncthreads();                        // the next scan writes here
     return before + inc - x;
 }
 
@@ -173,14 +179,16 @@ pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
     }
     __syncthreads();
     const int per = (words + CP_THREADS - 1) / CP_THREADS, w0 = min(words, tid * per), w1 = min(words, w0 + per);
-    int mine = 0, live, holes, movers;
+    unsigned long long mine = 0, total;
     for (int w = w0; w < w1; ++w) mine += __popc(bits[w]);
-    block_scan(mine, live);
+    block_scan(mine, total);
+    const int live = (int)total;
     // of word w: the dead pages before `live`, and the live ones from there on
     auto low = [&](int w) { return w * 32 + 32 <= live ? ~0u : w * 32 >= live ? 0u : (1u << (live - w * 32)) - 1; };
-    int nh = 0, nm = 0;
-    for (int w = w0; w < w1; ++w) { nh += __popc(~bits[w] & low(w)); nm += __popc(bits[w] & ~low(w)); }
-    int h = block_scan(nh, holes), v = block_scan(nm, movers);
+    mine = 0;
+    for (int w = w0; w < w1; ++w) mine += __popc(~bits[w] & low(w)) + ((unsigned long long)__popc(bits[w] & ~low(w)) << 32);
+    const unsigned long long at = block_scan(mine, total);
+    int h = (int)at, v = (int)(at >> 32);
     for (int w = w0; w < w1; ++w) {
         for (uint32_t x = ~bits[w] & low(w); x; x &= x - 1) c.dst[h++] = w * 32 + __ffs(x) - 1;
         for (uint32_t x = bits[w] & ~low(w); x; x &= x - 1) {
@@ -189,7 +197,7 @@ pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
             c.src[v++] = id;
         }
     }
-    if (tid == 0) { *c.count = movers; *c.live = live; }
+    if (tid == 0) { *c.count = (int)(total >> 32); *c.live = live; }
 }
 
 // Moves the pages and writes the new table: every entry, those behind a
