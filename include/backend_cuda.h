@@ -425,7 +425,9 @@ int  coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, cons
  * that decodes beside others that prefill); rows outside all chunks are left
  * as they were. A request has one chunk in a call, and the pages that it is
  * appended to are that request's alone. q and the probabilities enter the
- * tensor cores as bf16. bf16 activations (dtype 1) only. S <= 2^24,
+ * tensor cores as bf16. A non-finite v row of the chunk itself can reach rows
+ * up to 127 positions before it (0 * inf in the matrix product); stale rows of
+ * pages, of whatever contents, reach none. bf16 activations (dtype 1) only. S <= 2^24,
  * max_pages * page <= 2^30 (decode too). */
 int  coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, int S, const int *cu,
                                      const int *pos_base, const void *qg, const void *k, const void *v,
@@ -439,7 +441,7 @@ int  coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const
 /* Request child[i] becomes a copy of request parent[i], i < n < n_req: it
  * shares the pages that the parent has filled, len[child] = len[parent], and
  * where the parent's last page is only started, its rows are copied to page
- * fresh[i] (else fresh[i] is not used). A parent may have many children; a
+ * fresh[i], which no request holds (else fresh[i] is not used). A parent may have many children; a
  * child named twice or also as a parent, and a fresh page named twice, are
  * left out and reported. len int32 [n_req], table int32 [n_req][max_pages]. */
 int  coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, const int *child, const int *fresh,

@@ -123,7 +123,6 @@ template <typename TI> struct Raw8;
 template <> struct Raw8<__nv_bfloat16> {
     uint4 u;
     __device__ __forceinline__ void load(const __nv_bfloat16 *src) { u = *reinterpret_cast<const uint4 *>(src); }
-    __device__ __forceinline__ void store(__nv_bfloat16 *dst) const { *reinterpret_cast<uint4 *>(dst) = u; }
     __device__ __forceinline__ void unpack(float (&x)[8]) const
     {
         const __nv_bfloat162 *b = reinterpret_cast<const __nv_bfloat162 *>(&u);
@@ -136,10 +135,6 @@ template <> struct Raw8<float> {
     __device__ __forceinline__ void load(const float *src)
     {
         a = reinterpret_cast<const float4 *>(src)[0]; b = reinterpret_cast<const float4 *>(src)[1];
-    }
-    __device__ __forceinline__ void store(float *dst) const
-    {
-        reinterpret_cast<float4 *>(dst)[0] = a; reinterpret_cast<float4 *>(dst)[1] = b;
     }
     __device__ __forceinline__ void unpack(float (&x)[8]) const
     {

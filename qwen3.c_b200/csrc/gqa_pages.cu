@@ -237,9 +237,16 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
 //
 // Short calls are bound by latency, instruction fetch a large part of it: what
 // runs once per unit is kept in rolled loops over heads.
+//
+// Measured with the join (H / KH = 8, KH = 2 unless said): 64 requests at 32k tokens,
+// 4.25 GB, 651 us, 6.53 TB/s (the device's copies: 6.56); 48 ragged requests of up to 8k
+// tokens, fp32, KH = 4, 305 MB, 57 us replayed from a graph (82 us called one by one behind a
+// flush of L2), 47 us at the copy rate; one request of 4k tokens, 15 us from a graph: the join's
+// launch, 4 us, and one pass through cold instructions.
 constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_STAGES = 3, PD_STAGE = 2 * GQA_TILE_BYTES;
 // Entries that a unit counts more than it has when the list is cut: its q and
-// gate take a warp about as long as PD_EXTRA + 2 tiles.
+// gate take a warp about as long as PD_EXTRA + 2 tiles. With 0, 1, 2, 3, 4: 69, 62, 57, 59,
+// 55 us for the 48 ragged requests, 21.8, 22.5, 20.9, 22.3, 24.5 for 64 of 512 tokens.
 constexpr int PD_EXTRA = 2;
 constexpr int PD_OROW = 132;                 // floats between heads of O: 8 banks apart for the writers' heads
 template <typename TI> struct PdEntry {      // layout of the q entry and of the gate entry in a stage
@@ -936,8 +943,14 @@ cudaError_t launch_pages_decode(const CUtensorMap &tkv, const GqaPagesArgs &a, c
 //   (boxes outside the pool; the last few rows of a group cleared in shared memory),
 //   so non-finite stale rows cannot come through as 0 * inf.
 // TMEM (512 columns): scores 128 | O 256 | Q 128 (bf16 pairs). Q and P are
-// rounded to bf16 (2^-9 of each element): a second part of either would double
+// rounded to bf16 (2^-9 of each element on average): a second part of either would double
 // its MMAs, and the tensor pipe is the bound here.
+// Measured, H / KH = 8, KH = 2: 4096 rows after 28672, 2.06 TFLOP of causal products, 1.55 ms
+// (1.33 PFLOP/s, 0.82 of the GPU's 8192^3 product; up to 1.79 ms under its power cap); nine
+// chunks of up to 1023 rows after up to 4096, 155 GFLOP, 185 us from a graph (0.84 PFLOP/s; masked
+// halves of diagonal tiles, units cut at CTAs' ends and their join are the rest); three short
+// prompts 20 us, latency of three launches. In a tile's 2700 cycles shared memory is read for
+// about 2500 (K and V by the MMAs, P written and read): next to the tensor pipe the second bound.
 constexpr int PP_BM = 128, PP_BN = 128;
 constexpr int PP_TILE = PP_BN * GQA_HD * 2, PP_P = PP_BM * PP_BN * 2;
 constexpr int PP_SOFTMAX = 256, PP_THREADS = 96 + PP_SOFTMAX;
@@ -1033,6 +1046,8 @@ __device__ __forceinline__ void pp_plan(const GqaPagesArgs &p, int cta, int ctas
     __syncthreads();
 }
 
+// One pass over the new rows, bound by HBM for long chunks (4096 rows, KH = 2: 16.8 MB moved) and hidden
+// behind the tiles of earlier rows; a chunk at position 0 waits for it, about 4 us.
 constexpr int PA_WARPS = 8;
 __global__ void __launch_bounds__(PA_WARPS * 32)
 pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
@@ -1516,8 +1531,9 @@ __device__ __forceinline__ bool pp_split_unit(const PagesPart &part, int a, int 
 // rows, 128 dims) adds them up, lane = row, a warp 4 x 4 dims whose loads go out
 // together, then turns the block to write 256-byte runs. Few units (a quarter of
 // the CTAs or less): many pieces each, and one CTA per (unit, 32 rows, 32 dims) has
-// its warps take every eighth of them. 16 rows at 28k: 62 us with
-// the second, 93 with the first.
+// its warps take every eighth of them. A call with 16 rows
+// after 28672 takes 50 us with the second and 93 with the first, one row after 4096 24 and 29; 1024
+// rows (128 units) 45 with the second and 38 with the first, nine mixed chunks 195 and 183.
 constexpr int PJ_THREADS = 256, PJ_DIMS = 128;
 __global__ void __launch_bounds__(PJ_THREADS)
 pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)

@@ -9,7 +9,7 @@
 
 namespace coli {
 
-constexpr int MV_THREADS = 256;
+constexpr int MV_THREADS = 256, MV_CTAS = 148 * 128;
 
 // Page `id` of plane y = 2 * layer + (0 K, 1 V).
 __device__ __forceinline__ uint4 *page_at(const PageMoveArgs &m, int plane, int id)
@@ -32,9 +32,13 @@ __device__ __forceinline__ void copy_words(uint4 *to, const uint4 *from, int wor
 }
 
 // ------------------------------------------------------------------ copy
-// One CTA per (pair, plane). A pair is left out when its destination is
-// named by another pair too, or when its source is another pair's
-// destination: either would make the result a matter of timing.
+// A CTA per pair and as many planes as leave MV_CTAS of them: each looks through all
+// pairs first, which for many pairs and planes would otherwise cost more than the copies
+// (45000 of 8 planes of 16 KiB: 2.98 ms, with a CTA per plane 10.6; 800 of 20 planes of 64 KiB:
+// 319 us, 6.57 TB/s, either way, 327-336 with a quarter and a 16th of the CTAs). 8 pages of
+// 20 planes of 16 KiB: 2.6 us in a graph, the latency of a launch and two dependent loads. A
+// pair is left out when its destination is named by another pair too, or when its source is
+// another pair's destination: either would make the result a matter of timing.
 __global__ void __launch_bounds__(MV_THREADS)
 pages_copy_kernel(PageMoveArgs m, int n, const int *src, const int *dst)
 {
@@ -51,18 +55,24 @@ pages_copy_kernel(PageMoveArgs m, int n, const int *src, const int *dst)
         return;
     }
     if (s == d) return;
-    copy_words(page_at(m, blockIdx.y, d), page_at(m, blockIdx.y, s), (int)(m.page_bytes / 16));
+    for (int y = blockIdx.y; y < 2 * m.layers; y += gridDim.y)
+        copy_words(page_at(m, y, d), page_at(m, y, s), (int)(m.page_bytes / 16));
 }
+
+// CTAs for n items in y, so that x * y come to about MV_CTAS.
+static int mv_rows(const PageMoveArgs &m, int n) { return std::max(1, std::min(2 * m.layers, (MV_CTAS + n - 1) / n)); }
 
 cudaError_t launch_pages_copy(const PageMoveArgs &m, int n, const int *src, const int *dst, cudaStream_t st)
 {
-    pages_copy_kernel<<<dim3(n, 2 * m.layers), MV_THREADS, 0, st>>>(m, n, src, dst);
+    pages_copy_kernel<<<dim3(n, mv_rows(m, n)), MV_THREADS, 0, st>>>(m, n, src, dst);
     return cudaGetLastError();
 }
 
 // ------------------------------------------------------------------ fork
-// One CTA per (fork, plane): the parent's started page is copied as far as
-// it is filled; the CTAs of plane 0 write the child's table row and length.
+// CTAs as in a copy, per fork: the parent's started page is copied as far as it
+// is filled; the CTAs of plane 0 write the child's table row and length. 256 forks of a
+// page of 20 planes of 64 KiB: 43 us (359 MB; parents' pages are shared by 8 forks and read
+// from L2); 4 forks: 4.4 us, the chain of dependent loads parent -> length -> page id -> rows.
 __global__ void __launch_bounds__(MV_THREADS)
 pages_fork_kernel(PageMoveArgs m, PageForkArgs f)
 {
@@ -104,14 +114,16 @@ pages_fork_kernel(PageMoveArgs m, PageForkArgs f)
     }
     if (tail == 0) return;
     const size_t per = (size_t)m.page * 32;      // 16-byte words of one head's rows in a page
-    const uint4 *from = page_at(m, blockIdx.y, from_id);
-    uint4 *to = page_at(m, blockIdx.y, to_id);
-    for (int kh = 0; kh < m.KH; ++kh) copy_words(to + kh * per, from + kh * per, tail * 32);
+    for (int y = blockIdx.y; y < 2 * m.layers; y += gridDim.y) {
+        const uint4 *from = page_at(m, y, from_id);
+        uint4 *to = page_at(m, y, to_id);
+        for (int kh = 0; kh < m.KH; ++kh) copy_words(to + kh * per, from + kh * per, tail * 32);
+    }
 }
 
 cudaError_t launch_pages_fork(const PageMoveArgs &m, const PageForkArgs &f, cudaStream_t st)
 {
-    pages_fork_kernel<<<dim3(f.n, 2 * m.layers), MV_THREADS, 0, st>>>(m, f);
+    pages_fork_kernel<<<dim3(f.n, mv_rows(m, f.n)), MV_THREADS, 0, st>>>(m, f);
     return cudaGetLastError();
 }
 
@@ -160,7 +172,9 @@ __device__ __forceinline__ int pages_held(const PageMoveArgs &m, const PageCompa
 // One CTA, a bit per page in shared memory: mark what a request holds, count
 // the live pages, then pair the k-th live page behind the count (a mover)
 // with the k-th dead page before it (a hole). As many of the one as of the
-// other: dead pages before n_live = n_live - (live pages before it).
+// other: dead pages before n_live = n_live - (live pages before it). Latency alone: it and the
+// move of 2.6 GB (half of 4000 pages of 20 planes of 64 KiB) take 414 us, 6.3 TB/s; with the
+// 79 MB of half of 500 pages of 16 KiB 15.7 us in a graph, 12.1 of them the copy's.
 __global__ void __launch_bounds__(CP_THREADS, 1)
 pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
 {
@@ -201,7 +215,8 @@ pages_compact_plan_kernel(PageMoveArgs m, PageCompactArgs c)
 }
 
 // Moves the pages and writes the new table: every entry, those behind a
-// request's length as they are.
+// request's length as they are. A page goes in pieces of 32 KiB, so that a few movers
+// fill the GPU as many do.
 __global__ void __launch_bounds__(MV_THREADS)
 pages_compact_move_kernel(PageMoveArgs m, PageCompactArgs c, int piece)
 {

@@ -5,8 +5,10 @@ q and the softmax's numerators are rounded to parts of relative error u, an
 output differs from the exact one by at most
     (exp(2 d) - 1 + u) * sum_t p_t |v_t| * gate,   d = u * max_t sum_i |q_i k_ti| / 16
 (every score is off by at most d, the numerators by u more), plus the rounding
-of the output itself. u is 2^-8 for bf16 activations and 2^-16 for fp32 ones
-(two bf16 parts); the 32-bit sums add less than 2^-14 of the same terms.
+of the output itself. A bf16 part leaves 2^-8 of what it rounds, so u is 2^-8
+with one (prefill), 2^-16 with two (decode, bf16 activations) and 2^-24 with three
+(decode, fp32 activations), plus 2^-19 for the 32-bit norm, rotation, products and
+exponentials; the 32-bit sums add less than 2^-14 of the same terms.
 """
 import numpy as np
 

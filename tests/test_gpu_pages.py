@@ -78,10 +78,11 @@ def poison(P, table, lens):
     P.kv.copy_(t.where(held[None, None, :, None, :, None], P.kv, junk))
 
 
-def check_rows(P, before, qg, k, v, ctx, table, placed, group, dtype, rot=ROT, theta=THETA):
-    """placed: (row, request, position) of every row the call was to compute, in cache order."""
+def check_rows(P, before, qg, k, v, ctx, table, placed, group, dtype, rot=ROT, theta=THETA, parts=None):
+    """placed: (row, request, position) of every row the call was to compute, in cache order;
+    parts: bf16 parts of q and the probabilities (None: a decode call's)."""
     after = P.host()
-    u, u_out = (2.0 ** -8, 2.0 ** -8) if dtype else (2.0 ** -16, 2.0 ** -24)
+    u, u_out = 2.0 ** (-8 * (parts or (2 if dtype else 3))) + 2.0 ** -19, 2.0 ** -8 if dtype else 2.0 ** -24
     qg64, k64, v64 = (x.double().cpu().numpy() for x in (qg, k, v))
     got = ctx.double().cpu().numpy()
     row, req, pos = (np.array(x) for x in zip(*placed))
@@ -186,7 +187,7 @@ def test_prefill(be, chunks, page, KH, group, behind):
                         td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group, rot=ROT, eps=EPS, theta=THETA)
     be.sync()
     placed = [(int(cu[r]) + i, r, c + i) for r, (n, c) in enumerate(chunks) for i in range(n)]
-    check_rows(P, before, qg, k, v, ctx, table, placed, group, 1)
+    check_rows(P, before, qg, k, v, ctx, table, placed, group, 1, parts=1)
     assert (ctx[int(cu[-1]):] == 7).all(), "rows behind the last chunk were written"
 
 
@@ -219,7 +220,7 @@ def test_bad_ids_and_positions_are_reported_and_left_out(be):
 
 
 # ------------------------------------------------------------------ page moves
-@pytest.mark.parametrize("n,page,KH,layers", [(1, 16, 1, 1), (3, 48, 2, 3), (7, 1024, 1, 2), (60, 16, 2, 10)])
+@pytest.mark.parametrize("n,page,KH,layers", [(1, 16, 1, 1), (3, 48, 2, 3), (7, 1024, 1, 2), (60, 16, 2, 10), (1000, 16, 1, 3), (5000, 16, 1, 2)])
 def test_copy(be, n, page, KH, layers):
     P = Pool(be, 2 * n + 3, page, KH, layers, seed=n)
     ids = np.random.default_rng(n).permutation(2 * n + 3)
@@ -260,7 +261,8 @@ def fork_want(P, table, lens, parent, child, fresh):
     return kv, table, lens
 
 
-@pytest.mark.parametrize("page,KH,layers,lens", [(16, 2, 2, [0, 1, 15, 16, 17, 100]), (64, 1, 10, [63, 64, 65, 640]), (1024, 2, 1, [1023, 1])])
+@pytest.mark.parametrize("page,KH,layers,lens", [(16, 2, 2, [0, 1, 15, 16, 17, 100]), (64, 1, 10, [63, 64, 65, 640]), (1024, 2, 1, [1023, 1]),
+                                                 (16, 1, 3, [n % 40 for n in range(1200)])])
 def test_fork(be, page, KH, layers, lens):
     kids = 2 * len(lens)
     held = sum(-(-n // page) for n in lens)
@@ -563,7 +565,7 @@ def test_prefill_many_chunks(be):
                         td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group)
     be.sync()
     check_rows(P, before, qg, k, v, ctx, table, [(int(cu[r]) + i, r, c + i) for r, (n, c) in enumerate(chunks) for i in range(n)],
-               group, 1)
+               group, 1, parts=1)
 
 
 @pytest.mark.parametrize("rot,group", [(256, 1), (256, 8), (36, 2), (2, 4)])
@@ -580,7 +582,7 @@ def test_prefill_rotary_widths(be, rot, group):
                         table.shape[1], ctx.data_ptr(), H=KH * group, rot=rot, theta=5e5)
     be.sync()
     placed = [(i, 0, 10 + i) for i in range(150)] + [(150 + i, 1, 77 + i) for i in range(9)]
-    check_rows(P, before, qg, k, v, ctx, table, placed, group, 1, rot, 5e5)
+    check_rows(P, before, qg, k, v, ctx, table, placed, group, 1, rot, 5e5, parts=1)
 
 
 def test_gate_extremes(be):
@@ -639,7 +641,7 @@ def test_offsets_beyond_32_bits(be):
     cu, base = ints([0, 30, 40]), ints([150, 101])
     cache.prefill_dev(0, 2, 40, cu.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(), td.data_ptr(), 3, ctx.data_ptr())
     be.sync()
-    check_rows(P, before, qg, k, v, ctx, near, [(i, 0, 150 + i) for i in range(30)] + [(30 + i, 1, 101 + i) for i in range(10)], 8, 1)
+    check_rows(P, before, qg, k, v, ctx, near, [(i, 0, 150 + i) for i in range(30)] + [(30 + i, 1, 101 + i) for i in range(10)], 8, 1, parts=1)
     src, dst = ints([n_pages - 12]), ints([n_pages - 1])
     cache.copy_dev(1, src.data_ptr(), dst.data_ptr())
     table, ln = ints([[n_pages - 12, n_pages - 11], [0, 0]]), ints([100, 0])
