@@ -12,6 +12,7 @@
 #include <new>
 
 struct ColiCudaPages {
+    uintptr_t handle;         // what the caller holds in its place
     int layers, n_pages, page, KH;
     uint8_t *base;
     bool own_base;
@@ -29,7 +30,10 @@ namespace {
 
 constexpr int PAGES_MAX_LAYERS = MAX_LAYERS, PAGES_MAX_REQ = 1024, PAGES_MAX_PAGES = 1 << 20;
 constexpr int PAGES_MAX_HANDLES = 256;
-ColiCudaPages *g_pages[PAGES_MAX_HANDLES] = {};   // live handles; a call with another pointer is refused
+// Live pools. A caller's handle is no address but a count of pools made * 256 + slot, so that one
+// kept past its pool's end (coli_cuda_pages_free, a shutdown) never names a later pool.
+ColiCudaPages *g_pages[PAGES_MAX_HANDLES] = {};
+uintptr_t g_pages_made = 0;
 bool g_pages_ran = false;                         // an operator ran since the last look at g_pages_error
 
 size_t pages_page_bytes(int KH, int page) { return (size_t)KH * page * GQA_HD * 2; }
@@ -79,12 +83,16 @@ int pages_geometry(int layers, int n_pages, int page, int KH, int hd)
     return 1;
 }
 
-int pages_handle(const ColiCudaPages *p)
+ColiCudaPages *pages_find(const ColiCudaPages *handle)
+{
+    ColiCudaPages *p = g_pages[(uintptr_t)handle % PAGES_MAX_HANDLES];
+    return p && p->handle == (uintptr_t)handle ? p : nullptr;
+}
+int pages_usable(ColiCudaPages **p, const ColiCudaPages *handle)
 {
     READY();
-    bool known = false;
-    for (int i = 0; p && i < PAGES_MAX_HANDLES && !known; ++i) known = g_pages[i] == p;
-    if (!known) return fail("pages: not a live handle (coli_cuda_pages_create)");
+    *p = pages_find(handle);
+    if (!*p) return fail("pages: not a live handle (coli_cuda_pages_create)");
     int dev = -1;
     CK(cudaGetDevice(&dev));
     if (dev != G.device) return fail("pages: device %d is current, the backend runs on device %d", dev, G.device);
@@ -251,27 +259,27 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
              make_pages_tmap(m + 2, v, rows, p->box_rows, 1, 0) && make_pages_tmap(m + 3, v, rows, 8, 1, 0);
     }
     if (!ok) { pages_release(p); return 0; }
+    p->handle = ++g_pages_made * PAGES_MAX_HANDLES + slot;
     g_pages[slot] = p;
-    *pages = p;
+    *pages = (ColiCudaPages *)p->handle;
     return 1;
 }
 
-void coli_cuda_pages_free(ColiCudaPages *pages)
+void coli_cuda_pages_free(ColiCudaPages *handle)
 {
-    if (!pages) return;
-    for (int i = 0; i < PAGES_MAX_HANDLES; ++i) {
-        if (g_pages[i] != pages) continue;
-        if (g_pages_freed[i]) return;      // as many are waiting for a capture to end as there can be handles
-        g_pages[i] = nullptr;
-        g_pages_freed[i] = pages;
-        if (!pages_capturing()) pages_release_freed();
-        return;
-    }
+    ColiCudaPages *p = pages_find(handle);
+    if (!p) return;
+    const int slot = (int)(p->handle % PAGES_MAX_HANDLES);
+    if (g_pages_freed[slot]) return;       // as many are waiting for a capture to end as there can be handles
+    g_pages[slot] = nullptr;
+    g_pages_freed[slot] = p;
+    if (!pages_capturing()) pages_release_freed();
 }
 
-int coli_cuda_pages_device_ptr(const ColiCudaPages *pages, int layer, void **k, void **v)
+int coli_cuda_pages_device_ptr(const ColiCudaPages *handle, int layer, void **k, void **v)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (layer < 0 || layer >= pages->layers) return fail("pages: layer %d out of range", layer);
     const size_t plane = (size_t)pages->n_pages * pages_page_bytes(pages->KH, pages->page);
     if (k) *k = pages->base + 2 * layer * plane;
@@ -279,9 +287,10 @@ int coli_cuda_pages_device_ptr(const ColiCudaPages *pages, int layer, void **k, 
     return 1;
 }
 
-int coli_cuda_pages_norm_weight(ColiCudaPages *pages, int layer, const float *qnw, const float *knw, int hd)
+int coli_cuda_pages_norm_weight(ColiCudaPages *handle, int layer, const float *qnw, const float *knw, int hd)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (layer < 0 || layer >= pages->layers) return fail("pages: layer %d out of range", layer);
     if (hd != GQA_HD || !qnw || !knw) return fail("pages: bad norm weights (hd=%d)", hd);
     if (pages_capturing()) return fail("pages: norm weights cannot be set while the backend stream is capturing");
@@ -293,25 +302,28 @@ int coli_cuda_pages_norm_weight(ColiCudaPages *pages, int layer, const float *qn
     return 1;
 }
 
-size_t coli_cuda_pages_workspace_bytes(const ColiCudaPages *pages)
+size_t coli_cuda_pages_workspace_bytes(const ColiCudaPages *handle)
 {
-    return pages_handle(pages) ? pages_ws_bytes(pages->n_pages) : 0;
+    ColiCudaPages *pages;
+    return pages_usable(&pages, handle) ? pages_ws_bytes(pages->n_pages) : 0;
 }
 
-int coli_cuda_pages_set_workspace(ColiCudaPages *pages, void *ws, size_t bytes)
+int coli_cuda_pages_set_workspace(ColiCudaPages *handle, void *ws, size_t bytes)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (ws && (bytes < pages_ws_bytes(pages->n_pages) || ((uintptr_t)ws & 255)))
         return fail("pages: the workspace needs %zu bytes, 256-byte aligned", pages_ws_bytes(pages->n_pages));
     pages->ws = ws ? (uint8_t *)ws : pages->own_ws;
     return 1;
 }
 
-int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const void *qg, const void *k, const void *v,
+int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *handle, int layer, int B, const void *qg, const void *k, const void *v,
                                    const int *pos_dev, const int *table, int max_pages, void *ctx, int H, int KH, int hd,
                                    int rot, float eps, float theta, int dtype)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (dtype != 0 && dtype != 1) return fail("dtype must be 0 (fp32) or 1 (bf16)");
     if (B < 0 || B > PAGES_MAX_REQ) return fail("pages: batch %d out of 0..%d", B, PAGES_MAX_REQ);
     if (B == 0) return 1;
@@ -327,11 +339,12 @@ int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, const
     return 1;
 }
 
-int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, int S, const int *cu, const int *pos_base,
+int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *handle, int layer, int n_seq, int S, const int *cu, const int *pos_base,
                                     const void *qg, const void *k, const void *v, const int *table, int max_pages,
                                     void *ctx, int H, int KH, int hd, int rot, float eps, float theta, int dtype)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (dtype != 1) return fail("pages: prefill takes bf16 activations (dtype 1)");
     if (n_seq < 0 || n_seq > PAGES_MAX_REQ) return fail("pages: %d sequences out of 0..%d", n_seq, PAGES_MAX_REQ);
     if (S < 0 || S > 1 << 24) return fail("pages: %d rows out of 0..2^24", S);
@@ -352,9 +365,10 @@ int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, 
     return 1;
 }
 
-int coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const int *dst)
+int coli_cuda_pages_copy_dev(ColiCudaPages *handle, int n, const int *src, const int *dst)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (n < 0 || n > pages->n_pages) return fail("pages: %d pairs for %d pages", n, pages->n_pages);
     if (n == 0) return 1;
     if (!src || !dst) return fail("pages: a null pointer among the arguments");
@@ -365,10 +379,11 @@ int coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const 
     return 1;
 }
 
-int coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, const int *child, const int *fresh, int *len,
+int coli_cuda_pages_fork_dev(ColiCudaPages *handle, int n, const int *parent, const int *child, const int *fresh, int *len,
                              int *table, int n_req, int max_pages)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 1 << 30)
         return fail("pages: bad table %d x %d", n_req, max_pages);
     if (n < 0 || n >= n_req) return fail("pages: %d forks among %d requests", n, n_req);
@@ -385,10 +400,11 @@ int coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, con
     return 1;
 }
 
-int coli_cuda_pages_compact_dev(ColiCudaPages *pages, int n_req, const int *len, const int *table, int max_pages,
+int coli_cuda_pages_compact_dev(ColiCudaPages *handle, int n_req, const int *len, const int *table, int max_pages,
                                 int *table_out, int *live)
 {
-    if (!pages_handle(pages)) return 0;
+    ColiCudaPages *pages;
+    if (!pages_usable(&pages, handle)) return 0;
     if (n_req < 1 || max_pages < 1 || (long long)max_pages * pages->page > 1 << 30)
         return fail("pages: bad table %d x %d", n_req, max_pages);
     if (!len || !table || !table_out || !live) return fail("pages: a null pointer among the arguments");

@@ -800,3 +800,24 @@ def test_a_pool_of_its_own_and_handles_that_end(be):
         m.free()
     be.sync()
     assert be.mem_info() == before
+
+
+def test_a_handle_ends_with_its_pool(be):
+    """A handle kept past its pool's end names no later pool, in calls or in a second free."""
+    pkg = load_pkg()
+    P = Pool(be, 4, 16, 1)
+    x, y = ints([0]), ints([1])
+    old = [P.cache.h]
+    P.cache.free()
+    for _ in range(5):
+        c = pkg.PagedCache(be, 1, 4, 16, 1, kv=P.kv.data_ptr())
+        assert c.h not in old
+        for h in old:
+            be.lib.coli_cuda_pages_free(h)
+            assert be.lib.coli_cuda_pages_copy_dev(h, 1, x.data_ptr(), y.data_ptr()) == 0
+            assert b"live handle" in be.lib.coli_cuda_last_error()
+        c.copy_dev(1, x.data_ptr(), y.data_ptr())
+        be.sync()
+        assert P.torch.equal(P.kv[:, :, 0].view(P.torch.int16), P.kv[:, :, 1].view(P.torch.int16))
+        old.append(c.h)
+        c.free()
