@@ -240,14 +240,16 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
 //
 // Measured with the join (H / KH = 8, KH = 2 unless said): 64 requests at 32k tokens,
 // 4.25 GB, 651 us, 6.53 TB/s (the device's copies: 6.56); 48 ragged requests of up to 8k
-// tokens, fp32, KH = 4, 305 MB, 57 us replayed from a graph (82 us called one by one behind a
-// flush of L2), 47 us at the copy rate; one request of 4k tokens, 15 us from a graph: the join's
+// tokens, fp32, KH = 4, 305 MB, 74 us from a graph, 47 at the copy rate; one request of 4k tokens, 15 us from a graph: the join's
 // launch, 4 us, and one pass through cold instructions.
 constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_STAGES = 3, PD_STAGE = 2 * GQA_TILE_BYTES;
-// Entries that a unit counts more than it has when the list is cut: its q and
-// gate take a warp about as long as PD_EXTRA + 2 tiles. With 0, 1, 2, 3, 4: 69, 62, 57, 59,
-// 55 us for the 48 ragged requests, 21.8, 22.5, 20.9, 22.3, 24.5 for 64 of 512 tokens.
-constexpr int PD_EXTRA = 2;
+// Entries that a unit counts more than it has when the list is cut. A warp pays for the q of
+// every piece; one that starts and ends in its range it also finishes and writes by itself. So a
+// unit longer than a range counts PD_EXTRA more (0, 1, 2, 3, 4: 64 requests of 512 tokens 21.8, 22.5,
+// 20.9, 22.3, 24.5 us) and one that fits into a range PD_WHOLE (48 requests of 1 to 8191 tokens,
+// spread over the logarithm: 40 us with 8 or 12, 45 with 4, 52 with PD_EXTRA for all; fp32 43, 51,
+// 61). Where a range has less than PD_WHOLE entries it rarely holds a whole unit, and all count alike.
+constexpr int PD_EXTRA = 2, PD_WHOLE = 8;
 constexpr int PD_OROW = 132;                 // floats between heads of O: 8 banks apart for the writers' heads
 template <typename TI> struct PdEntry {      // layout of the q entry and of the gate entry in a stage
     static constexpr bool F32 = sizeof(TI) == 4;
@@ -305,6 +307,7 @@ struct PdSmem {
     float2 ml[PD_WARPS][2][GQA_GRP];        // (max, sum) of a warp's continued / opened piece
     int4 cont[PD_WARPS], open[PD_WARPS];    // (there: 1, and ends here: 2; request; KV head; parked / last CTA)
     int pre[1024 + 4];                      // entries (of one KV head) before each request
+    uint32_t cut[32];                       // a bit per request: its units are longer than a range
     int part[PD_WARPS];
     uint64_t full[PD_WARPS][PD_STAGES];
 };
@@ -355,10 +358,13 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
     griddep_launch();                       // the join may be scheduled; it waits for this grid
     // entries before each request: its tiles, a q and a gate entry. Up to 32
     // requests every warp counts for itself (all write the same), with no barrier.
-    auto entries = [&](int r) {
+    auto tiles = [&](int r) {               // 0: idle
         int row0, pos0;
-        return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 3 + PD_EXTRA : 0;
+        return pages_rows_of(p, r, row0, pos0) ? pos0 / GQA_TILE + 1 : 0;
     };
+    const int workers = gridDim.x * PD_WARPS;
+    int whole = 0;                          // tiles of a unit that a range can hold
+    auto entries = [&](int nt) { return nt == 0 ? 0 : nt + 2 + (nt <= whole ? PD_WHOLE : PD_EXTRA); };
     // the norm weights and rotary frequencies: loads in flight until the first
     // tiles are, then every warp writes the same
     float4 w_in[4];
@@ -367,13 +373,37 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
     {
         const int each = (p.n_req + PD_THREADS - 1) / PD_THREADS, small = p.n_req <= 32;
         const int r0 = min(p.n_req, small ? lane : tid * each), r1 = min(p.n_req, small ? lane + 1 : r0 + each);
-        int mine = 0;
+        int nt = 0, sum = 0;                // (the last of r0 .. r1 - 1, the only one where small)
 #pragma unroll 1
-        for (int r = r0; r < r1; ++r) mine += entries(r);
+        for (int r = r0; r < r1; ++r) { nt = tiles(r); sum += entries(nt); }
         if (lane == 0) {
             for (int s = 0; s < PD_STAGES; ++s) mbar_init(&sm.full[warp][s], 1);
             fence_mbar_init();
             sm.cont[warp] = sm.open[warp] = make_int4(0, 0, 0, 0);
+        }
+        if (p.n_req > 1) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (!small) {
+                if (lane == 0) sm.part[warp] = sum;
+                if (tid < 32) sm.cut[tid] = 0;
+                __syncthreads();
+                sum = 0;
+                for (int w = 0; w < PD_WARPS; ++w) sum += sm.part[w];
+                __syncthreads();            // read before it is written again
+            }
+            whole = (sum * KH + workers - 1) / workers;
+            if (whole < PD_WHOLE) whole = 0;
+        }
+        int mine = entries(nt);
+        if (!small) {
+            mine = 0;
+#pragma unroll 1
+            for (int r = r0; r < r1; ++r) {
+                nt = tiles(r);
+                mine += entries(nt);
+                if (nt > whole) atomicOr(&sm.cut[r >> 5], 1u << (r & 31));
+            }
         }
         int inc = mine;
 #pragma unroll
@@ -383,20 +413,22 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
         }
         int at = inc - mine;
         if (small) {
+            const unsigned cut = __ballot_sync(0xffffffffu, nt > whole);
             if (lane < p.n_req) sm.pre[lane] = at;
-            if (lane == 31) sm.pre[p.n_req] = inc;
+            if (lane == 31) { sm.pre[p.n_req] = inc; sm.cut[0] = cut; }
             __syncwarp();
         } else {
             if (lane == 31) sm.part[warp] = inc;
             __syncthreads();
             for (int w = 0; w < warp; ++w) at += sm.part[w];
 #pragma unroll 1
-            for (int r = r0; r < r1; ++r) { sm.pre[r] = at; at += entries(r); }
+            for (int r = r0; r < r1; ++r) { sm.pre[r] = at; at += entries(tiles(r)); }
             if (tid == PD_THREADS - 1) sm.pre[p.n_req] = at;
             __syncthreads();
         }
     }
-    const int total = sm.pre[p.n_req] * KH, workers = gridDim.x * PD_WARPS;
+    auto extra = [&](int r) { return sm.cut[r >> 5] >> (r & 31) & 1 ? PD_EXTRA : PD_WHOLE; };
+    const int total = sm.pre[p.n_req] * KH;
     const int per = max(1, (total + workers - 1) / workers);
     const int v0 = min(total, (cta * PD_WARPS + warp) * per), v1 = min(total, v0 + per);
     // request of entry v: the last r with pre[r] * KH <= v
@@ -423,7 +455,7 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
         int kh = (int)__fdividef((float)rel0, (float)n);        // at most KH <= 64: off by one at most
         kh -= kh * n > rel0;
         kh += (kh + 1) * n <= rel0;
-        const int rel = rel0 - kh * n - PD_EXTRA, nt = n - 2 - PD_EXTRA;       // 0: q, 1 ..: tiles, nt + 1: gate
+        const int ex = extra(r), rel = rel0 - kh * n - ex, nt = n - 2 - ex;    // 0: q, 1 ..: tiles, nt + 1: gate
         const bool begins = at - rel + 1 >= v0;                 // the unit's first tile is in the range
         if (v < v0) ahead = rel >= 1 && rel <= nt ? 1 : -1;
         else if (v == v1) ahead = rel == nt && begins ? 2 : -1;
@@ -502,11 +534,12 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                     if (next_v >= v1) break;
                     r = next_r; kh = next_kh;
                     const int n = sm.pre[r + 1] - sm.pre[r];
-                    nt = n - 2 - PD_EXTRA;
-                    u0 = sm.pre[r] * KH + kh * n;
-                    tile = max(next_v - u0 - 1 - PD_EXTRA, 0);
-                    end_tile = min(v1 - u0 - 1 - PD_EXTRA, nt);
-                    next_v = min(v1, u0 + n);
+                    const int ex = extra(r);
+                    nt = n - 2 - ex;
+                    u0 = sm.pre[r] * KH + kh * n + ex;      // its q entry
+                    tile = max(next_v - u0 - 1, 0);
+                    end_tile = min(v1 - u0 - 1, nt);
+                    next_v = min(v1, u0 + nt + 2);
                     if (++next_kh == KH) {
                         next_kh = 0;
                         for (++next_r; next_r < p.n_req && sm.pre[next_r + 1] == sm.pre[next_r];) ++next_r;
@@ -694,7 +727,7 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                         const int kind = begins ? 1 : 0;
                         const bool last = next_v >= v1;
                         if (lane == 0) {
-                            if (begins) sm.open[warp] = make_int4(1, r, kh, (u0 + PD_EXTRA + nt) / per / PD_WARPS);
+                            if (begins) sm.open[warp] = make_int4(1, r, kh, (u0 + nt) / per / PD_WARPS);
                             else sm.cont[warp] = make_int4(ends ? 3 : 1, r, kh, last ? 0 : 1);
                         }
                         if (lane < 4) { sm.ml[warp][kind][h0] = make_float2(m0, l0); sm.ml[warp][kind][h0 + 1] = make_float2(m1, l1); }

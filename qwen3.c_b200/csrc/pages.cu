@@ -329,7 +329,7 @@ int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *handle, int layer, int B, cons
     if (B == 0) return 1;
     GqaPagesArgs a{};
     if (!pages_attend_args(a, pages, layer, qg, k, v, pos_dev, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
-    if (((long long)max_pages * (pages->page / GQA_TILE) + PD_EXTRA + 3) * B * pages->KH > 1 << 30)
+    if (((long long)max_pages * (pages->page / GQA_TILE) + PD_WHOLE + 3) * B * pages->KH > 1 << 30)
         return fail("pages: a table of %d x %d pages passes 2^30 tiles", B, max_pages);
     a.n_req = a.S = B;
     g_pages_ran = true;
