@@ -512,6 +512,26 @@ def test_compact_twice_is_the_identity(be):
     assert lv.item() == live == live2 and not moves and np.array_equal(again, want)
 
 
+# lengths over the whole range, enough of them that some units fit into a warp's range and some are cut
+@pytest.mark.parametrize("B,KH,group,dtype", [(30, 4, 2, 1), (60, 2, 8, 0)])
+def test_decode_short_beside_long(be, B, KH, group, dtype):
+    rng = np.random.default_rng(B)
+    lens = [0, 6000, 6000] + [int(n) for n in np.exp(rng.uniform(0, np.log(6000), size=B - 3))]
+    page = 32
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    P = Pool(be, n_pages, page, KH, seed=B)
+    table = pages_for(lens, page, n_pages, seed=B)
+    poison(P, table, lens)
+    before = P.host()
+    qg, k, v, ctx = P.inputs(B, KH * group, dtype)
+    pos, td = ints([n - 1 for n in lens]), ints(table)
+    P.cache.decode_dev(0, B, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), table.shape[1],
+                       ctx.data_ptr(), H=KH * group, rot=ROT, eps=EPS, theta=THETA, dtype=dtype)
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, table, [(r, r, n - 1) for r, n in enumerate(lens) if n], group, dtype)
+    assert (ctx[0] == 7).all()
+
+
 # the most requests of a call, some idle, and more of them than a warp counts alone
 @pytest.mark.parametrize("B,KH,group,dtype", [(1024, 1, 2, 1), (33, 2, 8, 0), (200, 3, 4, 1)])
 def test_decode_many_requests(be, B, KH, group, dtype):
