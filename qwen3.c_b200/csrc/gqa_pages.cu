@@ -240,8 +240,8 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
 //
 // Measured with the join (H / KH = 8, KH = 2 unless said): 64 requests at 32k tokens,
 // 4.25 GB, 651 us, 6.53 TB/s (the device's copies: 6.56); 48 ragged requests of up to 8k
-// tokens, fp32, KH = 4, 305 MB, 74 us from a graph, 47 at the copy rate; one request of 4k tokens, 15 us from a graph: the join's
-// launch, 4 us, and one pass through cold instructions.
+// tokens, fp32, KH = 4, 305 MB, 74 us from a graph, 47 at the copy rate; one request of 4k
+// tokens, 15 us from a graph: the join's launch, 4 us, and one pass through cold instructions.
 constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_STAGES = 3, PD_STAGE = 2 * GQA_TILE_BYTES;
 // Entries that a unit counts more than it has when the list is cut. A warp pays for the q of
 // every piece; one that starts and ends in its range it also finishes and writes by itself. So a
@@ -980,10 +980,11 @@ cudaError_t launch_pages_decode(const CUtensorMap &tkv, const GqaPagesArgs &a, c
 // its MMAs, and the tensor pipe is the bound here.
 // Measured, H / KH = 8, KH = 2: 4096 rows after 28672, 2.06 TFLOP of causal products, 1.55 ms
 // (1.33 PFLOP/s, 0.82 of the GPU's 8192^3 product; up to 1.79 ms under its power cap); nine
-// chunks of up to 1023 rows after up to 4096, 155 GFLOP, 185 us from a graph (0.84 PFLOP/s; masked
-// halves of diagonal tiles, units cut at CTAs' ends and their join are the rest); three short
-// prompts 20 us, latency of three launches. In a tile's 2700 cycles shared memory is read for
-// about 2500 (K and V by the MMAs, P written and read): next to the tensor pipe the second bound.
+// chunks of up to 1023 rows after up to 4096, 155 GFLOP, 183 us from a graph (0.84 PFLOP/s; the
+// rest are units' starts and ends, 15500 cycles each where a tile takes 2750, masked halves of
+// diagonal tiles and the join of units cut at CTAs' ends); three short prompts 19 us, latency of
+// three launches. In a tile's cycles shared memory is read for about 2500 (K and V by the MMAs, P
+// written and read): next to the tensor pipe the second bound.
 constexpr int PP_BM = 128, PP_BN = 128;
 constexpr int PP_TILE = PP_BN * GQA_HD * 2, PP_P = PP_BM * PP_BN * 2;
 constexpr int PP_SOFTMAX = 256, PP_THREADS = 96 + PP_SOFTMAX;
