@@ -1210,7 +1210,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const int box = p.box_rows, boxes = PP_BN / box, beyond = (int)((long long)p.pv.n_pages * KH * p.pv.page >> 3);
         bool ok = true;
         bool appended = false;              // .. the rows that the kernel before appends are visible
-        int gate_in[2] = {-1, -1}, wholes = 0, pc = 0;
+        int gate_in = -1, wholes = 0, pc = 0;   // the stage of the last gate tile, until its epilogue is known to be done
         for (; ok && w.piece(tokens); w.next(p, tokens), ++pc) {
             const int end = w.base + w.n;   // the request's rows
             if (warp == 1) ok = mbar_wait(&bars.q_tmem, pc & 1);   // Q has left the V buffer
@@ -1231,7 +1231,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 }
                 if (warp == 0) {
                     if (jj >= 2) ok = mbar_wait(&bars.k_empty[s], ((jj >> 1) - 1) & 1);
-                    if (ok && gate_in[s] >= 0) { ok = mbar_wait(&bars.epi_done, gate_in[s] & 1); gate_in[s] = -1; }
+                    if (ok && gate_in == s) { ok = mbar_wait(&bars.epi_done, (wholes - 1) & 1); gate_in = -1; }
                 } else if (jj >= 1) {
                     ok = mbar_wait(&bars.v_empty, (jj - 1) & 1);
                 }
@@ -1245,16 +1245,22 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 __syncwarp();
             }
             if (warp == 0 && ok && w.ends && w.at.w == 0) {
-                // the gate tile, into the stage of the last K tile once S has read it
+                // the gate tile, into the stage of the last K tile once S has read it, and once the
+                // gate before is used up: g_full is one barrier for all of them, and where this unit is a
+                // single tile no K load has waited for that. The epilogue before needs nothing that
+                // this warp does from here on. One gate is unfinished at a time, so the parities are plain.
                 const int s = (jj - 1) & 1;
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars.k_empty[s], ((jj - 1) >> 1) & 1));
+                ok = mbar_wait(&bars.k_empty[s], ((jj - 1) >> 1) & 1);
+                if (ok && gate_in >= 0) ok = mbar_wait(&bars.epi_done, (wholes - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
                 if (ok && lane == 0) {
                     mbar_expect_tx(&bars.g_full, PP_TILE);
                     for (int c = 0; c < 4; ++c)
                         tma_load_3d(sK + s * PP_TILE + c * (PP_BM * 128), &tmG, GQA_HD + 64 * c, w.at.y * group,
                                     w.row0 + w.at.z * tokens, &bars.g_full);
                 }
-                gate_in[s] = wholes++;
+                gate_in = s;
+                ++wholes;
             }
         }
     } else if (warp == 2) {

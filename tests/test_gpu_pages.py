@@ -841,3 +841,35 @@ def test_a_handle_ends_with_its_pool(be):
         assert P.torch.equal(P.kv[:, :, 0].view(P.torch.int16), P.kv[:, :, 1].view(P.torch.int16))
         old.append(c.h)
         c.free()
+
+
+def test_prefill_many_whole_units_of_one_tile(be):
+    """Prompts that end inside their first 128 positions, so many that every CTA works through whole units of one key
+    tile each, one behind the other; repeated calls give the same bits."""
+    rng = np.random.default_rng(11)
+    chunks = [(int(n), int(c)) for n, c in zip(rng.integers(17, 41, size=256), rng.integers(0, 80, size=256))]
+    page, KH, group = 64, 2, 8
+    total = [n + c for n, c in chunks]
+    n_pages = sum(-(-n // page) for n in total) + 1
+    P = Pool(be, n_pages, page, KH, seed=12)
+    table = pages_for(total, page, n_pages, seed=12)
+    poison(P, table, total)
+    before = P.host()
+    cu = np.concatenate([[0], np.cumsum([n for n, _ in chunks])])
+    S = int(cu[-1])
+    qg, k, v, ctx = P.inputs(S, KH * group, 1)
+    cu_d, base, td = ints(cu), ints([c for _, c in chunks]), ints(table)
+
+    def call():
+        P.cache.prefill_dev(0, len(chunks), S, cu_d.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(),
+                            td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group)
+        be.sync()
+
+    call()
+    check_rows(P, before, qg, k, v, ctx, table, [(int(cu[r]) + i, r, c + i) for r, (n, c) in enumerate(chunks) for i in range(n)],
+               group, 1, parts=1)
+    first, rows = ctx.clone(), P.kv.clone()
+    for _ in range(20):
+        ctx.fill_(7.0)
+        call()
+        assert P.torch.equal(ctx, first) and P.torch.equal(P.kv.view(P.torch.int16), rows.view(P.torch.int16))
