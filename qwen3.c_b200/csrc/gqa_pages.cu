@@ -62,10 +62,18 @@ __device__ __forceinline__ void gate4(float *o, const float *g)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= g[i] == g[i] ? s[i] : g[i];
 }
-__device__ __forceinline__ float rms_factor(float s2, float eps)     // 1 / sqrt(s2 / hd + eps), one Newton step
+// 1 / sqrt(s2 / hd + eps), one Newton step; 0 where s2 is infinite (its row has an infinity)
+__device__ __forceinline__ float rms_factor(float s2, float eps)
 {
     const float a = fmaf(s2, 1.f / GQA_HD, eps), r = rsqrtf(a);
-    return r * fmaf(-0.5f * a * r, r, 1.5f);
+    return r * fmaf(-0.5f * fminf(a, 3.402823466e38f) * r, r, 1.5f);
+}
+// Squares are summed in fp32. Where that leaves the type's range (elements of 1e18 and
+// more, or, without an eps, below 2^-48), the row's sum is formed once more of up * x, and the
+// factor is up / sqrt(sum / hd + up^2 eps): rows of any normal numbers have one.
+__device__ __forceinline__ float rms_rescale(float s2, float eps)    // 1: none needed
+{
+    return !(s2 <= 3.402823466e38f) ? 0x1p-72f : fmaf(s2, 1.f / GQA_HD, eps) < 0x1p-96f ? 0x1p72f : 1.f;
 }
 
 // First row of K/V of request r, KV head kh, position pos; -1 for a page id
@@ -110,7 +118,15 @@ __device__ __forceinline__ void pages_norm_rope(float (&x)[8], const float (&w1)
     for (int i = 0; i < 8; ++i) s2 = fmaf(x[i], x[i], s2);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-    const float rs = rms_factor(s2, eps);
+    const float up = rms_rescale(s2, eps);
+    if (__builtin_expect(up != 1.f, 0)) {   // (the same in all lanes)
+        s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s2 = fmaf(x[i] * up, x[i] * up, s2);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+    }
+    const float rs = up * rms_factor(s2, eps * up * up);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] *= rs * w1[i];
     const int half = rot >> 1, d0 = lane * 8;
@@ -161,7 +177,18 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
     s0 += s1;
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-    const float rs = rms_factor(s0, eps);
+    const float up = rms_rescale(s0, eps);
+    if (__builtin_expect(__any_sync(0xffffffffu, up != 1.f), 0)) {
+        s0 = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < GQA_HD / LANES; ++k) {
+            const float x = row.load1(LANES * k + q) * up;
+            s0 = fmaf(x, x, s0);
+        }
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+    }
+    const float rs = up * rms_factor(s0, eps * up * up);
     __syncwarp();
     const int half = rot >> 1;
     if ((half & 7) == 0) {
@@ -177,7 +204,7 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
             load8<float>(sn + 8 * c, si);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float x = a[i] * wa[i] * rs, y = b[i] * wb[i] * rs;
+                const float x = a[i] * rs * wa[i], y = b[i] * rs * wb[i];   // the factor first: a * wa can overflow
                 a[i] = x * co[i] - y * si[i];
                 b[i] = y * co[i] + x * si[i];
             }
@@ -190,18 +217,18 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
             row.load(c, a);
             load8<float>(w1 + 8 * c, wa);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] *= wa[i] * rs;
+            for (int i = 0; i < 8; ++i) a[i] = a[i] * rs * wa[i];
             row.store(c, a);
         }
     } else {
 #pragma unroll 1
         for (int j = q; j < half; j += LANES) {
-            const float x = row.load1(j) * w1[j] * rs, y = row.load1(j + half) * w1[j + half] * rs;
+            const float x = row.load1(j) * rs * w1[j], y = row.load1(j + half) * rs * w1[j + half];
             row.store1(j, x * cs[j] - y * sn[j]);
             row.store1(j + half, y * cs[j] + x * sn[j]);
         }
 #pragma unroll 1
-        for (int d = rot + q; d < GQA_HD; d += LANES) row.store1(d, row.load1(d) * w1[d] * rs);
+        for (int d = rot + q; d < GQA_HD; d += LANES) row.store1(d, row.load1(d) * rs * w1[d]);
     }
     __syncwarp();
 }
@@ -575,7 +602,7 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                         for (int e = 0; e < 8; ++e) s2 += (double)x[e] * x[e];
 #pragma unroll
                         for (int o = 16; o > 0; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
-                        const double a = s2 * (1.0 / GQA_HD) + p.eps, r0 = rsqrtf((float)a), r = r0 * (1.5 - 0.5 * a * r0 * r0);
+                        const double r = rsqrt(s2 * (1.0 / GQA_HD) + p.eps);
                         const int half = p.rot >> 1;
 #pragma unroll 1
                         for (int j = lane; j < half; j += 32) {

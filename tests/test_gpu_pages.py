@@ -873,3 +873,58 @@ def test_prefill_many_whole_units_of_one_tile(be):
         ctx.fill_(7.0)
         call()
         assert P.torch.equal(ctx, first) and P.torch.equal(P.kv.view(P.torch.int16), rows.view(P.torch.int16))
+
+
+# rows from where the squares leave fp32 (2^128) downwards; without eps also rows whose squares vanish
+@pytest.mark.parametrize("scales,eps", [([1e18, 3e19, 1.1e38, 1.0, 1e-30], 1e-6), ([1e-18, 1e-25, 1e-35, 1e30, 1.0], 0.0)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_decode_rows_of_any_finite_scale(be, monkeypatch, scales, eps, dtype):
+    monkeypatch.setitem(globals(), "EPS", eps)      # what check_rows norms with
+    lens, page, KH, group = [40, 17, 700, 33, 64], 16, 2, 4
+    n_pages = sum(-(-n // page) for n in lens)
+    P = Pool(be, n_pages, page, KH, seed=21)
+    table = pages_for(lens, page, n_pages, seed=21)
+    before = P.host()
+    qg, k, v, ctx = P.inputs(5, KH * group, dtype)
+    by = P.torch.tensor(scales, device="cuda")[:, None, None]
+    qg[..., :HD] = (qg[..., :HD].float().clamp(-3, 3) * by).to(qg.dtype)
+    k = (k.float().clamp(-3, 3) * by).to(k.dtype)
+    pos, td = ints([n - 1 for n in lens]), ints(table)
+    P.cache.decode_dev(0, 5, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), table.shape[1],
+                       ctx.data_ptr(), H=KH * group, eps=eps, dtype=dtype)
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, table, [(r, r, n - 1) for r, n in enumerate(lens)], group, dtype)
+
+
+@pytest.mark.parametrize("scale,eps,rot", [(2e19, 1e-6, 64), (1.1e38, 1e-6, 64), (1.1e38, 1e-6, 36), (1e-25, 0.0, 64), (1e-25, 0.0, 36)])
+def test_prefill_rows_of_any_finite_scale(be, monkeypatch, scale, eps, rot):
+    """Rows of 1 and of `scale` in turn, whose norms a warp takes together."""
+    monkeypatch.setitem(globals(), "EPS", eps)
+    page, KH, group = 32, 2, 8
+    P = Pool(be, 4, page, KH, seed=22)
+    table = pages_for([70], page, 4, seed=22)
+    before = P.host()
+    qg, k, v, ctx = P.inputs(50, KH * group, 1)
+    by = P.torch.tensor([1.0, scale] * 25, device="cuda")[:, None, None]
+    qg[..., :HD] = (qg[..., :HD].float().clamp(-3, 3) * by).bfloat16()
+    k = (k.float().clamp(-3, 3) * by).bfloat16()
+    cu, base, td = ints([0, 50]), ints([20]), ints(table)
+    P.cache.prefill_dev(0, 1, 50, cu.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(), td.data_ptr(),
+                        table.shape[1], ctx.data_ptr(), H=KH * group, rot=rot, eps=eps)
+    be.sync()
+    check_rows(P, before, qg, k, v, ctx, table, [(i, 0, 20 + i) for i in range(50)], group, 1, rot=rot, parts=1)
+
+
+def test_rows_with_an_infinity(be):
+    """x / rms(x) of a row with an infinity: 0 for its finite elements, NaN for the infinite ones, so NaN as an output."""
+    P = Pool(be, 8, 16, 1, seed=23)
+    for dtype in (0, 1):
+        qg, k, v, ctx = P.inputs(2, 8, dtype)
+        qg[0, 3, 100] = float("inf")
+        pos, td = ints([20, 20]), ints([[0, 1], [2, 3]])
+        P.cache.decode_dev(0, 2, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), 2, ctx.data_ptr(),
+                           H=8, dtype=dtype)
+        be.sync()
+        bad = P.torch.zeros(2, 8, dtype=P.torch.bool, device="cuda")
+        bad[0, 3] = True
+        assert ctx[bad].isnan().all() and ctx[~bad].isfinite().all()
