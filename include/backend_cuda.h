@@ -442,9 +442,10 @@ int  coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const
 /* Request child[i] becomes a copy of request parent[i], i < n < n_req: it
  * shares the pages that the parent has filled, len[child] = len[parent], and
  * where the parent's last page is only started, its rows are copied to page
- * fresh[i], which no request holds (else fresh[i] is not used). A parent may have many children; a
- * child named twice or also as a parent, and a fresh page named twice, are
- * left out and reported. len int32 [n_req], table int32 [n_req][max_pages]. */
+ * fresh[i], which no request holds (else fresh[i] is not used, and may be
+ * anything). A parent may have many children; a child named twice or also as
+ * a parent, and a fresh page that is used twice or that another fork copies
+ * from, are left out and reported. len int32 [n_req], table int32 [n_req][max_pages]. */
 int  coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, const int *child, const int *fresh,
                               int *len, int *table, int n_req, int max_pages);
 /* Renumber the pages that the requests hold (the first ceil(len / page) of

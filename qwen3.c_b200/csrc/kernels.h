@@ -238,6 +238,7 @@ struct PageForkArgs {
     const int *parent, *child, *fresh;
     int *len, *table;
     int n, n_req, max_pages;
+    FastDiv page_div;     // by the tokens of a page
 };
 cudaError_t launch_pages_fork(const PageMoveArgs &m, const PageForkArgs &f, cudaStream_t st);
 struct PageCompactArgs {

@@ -72,7 +72,9 @@ cudaError_t launch_pages_copy(const PageMoveArgs &m, int n, const int *src, cons
 // CTAs as in a copy, per fork: the parent's started page is copied as far as it
 // is filled; the CTAs of plane 0 write the child's table row and length. 256 forks of a
 // page of 20 planes of 64 KiB: 43 us (359 MB; parents' pages are shared by 8 forks and read
-// from L2); 4 forks: 4.4 us, the chain of dependent loads parent -> length -> page id -> rows.
+// from L2); 4 forks: 4.5 us, the chain of dependent loads parent -> length -> page id -> rows.
+// Every CTA looks through all forks for conflicts, as a copy's do: 1000 forks of short tails
+// (4 layers, pages of 16 rows) take 42 us, 32 without the look at the other forks' started pages.
 __global__ void __launch_bounds__(MV_THREADS)
 pages_fork_kernel(PageMoveArgs m, PageForkArgs f)
 {
@@ -93,12 +95,19 @@ pages_fork_kernel(PageMoveArgs m, PageForkArgs f)
         pages_error(PAGES_BAD_ID);
         return;
     }
-    // A child named twice, one that is also a parent, or a fresh page named
-    // twice: left out.
-    int bad = a == c || (tail && to_id == from_id);
+    // A child named twice, one that is also a parent, or a fresh page that another fork
+    // uses too, as its own fresh one or as the started page that it copies: left out. The fresh
+    // page of a parent that ends with a page is not used, whatever it says. (A parent's length and
+    // row are written by no fork: its child would be a parent.)
+    int bad = a == c;
     for (int j = threadIdx.x; j < f.n; j += MV_THREADS) {
-        if (f.parent[j] == c || (j != i && (f.child[j] == c || f.child[j] == a))) bad = 1;
-        if (tail && j != i && f.fresh[j] == to_id) bad = 1;
+        const int pj = f.parent[j], cj = f.child[j];
+        if (pj == c || (j != i && (cj == c || cj == a))) bad = 1;
+        if (tail && (unsigned)pj < (unsigned)f.n_req) {
+            const int lj = max(f.len[pj], 0), fj = f.page_div(lj);
+            if (fj < f.max_pages && lj - fj * m.page > 0 &&
+                ((j != i && f.fresh[j] == to_id) || f.table[(size_t)pj * f.max_pages + fj] == to_id)) bad = 1;
+        }
     }
     if (__syncthreads_or(bad)) {
         pages_error(PAGES_CONFLICT);

@@ -393,7 +393,7 @@ int coli_cuda_pages_fork_dev(ColiCudaPages *handle, int n, const int *parent, co
         return fail("pages: index arrays must be 4-byte aligned");
     PageForkArgs f{};
     f.parent = parent; f.child = child; f.fresh = fresh; f.len = len; f.table = table;
-    f.n = n; f.n_req = n_req; f.max_pages = max_pages;
+    f.n = n; f.n_req = n_req; f.max_pages = max_pages; f.page_div = FastDiv::of(pages->page);
     g_pages_ran = true;
     CK(launch_pages_fork(pages_move_args(pages), f, stream()));
     g_launches += 1;

@@ -928,3 +928,44 @@ def test_rows_with_an_infinity(be):
         bad = P.torch.zeros(2, 8, dtype=P.torch.bool, device="cuda")
         bad[0, 3] = True
         assert ctx[bad].isnan().all() and ctx[~bad].isfinite().all()
+
+
+def test_fork_ignores_fresh_pages_that_are_not_used(be):
+    """Parents that end with a page need no fresh one: what stands in its place may repeat another's or be no page at all."""
+    P = Pool(be, 14, 16, 2, 2, seed=31)
+    lens = [32, 20, 16, 0, 0, 0, 0, 0, 0, 0]
+    table = np.array([[0, 1], [2, 3], [4, -1]] + [[-1, -1]] * 7, np.int32)
+    parent, child, fresh = [0, 1, 2, 0, 1, 2], [3, 4, 5, 6, 7, 8], [9, 9, 9, -1, 10, 3]
+    want_kv, want_table, want_lens = fork_want(P, table, lens, parent, child, fresh)
+    p, c, f, td, ld = ints(parent), ints(child), ints(fresh), ints(table), ints(lens)
+    P.cache.fork_dev(6, p.data_ptr(), c.data_ptr(), f.data_ptr(), ld.data_ptr(), td.data_ptr(), 10, 2)
+    be.sync()
+    np.testing.assert_array_equal(td.cpu().numpy(), want_table)
+    assert ld.tolist() == want_lens
+    assert P.torch.equal(P.kv.view(P.torch.int16), want_kv.view(P.torch.int16))
+
+
+@pytest.mark.parametrize("extra", [0, 400])
+def test_fork_leaves_out_a_fresh_page_that_another_fork_copies(be, extra):
+    """Page 3 is request 1's started page: a fork that would write to it is left out, the one that reads it is not."""
+    BackendError = load_pkg().BackendError
+    n = 4 + 2 * (3 + extra)
+    P = Pool(be, 8 + extra, 16, 1, 2, seed=32)
+    lens = [5, 20, 9] + [0] * (n - 3)
+    table = np.full((n, 2), -1, np.int32)
+    table[0, 0], table[1], table[2, 0] = 0, [2, 3], 4
+    parent, child, fresh = [0, 1, 2], [3, 4, 5], [3, 5, 6]
+    for i in range(extra):                     # many more, so that the two stand far apart
+        parent.insert(1, 2)
+        child.insert(1, 6 + i)
+        fresh.insert(1, 8 + i)
+    keep = [i for i in range(len(parent)) if i != 0]
+    want_kv, want_table, want_lens = fork_want(P, table, lens, *([x[i] for i in keep] for x in (parent, child, fresh)))
+    p, c, f, td, ld = ints(parent), ints(child), ints(fresh), ints(table), ints(lens)
+    P.cache.fork_dev(len(parent), p.data_ptr(), c.data_ptr(), f.data_ptr(), ld.data_ptr(), td.data_ptr(), n, 2)
+    with pytest.raises(BackendError, match="named twice"):
+        be.sync()
+    be.sync()
+    np.testing.assert_array_equal(td.cpu().numpy(), want_table)
+    assert ld.tolist() == want_lens
+    assert P.torch.equal(P.kv.view(P.torch.int16), want_kv.view(P.torch.int16))
