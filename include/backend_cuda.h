@@ -437,7 +437,8 @@ int  coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq,
 
 /* Page src[i] over page dst[i] in every layer, i < n. A pair whose destination
  * is named twice, or whose source is another pair's destination, is left out
- * and reported. */
+ * and reported; a page onto itself is a destination, but no bar to pairs that
+ * read it. */
 int  coli_cuda_pages_copy_dev(ColiCudaPages *pages, int n, const int *src, const int *dst);
 /* Request child[i] becomes a copy of request parent[i], i < n < n_req: it
  * shares the pages that the parent has filled, len[child] = len[parent], and

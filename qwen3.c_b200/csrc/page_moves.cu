@@ -38,7 +38,8 @@ __device__ __forceinline__ void copy_words(uint4 *to, const uint4 *from, int wor
 // 319 us, 6.57 TB/s, either way, 327-336 with a quarter and a 16th of the CTAs). 8 pages of
 // 20 planes of 16 KiB: 2.6 us in a graph, the latency of a launch and two dependent loads. A
 // pair is left out when its destination is named by another pair too, or when its source is
-// another pair's destination: either would make the result a matter of timing.
+// another pair's destination: either would make the result a matter of timing. A page onto
+// itself is written by nobody, so other pairs may read it.
 __global__ void __launch_bounds__(MV_THREADS)
 pages_copy_kernel(PageMoveArgs m, int n, const int *src, const int *dst)
 {
@@ -49,7 +50,7 @@ pages_copy_kernel(PageMoveArgs m, int n, const int *src, const int *dst)
     }
     int bad = 0;
     for (int j = threadIdx.x; j < n; j += MV_THREADS)
-        if (j != i && (dst[j] == d || dst[j] == s)) bad = 1;
+        if (j != i && (dst[j] == d || (dst[j] == s && src[j] != s))) bad = 1;
     if (__syncthreads_or(bad)) {
         pages_error(PAGES_CONFLICT);
         return;

@@ -969,3 +969,23 @@ def test_fork_leaves_out_a_fresh_page_that_another_fork_copies(be, extra):
     np.testing.assert_array_equal(td.cpu().numpy(), want_table)
     assert ld.tolist() == want_lens
     assert P.torch.equal(P.kv.view(P.torch.int16), want_kv.view(P.torch.int16))
+
+
+def test_copy_of_a_page_onto_itself_stands_beside_its_copies(be):
+    """A page onto itself writes nothing, so pairs that read it are copied; one that writes to it is still left out."""
+    BackendError = load_pkg().BackendError
+    P = Pool(be, 12, 16, 2, 2, seed=33)
+    want = P.kv.clone()
+    src, dst = [3, 3, 3, 5], [3, 4, 6, 5]
+    want[:, :, [4, 6]] = P.kv[:, :, [3, 3]]
+    s, d = ints(src), ints(dst)
+    P.cache.copy_dev(4, s.data_ptr(), d.data_ptr())
+    be.sync()
+    assert P.torch.equal(P.kv.view(P.torch.int16), want.view(P.torch.int16))
+    s, d = ints([7, 8, 9]), ints([7, 7, 10])     # 8 over the page that another pair names
+    want[:, :, 10] = P.kv[:, :, 9]
+    P.cache.copy_dev(3, s.data_ptr(), d.data_ptr())
+    with pytest.raises(BackendError, match="named twice"):
+        be.sync()
+    be.sync()
+    assert P.torch.equal(P.kv.view(P.torch.int16), want.view(P.torch.int16))
