@@ -878,6 +878,11 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
     if (tid == 0) part.units[cta] = make_int4(n > 0 && opened ? unit.w : -1, unit.y, unit.z, 0);
 }
 
+// A piece (max, sum) that weighs nothing: all its keys are masked, or their scores -infinity. Scores
+// that are all NaN leave the maximum at -infinity as well (fmaxf passes NaN over), but not the sum at
+// 0: such a piece's NaN is the result's.
+__device__ __forceinline__ bool piece_empty(const float2 &ml) { return ml.x == -INFINITY && ml.y == 0.f; }
+
 // One CTA of four warps per (CTA of the kernel before, query head): merges the
 // pieces of the unit that begins there and goes on. Warp w takes pieces w, w + 4,
 // .. with a running maximum, lane = 8 dims; then thread d merges the four results
@@ -918,7 +923,7 @@ pages_join_kernel(GqaPagesArgs p, PagesPart part)
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (ml[u].x == -INFINITY) continue;
+            if (piece_empty(ml[u])) continue;
             const float mn = fmaxf(m, ml[u].x);
             const float fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fs = ex2_approx(ml[u].x - mn);
             const float v[8] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x, y[u].y, y[u].z, y[u].w};
@@ -1621,7 +1626,7 @@ pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             x[c] = reinterpret_cast<const float4 *>(part.o)[slot * (PP_BM * GQA_HD / 4) + (block * (PJ_DIMS / 4) + 8 * c + j) * PP_BM + row];
-        if (ml.x == -INFINITY) continue;
+        if (piece_empty(ml)) continue;
         const float mn = fmaxf(m, ml.x), fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fs = ex2_approx(ml.x - mn);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -1672,7 +1677,7 @@ pages_prefill_join_deep_kernel(GqaPagesArgs p, PagesPart part)
 #pragma unroll
         for (int c = 0; c < 8; ++c)
             x[c] = reinterpret_cast<const float4 *>(part.o)[slot * (PP_BM * GQA_HD / 4) + (block * (PJ_DEEP / 4) + c) * PP_BM + row];
-        if (ml.x == -INFINITY) continue;
+        if (piece_empty(ml)) continue;
         const float mn = fmaxf(m, ml.x), fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fs = ex2_approx(ml.x - mn);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {

@@ -989,3 +989,44 @@ def test_copy_of_a_page_onto_itself_stands_beside_its_copies(be):
         be.sync()
     be.sync()
     assert P.torch.equal(P.kv.view(P.torch.int16), want.view(P.torch.int16))
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_decode_keeps_nan_keys_of_a_cut_request(be, dtype):
+    """K rows of NaN inside a request's length make its ctx NaN however its tiles are cut: a run of them at every offset
+    from where the cuts are, so that in some of the calls it fills whole pieces and no other."""
+    page, KH, group, n = 16, 1, 8, 5000
+    n_pages = -(-n // page)
+    P = Pool(be, n_pages, page, KH, seed=41)
+    table = pages_for([n], page, n_pages, seed=41)
+    kv = P.kv.clone()
+    qg, k, v, ctx = P.inputs(1, KH * group, dtype)
+    pos, td = ints([n - 1]), ints(table)
+    for first in range(100, 108):
+        P.kv.copy_(kv)
+        P.kv[0, 0, ints(table[0, first:first + 40]).long()] = float("nan")
+        ctx.zero_()
+        P.cache.decode_dev(0, 1, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), table.shape[1],
+                           ctx.data_ptr(), H=KH * group, dtype=dtype)
+        be.sync()
+        assert ctx.isnan().all(), f"tiles {first} .. {first + 39} were left out"
+
+
+# few units (many pieces each, the deep join) and many (a few pieces)
+@pytest.mark.parametrize("rows,before,runs", [(2, 9000, [(8 + o, 24 + o) for o in range(8)]), (700, 3000, [(0, n) for n in range(1, 23)])])
+def test_prefill_keeps_nan_keys_of_a_cut_unit(be, rows, before, runs):
+    page, KH, group = 128, 2, 8
+    n_pages = -(-(rows + before) // page)
+    P = Pool(be, n_pages, page, KH, seed=42)
+    table = pages_for([rows + before], page, n_pages, seed=42)
+    kv = P.kv.clone()
+    qg, k, v, ctx = P.inputs(rows, KH * group, 1)
+    cu, base, td = ints([0, rows]), ints([before]), ints(table)
+    for first, last in runs:                             # key tiles, here a page each, of NaN in KV head 0
+        P.kv.copy_(kv)
+        P.kv[0, 0, ints(table[0, first:last]).long(), 0] = float("nan")
+        ctx.zero_()
+        P.cache.prefill_dev(0, 1, rows, cu.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(),
+                            td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group)
+        be.sync()
+        assert ctx[:, :group].isnan().all() and ctx[:, group:].isfinite().all(), f"tiles {first} .. {last - 1}"
