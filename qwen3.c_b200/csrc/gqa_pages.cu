@@ -1129,9 +1129,12 @@ pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
     float x[8], v[8], w1[8];
     load8<__nv_bfloat16>(k + lane * 8, x);
     load8<__nv_bfloat16>(static_cast<const __nv_bfloat16 *>(p.v) + (size_t)item * GQA_HD + lane * 8, v);
-    int lo = -1, row0, b;                   // the last request that starts at or before the row
-    for (int r = lane; r - lane < p.n_req; r += 32) lo += __popc(__ballot_sync(0xffffffffu, r < p.n_req && p.cu[r] <= row));
-    if (lo < 0 || row < p.cu[lo] || row >= p.cu[lo + 1] || pages_rows_of(p, lo, row0, b) == 0) return;
+    int lo = -1, row0, b;                   // the request whose chunk holds the row, whatever the other offsets say
+    for (int r = lane; lo < 0 && r - lane < p.n_req; r += 32) {
+        const unsigned in = __ballot_sync(0xffffffffu, r < p.n_req && p.cu[r] <= row && row < p.cu[r + 1]);
+        if (in) lo = r - lane + __ffs(in) - 1;
+    }
+    if (lo < 0 || pages_rows_of(p, lo, row0, b) == 0) return;
     const int pos = b + row - row0;
     const long long at = pages_row(p.pv, lo, kh, pos);
     pages_rope_table(cs[warp], sn[warp], pos, p.rot, f.turn, lane, 32);

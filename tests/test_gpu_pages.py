@@ -1030,3 +1030,21 @@ def test_prefill_keeps_nan_keys_of_a_cut_unit(be, rows, before, runs):
                             td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group)
         be.sync()
         assert ctx[:, :group].isnan().all() and ctx[:, group:].isfinite().all(), f"tiles {first} .. {last - 1}"
+
+
+def test_offsets_that_descend_leave_the_good_chunks(be):
+    """Rows named by offsets that descend or pass the rows given belong to no chunk; the chunks before are computed."""
+    BackendError = load_pkg().BackendError
+    P = Pool(be, 8, 16, 2, seed=53)
+    table = np.array([[0, 1], [2, 3], [4, 5], [6, 7]], np.int32)
+    for cu in ([0, 3, 3, 9, 9], [0, 3, 2, 2, 2], [0, 3, 3, -5, -5]):
+        before = P.host()
+        qg, k, v, ctx = P.inputs(4, 16, 1)
+        cu_d, base, td = ints(cu), ints([2, 0, 2, 0]), ints(table)
+        P.cache.prefill_dev(0, 4, 4, cu_d.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(),
+                            td.data_ptr(), 2, ctx.data_ptr())
+        with pytest.raises(BackendError, match="offsets"):
+            be.sync()
+        be.sync()
+        check_rows(P, before, qg, k, v, ctx, table, [(i, 0, 2 + i) for i in range(3)], 8, 1, parts=1)
+        assert (ctx[3] == 7).all()
