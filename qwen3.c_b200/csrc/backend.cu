@@ -589,6 +589,7 @@ int coli_cuda_init(int device)
     G.encode = (EncodeTiledFn)fn;
     int zero = 0;
     CK(cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(int)));
+    CK(cudaMemcpyToSymbol(g_pages_error, &zero, sizeof(int)));
     G.device = device;
     G.ready = 1;
     snprintf(G.err, sizeof(G.err), "ok");

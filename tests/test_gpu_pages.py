@@ -1048,3 +1048,24 @@ def test_offsets_that_descend_leave_the_good_chunks(be):
         be.sync()
         check_rows(P, before, qg, k, v, ctx, table, [(i, 0, 2 + i) for i in range(3)], 8, 1, parts=1)
         assert (ctx[3] == 7).all()
+
+
+def test_an_argument_error_ends_with_its_session(be):
+    """A bad page id met before a shutdown is not reported to what runs after the next init."""
+    import torch
+    pkg = load_pkg()
+    P = Pool(be, 4, 16, 1)
+    bad, x, y = ints([99]), ints([0]), ints([1])
+    P.cache.copy_dev(1, bad.data_ptr(), x.data_ptr())
+    be.shutdown()
+    assert be.lib.coli_cuda_init(0) == 1
+    be.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    be.sync()
+    c = pkg.PagedCache(be, 1, 4, 16, 1, kv=P.kv.data_ptr())
+    c.copy_dev(1, x.data_ptr(), y.data_ptr())
+    be.sync()
+    assert torch.equal(P.kv[:, :, 0].view(torch.int16), P.kv[:, :, 1].view(torch.int16))
+    c.copy_dev(1, bad.data_ptr(), x.data_ptr())
+    with pytest.raises(pkg.BackendError, match="page id outside"):
+        be.sync()
+    be.sync()
