@@ -198,9 +198,9 @@ void *scratch(Slot s, size_t bytes)
     return G.slot[s];
 }
 
-// Page caches (pages.cu): the state of their device-side argument checks, and
+// Page caches (pages.cu): the report of their device-side argument checks, and
 // their release at shutdown.
-int pages_check_error();
+int pages_error_ok(int h);
 void pages_shutdown();
 
 int check_layer(int layer) { return layer >= 0 && layer < MAX_LAYERS; }
@@ -266,11 +266,20 @@ int download(void *host, const void *dev, size_t bytes)
 {
     cudaStream_t st = stream();
     CK(cudaMemcpyAsync(host, dev, bytes, cudaMemcpyDeviceToHost, st));
-    CK(cudaMemcpyFromSymbolAsync(g_err_pin ? g_err_pin : &g_err_host, g_dev_error, sizeof(int), 0,
+    CK(cudaMemcpyFromSymbolAsync(g_err_pin ? g_err_pin : &g_err_host, g_dev_errors, sizeof(int), 0,
                                  cudaMemcpyDeviceToHost, st));
     CK(cudaStreamSynchronize(st));
     if (g_err_pin) g_err_host = *g_err_pin;
     g_err_fresh = true;
+    return 1;
+}
+
+int dev_error_ok(int h)
+{
+    if (h) {
+        G.ready = 0;
+        return fail("device error word %d (%s)", h, h == 1 ? "pipeline wait timed out" : "kernel fault");
+    }
     return 1;
 }
 
@@ -282,14 +291,10 @@ int check_dev_error()
         g_err_fresh = false;
     } else {
         cudaStream_t st = stream();
-        CK(cudaMemcpyFromSymbolAsync(&h, g_dev_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+        CK(cudaMemcpyFromSymbolAsync(&h, g_dev_errors, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
         CK(cudaStreamSynchronize(st));
     }
-    if (h) {
-        G.ready = 0;
-        return fail("device error word %d (%s)", h, h == 1 ? "pipeline wait timed out" : "kernel fault");
-    }
-    return 1;
+    return dev_error_ok(h);
 }
 
 __global__ void iota_kernel(int *pos, int *creq, int n, int base, int req)
@@ -587,9 +592,8 @@ int coli_cuda_init(int device)
     CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
     if (!fn || q != cudaDriverEntryPointSuccess) return fail("cuTensorMapEncodeTiled entry point not found");
     G.encode = (EncodeTiledFn)fn;
-    int zero = 0;
-    CK(cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(int)));
-    CK(cudaMemcpyToSymbol(g_pages_error, &zero, sizeof(int)));
+    const DevErrors none{};
+    CK(cudaMemcpyToSymbol(g_dev_errors, &none, sizeof(none)));
     G.device = device;
     G.ready = 1;
     snprintf(G.err, sizeof(G.err), "ok");
@@ -717,8 +721,10 @@ int coli_cuda_sync(void)
 {
     READY();
     CK(cudaStreamSynchronize(stream()));
-    if (!check_dev_error()) return 0;
-    return pages_check_error();
+    DevErrors e{};
+    CK(cudaMemcpyFromSymbolAsync(&e, g_dev_errors, sizeof(e), 0, cudaMemcpyDeviceToHost, stream()));
+    CK(cudaStreamSynchronize(stream()));
+    return dev_error_ok(e.pipeline) && pages_error_ok(e.pages);
 }
 
 void *coli_cuda_get_stream(void) { return (void *)stream(); }

@@ -17,12 +17,17 @@
 
 namespace coli {
 
-// Device-side error word (first error wins). Codes:
+// Device-side error words (first error wins in each), side by side so that the host
+// reads both at once. Codes of the pipeline word, which ends the session:
 //   1 = mbarrier wait timed out, 2 = bad launch geometry, 3 = TMEM alloc failure.
+// The other one is an argument that a paged call met (gqa_pages.cu).
 // Defined once: the library is built as one translation unit (backend.cu).
-__device__ int g_dev_error;
+struct DevErrors {
+    int pipeline, pages;
+};
+__device__ DevErrors g_dev_errors;
 
-__device__ __forceinline__ void raise_error(int code) { atomicCAS(&g_dev_error, 0, code); }
+__device__ __forceinline__ void raise_error(int code) { atomicCAS(&g_dev_errors.pipeline, 0, code); }
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -83,7 +88,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255) == 0) {
             if (globaltimer_ns() - t0 > lim) break;
-            if (*(volatile int *)&g_dev_error) return false;  // another CTA gave up: bail out
+            if (*(volatile int *)&g_dev_errors.pipeline) return false;  // another CTA gave up: bail out
         }
     }
     raise_error(1);

@@ -8,18 +8,18 @@
 // head kh is row (table[r][pos / page] * KH + kh) * page + pos % page.
 //
 // Every page id and position is checked on the device before it is used; a
-// bad one raises g_pages_error, is left out, and touches no memory.
+// bad one raises g_dev_errors.pages, is left out, and touches no memory.
 #include "common.cuh"
 #include "kernels.h"
 #include "tc05.cuh"
 
 namespace coli {
 
-// Argument errors found on the device (first one wins, read and cleared by
-// the host): the backend stays usable.
+// Argument errors found on the device (first one wins, read by every
+// coli_cuda_sync, so that replayed graphs report theirs, and cleared there): the
+// backend stays usable.
 enum { PAGES_OK = 0, PAGES_BAD_ID = 1, PAGES_BAD_POS = 2, PAGES_BAD_ROWS = 3, PAGES_CONFLICT = 4, PAGES_BAD_REQ = 5 };
-__device__ int g_pages_error;
-__device__ __forceinline__ void pages_error(int code) { atomicCAS(&g_pages_error, 0, code); }
+__device__ __forceinline__ void pages_error(int code) { atomicCAS(&g_dev_errors.pages, 0, code); }
 
 // Angle table of position pos, entries [0, rot / 2): the angle in turns is the
 // fraction of an exact 64-bit product, so far positions lose nothing.

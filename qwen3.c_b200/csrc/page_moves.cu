@@ -3,7 +3,7 @@
 // kernels are plain copies, bound by HBM (each moved byte read and written).
 //
 // Page ids, request indices and lengths are checked on the device; what is
-// out of range or in conflict raises g_pages_error and is left out.
+// out of range or in conflict raises g_dev_errors.pages and is left out.
 #include "common.cuh"
 #include "kernels.h"
 

@@ -34,7 +34,6 @@ constexpr int PAGES_MAX_HANDLES = 256;
 // kept past its pool's end (coli_cuda_pages_free, a shutdown) never names a later pool.
 ColiCudaPages *g_pages[PAGES_MAX_HANDLES] = {};
 uintptr_t g_pages_made = 0;
-bool g_pages_ran = false;                         // an operator ran since the last look at g_pages_error
 
 size_t pages_page_bytes(int KH, int page) { return (size_t)KH * page * GQA_HD * 2; }
 size_t pages_norm_bytes(int layers) { return (size_t)layers * 2 * GQA_HD * 4; }
@@ -134,18 +133,14 @@ void pages_shutdown()
         if (g_pages[i]) pages_release(g_pages[i]);
         g_pages[i] = nullptr;
     }
-    g_pages_ran = false;
 }
 
-int pages_check_error()
+// The word as coli_cuda_sync read it: 1, or cleared and reported.
+int pages_error_ok(int h)
 {
-    if (!g_pages_ran) return 1;
-    int h = 0;
-    CK(cudaMemcpyFromSymbolAsync(&h, g_pages_error, sizeof(int), 0, cudaMemcpyDeviceToHost, stream()));
-    CK(cudaStreamSynchronize(stream()));
     if (h == PAGES_OK) return 1;
     const int zero = 0;
-    CK(cudaMemcpyToSymbolAsync(g_pages_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream()));
+    CK(cudaMemcpyToSymbolAsync(g_dev_errors, &zero, sizeof(int), offsetof(DevErrors, pages), cudaMemcpyHostToDevice, stream()));
     CK(cudaStreamSynchronize(stream()));
     static const char *const what[] = {"", "a page id outside the pool", "a position or length beyond the page table",
                                        "row offsets that do not ascend within the rows given",
@@ -332,7 +327,6 @@ int coli_cuda_gqa_decode_pages_dev(ColiCudaPages *handle, int layer, int B, cons
     if (((long long)max_pages * (pages->page / GQA_TILE) + PD_WHOLE + 3) * B * pages->KH > 1 << 30)
         return fail("pages: a table of %d x %d pages passes 2^30 tiles", B, max_pages);
     a.n_req = a.S = B;
-    g_pages_ran = true;
     CK(launch_pages_decode(pages->maps[4 * layer], a, pages_part(pages->ws), pages->freq, dtype,
                            G.num_sms, stream()));
     g_launches += 2;
@@ -355,7 +349,6 @@ int coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *handle, int layer, int n_seq,
     if (!pages_attend_args(a, pages, layer, qg, k, v, pos_base, table, max_pages, ctx, H, KH, hd, rot, eps, theta)) return 0;
     a.cu = cu;
     a.n_req = n_seq; a.S = S;
-    g_pages_ran = true;
     const CUtensorMap *m = pages->maps + 4 * layer;
     CUtensorMap gate;
     if (!make_pages_gate_tmap(&gate, qg, S, H, H / KH)) return 0;
@@ -373,7 +366,6 @@ int coli_cuda_pages_copy_dev(ColiCudaPages *handle, int n, const int *src, const
     if (n == 0) return 1;
     if (!src || !dst) return fail("pages: a null pointer among the arguments");
     if (((uintptr_t)src | (uintptr_t)dst) & 3) return fail("pages: index arrays must be 4-byte aligned");
-    g_pages_ran = true;
     CK(launch_pages_copy(pages_move_args(pages), n, src, dst, stream()));
     g_launches += 1;
     return 1;
@@ -394,7 +386,6 @@ int coli_cuda_pages_fork_dev(ColiCudaPages *handle, int n, const int *parent, co
     PageForkArgs f{};
     f.parent = parent; f.child = child; f.fresh = fresh; f.len = len; f.table = table;
     f.n = n; f.n_req = n_req; f.max_pages = max_pages; f.page_div = FastDiv::of(pages->page);
-    g_pages_ran = true;
     CK(launch_pages_fork(pages_move_args(pages), f, stream()));
     g_launches += 1;
     return 1;
@@ -416,7 +407,6 @@ int coli_cuda_pages_compact_dev(ColiCudaPages *handle, int n_req, const int *len
     c.src = (int *)pages->ws; c.dst = (int *)(pages->ws + list); c.remap = (int *)(pages->ws + 2 * list);
     c.count = (int *)(pages->ws + 3 * list);
     c.n_req = n_req; c.max_pages = max_pages;
-    g_pages_ran = true;
     CK(launch_pages_compact(pages_move_args(pages), c, stream()));
     g_launches += 2;
     return 1;
