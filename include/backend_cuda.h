@@ -387,8 +387,10 @@ int  coli_cuda_gdn_full_route(int layer, const float *x_in, const float *resid, 
  *   pages_create         kv_dev: the caller's memory (128-byte aligned, its
  *                        contents kept) or NULL for a zeroed pool of the
  *                        handle's own; up to 256 handles at a time
- *   pages_free           waits for the backend stream, then releases
- *                        (a handle whose pool has ended is refused from then on)
+ *   pages_free           waits for the backend stream, then releases (while that
+ *                        stream captures, the next create or free does); a
+ *                        handle whose pool has ended is refused from then on.
+ *                        Captures on other streams are left alone
  *   pages_norm_weight    q_norm / k_norm weights [hd] of a layer (host fp32)
  *   pages_set_workspace  pages_workspace_bytes bytes of device memory, 256-byte
  *                        aligned, for the calls from here on; NULL: the

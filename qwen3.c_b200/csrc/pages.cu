@@ -108,16 +108,29 @@ void pages_release(ColiCudaPages *p)
     delete p;
 }
 
-// Handles freed while the backend stream was capturing: freeing memory there
-// would end the capture, so it waits for the next call that may.
+// Handles freed while the backend stream was capturing: waiting for it there
+// would end the capture, so that is left to the next call that may.
 ColiCudaPages *g_pages_freed[PAGES_MAX_HANDLES] = {};
 bool pages_capturing()
 {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    return cudaStreamIsCapturing(stream(), &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream(), &st) != cudaSuccess) {
+        cudaGetLastError();                // the legacy stream, which cannot be used while a blocking stream captures
+        return true;
+    }
+    return st != cudaStreamCaptureStatusNone;
 }
+// A pool may be freed at any time (the Python object's is by garbage collection), so also while a
+// stream other than the backend's captures in the global mode, in which this thread's cudaFree would
+// end that capture: the memory is none of the capture's business, and the relaxed mode says so.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
 void pages_release_freed()
 {
+    RelaxedCapture relaxed;
     for (int i = 0; i < PAGES_MAX_HANDLES; ++i) {
         if (!g_pages_freed[i]) continue;
         cudaStreamSynchronize(stream());   // queued calls may still use the pool and the workspace

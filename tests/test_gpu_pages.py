@@ -1069,3 +1069,44 @@ def test_an_argument_error_ends_with_its_session(be):
     with pytest.raises(pkg.BackendError, match="page id outside"):
         be.sync()
     be.sync()
+
+
+def test_a_handle_freed_while_another_stream_captures(be):
+    """Freeing a pool (as garbage collection may at any time) leaves a capture on a stream that is not the backend's
+    alone, with the backend on a stream of its own as on the legacy stream, which a blocking stream's capture makes
+    unusable until it ends."""
+    import gc
+
+    import torch
+    pkg = load_pkg()
+    gc.collect()
+    before = be.mem_info()
+    x = torch.zeros(64, device="cuda")
+    side, own_stream = torch.cuda.Stream(), torch.cuda.Stream()
+    caches = [pkg.PagedCache(be, 1, 4, 16, 1) for _ in range(2)]
+    torch.cuda.synchronize()
+    be.set_stream(own_stream.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):     # the global mode
+        x += 1
+        caches.pop().free()
+    g.replay()
+    torch.cuda.synchronize()
+    assert (x == 1).all()
+    from cuda.bindings import runtime as cudart
+    err, blocking = cudart.cudaStreamCreate()
+    assert err == cudart.cudaError_t.cudaSuccess
+    be.set_stream(1)
+    err, = cudart.cudaStreamBeginCapture(blocking, cudart.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal)
+    assert err == cudart.cudaError_t.cudaSuccess
+    caches.pop().free()
+    with pytest.raises(pkg.BackendError, match="capturing"):
+        pkg.PagedCache(be, 1, 4, 16, 1)
+    err, graph = cudart.cudaStreamEndCapture(blocking)
+    assert err == cudart.cudaError_t.cudaSuccess, "the capture was ended from outside"
+    cudart.cudaGraphDestroy(graph)
+    cudart.cudaStreamDestroy(blocking)
+    be.set_stream(torch.cuda.current_stream().cuda_stream or 1)
+    pkg.PagedCache(be, 1, 4, 16, 1).free()
+    be.sync()
+    assert be.mem_info() == before
