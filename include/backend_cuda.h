@@ -455,7 +455,9 @@ int  coli_cuda_pages_fork_dev(ColiCudaPages *pages, int n, const int *parent, co
  * each table row; len <= 0: none) to 0 .. *live - 1: the k-th held page at or
  * behind *live moves to the k-th free page before it, in every layer. Pages
  * *live .. are free afterwards. table_out gets the new table (entries behind
- * a request's length as they were) and may be table itself. */
+ * a request's length as they were) and may be table itself. What a request
+ * with a length beyond the table names is not held, and an id outside the pool
+ * stays as it is; both are reported, the rest is served. */
 int  coli_cuda_pages_compact_dev(ColiCudaPages *pages, int n_req, const int *len, const int *table, int max_pages,
                                  int *table_out, int *live);
 

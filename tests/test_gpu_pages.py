@@ -1110,3 +1110,66 @@ def test_a_handle_freed_while_another_stream_captures(be):
     pkg.PagedCache(be, 1, 4, 16, 1).free()
     be.sync()
     assert be.mem_info() == before
+
+
+def test_moves_report_bad_lengths_and_ids_and_leave_them_out(be):
+    """Fork of a parent whose length passes its table; compaction of such a length and of ids outside the pool: the good
+    requests are served, and every other row of the pool, the table and the lengths is left alone."""
+    BackendError = load_pkg().BackendError
+    P = Pool(be, 12, 16, 1, 2, seed=51)
+    lens = [20, 33, -4, 5, 0, 0, 0, 0, 0]      # of 2 pages: ok, beyond, negative, its started page is no page
+    table = np.array([[0, 1], [2, 3], [4, 5], [12, -1]] + [[-1, -1]] * 5, np.int32)
+    parent, child, fresh = [0, 1, 2, 3, 0], [4, 5, 6, 7, 8], [8, 9, 10, 11, -1]
+    want_kv, want_table, want_lens = fork_want(P, table, lens, [0], [4], [8])
+    p, c, f, td, ld = ints(parent), ints(child), ints(fresh), ints(table), ints(lens)
+    P.cache.fork_dev(5, p.data_ptr(), c.data_ptr(), f.data_ptr(), ld.data_ptr(), td.data_ptr(), 9, 2)
+    with pytest.raises(BackendError, match="beyond the page table|page id outside"):
+        be.sync()
+    be.sync()
+    np.testing.assert_array_equal(td.cpu().numpy(), want_table)
+    assert ld.tolist() == want_lens
+    assert P.torch.equal(P.kv.view(P.torch.int16), want_kv.view(P.torch.int16))
+
+    lens = [33, 20, 32, 16]                    # beyond (holds nothing), ok, one id below and one behind the pool, ok
+    table = np.array([[0, 1], [11, 9], [-1, 12], [7, 12]], np.int32)
+    good = np.array([[0, 1], [11, 9], [-1, 12], [7, 12]], np.int32)
+    want_table, live, moves = ref.compact(good, [0, 20, 0, 16], 16, 12)
+    assert live == 3
+    want_kv = P.kv.clone()
+    s, d = (list(x) for x in zip(*moves))
+    want_kv[:, :, d] = P.kv[:, :, s]
+    ld, td, lv = ints(lens), ints(table), ints([-1])
+    P.cache.compact_dev(4, ld.data_ptr(), td.data_ptr(), 2, td.data_ptr(), lv.data_ptr())
+    with pytest.raises(BackendError, match="beyond the page table|page id outside"):
+        be.sync()
+    be.sync()
+    assert lv.item() == live
+    np.testing.assert_array_equal(td.cpu().numpy(), want_table)
+    assert P.torch.equal(P.kv.view(P.torch.int16), want_kv.view(P.torch.int16))
+
+
+@pytest.mark.parametrize("bad", [-1, 14, 1 << 30, -(1 << 31)])
+def test_prefill_leaves_out_bad_ids_and_positions(be, bad):
+    """A chunk with an id outside the pool, one that passes its table and one with a negative start beside two good
+    ones: those are computed, the bad ones append only where their own rows have a page, nothing else changes."""
+    BackendError = load_pkg().BackendError
+    page, KH, group = 16, 2, 8
+    P = Pool(be, 14, page, KH, seed=52)
+    chunks = [(20, 12), (17, 15), (9, 24), (5, -1), (3, 7)]     # the third: 33 rows in 2 pages
+    table = np.array([[0, 1], [2, bad], [4, 5], [6, 7], [8, bad]], np.int32)
+    cu = np.concatenate([[0], np.cumsum([n for n, _ in chunks])])
+    before = P.host()
+    qg, k, v, ctx = P.inputs(int(cu[-1]), KH * group, 1)
+    cu_d, base, td = ints(cu), ints([c for _, c in chunks]), ints(table)
+    P.cache.prefill_dev(0, 5, int(cu[-1]), cu_d.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(),
+                        td.data_ptr(), 2, ctx.data_ptr(), H=KH * group)
+    with pytest.raises(BackendError, match="page id outside|beyond the page table"):
+        be.sync()
+    be.sync()
+    # request 1's row at position 15 is in its good page; those from 16 on have none
+    one = P.host()[:, 2, :, 15]
+    before[:, 2, :, 15] = one
+    np.testing.assert_array_equal(one[1], ref.bf16(v[20].double().cpu().numpy()))
+    placed = [(i, 0, 12 + i) for i in range(20)] + [(int(cu[4]) + i, 4, 7 + i) for i in range(3)]
+    check_rows(P, before, qg, k, v, ctx, table, placed, group, 1, parts=1)
+    assert (ctx[int(cu[2]):int(cu[4])] == 7).all(), "a chunk that was left out was written"
