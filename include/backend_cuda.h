@@ -412,7 +412,9 @@ int    coli_cuda_pages_set_workspace(ColiCudaPages *pages, void *ws, size_t byte
  * the page of position pos[b] that request's alone (fork before). q and the
  * probabilities enter the tensor cores as two bf16 parts each with bf16
  * activations (dtype 1) and as three with fp32 ones (dtype 0), so ctx is good
- * to about 2^-17 and 2^-21 before its own rounding; the cache is bf16. RoPE
+ * to about 2^-16 and 2^-21 before its own rounding; the cache is bf16. The parts
+ * of a number have its sign and none is 0, so infinities in live rows come out
+ * as the formula says (down to weights of 2^-100). RoPE
  * angles are exact products, reduced before the sine (the contiguous calls
  * form them in fp32, 2e-3 off at position 32768). qg, k, v, ctx 16-byte
  * aligned. */

@@ -1173,3 +1173,58 @@ def test_prefill_leaves_out_bad_ids_and_positions(be, bad):
     placed = [(i, 0, 12 + i) for i in range(20)] + [(int(cu[4]) + i, 4, 7 + i) for i in range(3)]
     check_rows(P, before, qg, k, v, ctx, table, placed, group, 1, parts=1)
     assert (ctx[int(cu[2]):int(cu[4])] == 7).all(), "a chunk that was left out was written"
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_decode_infinite_values_and_keys(be, dtype):
+    """Infinities in live rows come out as the formula says: a value's in its own dim, those of both signs as NaN, a key's
+    that makes the score -infinity as a token without weight; whole units and cut ones."""
+    import torch
+    lens, page, KH, group = [40, 5000], 16, 1, 8
+    n_pages = sum(-(-n // page) for n in lens)
+    P = Pool(be, n_pages, page, KH, seed=61)
+    table = pages_for(lens, page, n_pages, seed=61)
+    qg, k, v, ctx = P.inputs(2, 8, dtype)
+    pos, td = ints([n - 1 for n in lens]), ints(table)
+    inf = float("inf")
+    qg[:, :, HD:].clamp_(-4, 4)
+
+    def call():
+        P.cache.decode_dev(0, 2, qg.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), td.data_ptr(), table.shape[1],
+                           ctx.data_ptr(), H=8, dtype=dtype)
+        be.sync()
+        return ctx.clone()
+
+    def row(which, r, t):
+        return P.kv[0, which, int(table[r, t // page]), 0, t % page]
+
+    plain = call()
+    for r, ts in ((0, (7, 30)), (1, (2000, 4990))):
+        row(1, r, ts[0])[5] = inf
+        row(1, r, ts[1])[9] = -inf
+        row(1, r, ts[0])[11] = inf
+        row(1, r, ts[1])[11] = -inf
+    v[:, :, 13] = inf
+    got = call()
+    assert (got[..., 5] == inf).all() and (got[..., 9] == -inf).all() and got[..., 11].isnan().all() and (got[..., 13] == inf).all()
+    rest = [d for d in range(HD) if d not in (5, 9, 11, 13)]
+    assert torch.equal(got[..., rest], plain[..., rest])
+
+    for r, t in ((0, 7), (1, 2000)):
+        row(1, r, t)[:] = 0
+    v[:, :, 13] = 0
+    for r, t in ((0, 30), (1, 4990)):
+        row(1, r, t)[:] = 0
+    for r, t in ((0, 7), (1, 2000)):
+        row(0, r, t)[200] = -inf               # behind the rotated dims: q keeps its sign there
+    got = call().double().cpu().numpy()
+    after, qg64 = P.host(), qg.double().cpu().numpy()
+    for r, t in ((0, 7), (1, 2000)):
+        rows = np.delete(ref.rows_of(after, table[r], page, lens[r]), t, axis=2)
+        q = ref.norm_rope(qg64[r:r + 1, :, :HD], P.qnw, np.array([lens[r] - 1]), ROT, EPS, THETA)[0]
+        u = 2.0 ** (-16 if dtype else -24) + 2.0 ** -19
+        o, tol = ref.attend(q, qg64[r, :, HD:], rows, group, u, 2.0 ** -8 if dtype else 2.0 ** -24)
+        seen = qg64[r, :, 200] < 0             # .. the score is +infinity: no softmax
+        assert 0 < seen.sum() < 8
+        assert np.isnan(got[r][seen]).all()
+        assert (np.abs(got[r] - o) <= tol)[~seen].all()
