@@ -289,23 +289,21 @@ template <typename TI> struct PdEntry {      // layout of the q entry and of the
     static constexpr int O = GQA_GRP * GROW;                  // gate entry: half of O, fp32, behind the gate rows
     static_assert((GQA_GRP + 2) * ROW <= PD_STAGE && O + GQA_GRP * PD_OROW * 4 <= PD_STAGE && GROW % 16 == 0, "");
 };
-// (x, y) as PARTS bf16 pairs whose sum is (x, y): all but the last part cut off (one byte permutation),
-// the last rounded, so two leave 2^-16 of it at most and three nothing. Parts have the sign of the
-// whole and are not 0 unless it is (2^-24 of it stands in for nothing left, down to 2^-109): an
-// infinity in the other operand stays that infinity, where rounded parts would make inf - inf or
-// 0 * inf of it. (Rounded parts of q take 0.2 us less at one request of 4k, those of the
-// probabilities nothing.)
-template <int PARTS, bool SIGNED>
+// (x, y) as PARTS bf16 pairs whose sum is (x, y): all parts but the last cut off (one byte
+// permutation), the last rounded, so two leave 2^-16 of it at most and three 2^-23. Every part has
+// the sign of the whole and is not 0 unless it is, since 2^-24 of the whole is added to what a cut
+// leaves (down to numbers of 2^-109): an infinity in the other operand stays that infinity, where
+// rounded parts would make inf - inf or 0 * inf of it. (Rounded ones: 0.2 us less of the 15 of a
+// request of 4k, nothing in the longer cases.)
+template <int PARTS>
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&out)[PARTS])
 {
-    const float dx = x * 0x1p-24f, dy = y * 0x1p-24f;
+    const float x0 = x, y0 = y;
 #pragma unroll
     for (int i = 0; i < PARTS - 1; ++i) {
         out[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-        x -= __uint_as_float(out[i] << 16);
-        y -= __uint_as_float(out[i] & 0xffff0000u);
-        x = !SIGNED ? fmaxf(x, dx) : x == 0.f ? dx : x;    // (what is left is 0 or at least 2^-24 of the whole)
-        y = !SIGNED ? fmaxf(y, dy) : y == 0.f ? dy : y;
+        x = fmaf(x0, 0x1p-24f, x - __uint_as_float(out[i] << 16));
+        y = fmaf(y0, 0x1p-24f, y - __uint_as_float(out[i] & 0xffff0000u));
     }
     out[PARTS - 1] = pack_bf16(x, y);
 }
@@ -319,7 +317,7 @@ template <> struct PdRow<__nv_bfloat16> {
     {
         uint32_t y[4][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_bf16<2, true>(x[2 * i], x[2 * i + 1], y[i]);
+        for (int i = 0; i < 4; ++i) split_bf16<2>(x[2 * i], x[2 * i + 1], y[i]);
         *reinterpret_cast<uint4 *>(at + 16 * c) = make_uint4(y[0][0], y[1][0], y[2][0], y[3][0]);
         *reinterpret_cast<uint4 *>(at + 512 + 16 * c) = make_uint4(y[0][1], y[1][1], y[2][1], y[3][1]);
     }
@@ -327,7 +325,7 @@ template <> struct PdRow<__nv_bfloat16> {
     __device__ __forceinline__ void store1(int d, float x) const
     {
         uint32_t y[2];
-        split_bf16<2, true>(x, 0.f, y);
+        split_bf16<2>(x, 0.f, y);
         reinterpret_cast<uint16_t *>(at)[d] = (uint16_t)y[0];
         reinterpret_cast<uint16_t *>(at + 512)[d] = (uint16_t)y[1];
     }
@@ -650,7 +648,7 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                         if constexpr (E::F32) {
                             const float2 x = *reinterpret_cast<const float2 *>(from);
                             uint32_t parts[PARTS];
-                            split_bf16<PARTS, true>(x.x, x.y, parts);
+                            split_bf16<PARTS>(x.x, x.y, parts);
 #pragma unroll
                             for (int q = 0; q < PARTS; ++q) qf[q][kk][e] = parts[q];
                         } else {
@@ -731,8 +729,8 @@ pages_decode_kernel(GqaPagesArgs p, PagesPart part, const __grid_constant__ CUte
                 l0 += p0 + p2;
                 l1 += p1 + p3;
                 uint32_t pa[PARTS], pb[PARTS];
-                split_bf16<PARTS, false>(p0, p1, pa);
-                split_bf16<PARTS, false>(p2, p3, pb);
+                split_bf16<PARTS>(p0, p1, pa);
+                split_bf16<PARTS>(p2, p3, pb);
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) { pa[q] = movmatrix_t(pa[q]); pb[q] = movmatrix_t(pb[q]); }
                 // O^T[256 dims x 8 heads] += V^T[256 x 16 tok] . P^T[16 tok x 8 heads]
