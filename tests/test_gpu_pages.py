@@ -1228,3 +1228,28 @@ def test_decode_infinite_values_and_keys(be, dtype):
         assert 0 < seen.sum() < 8
         assert np.isnan(got[r][seen]).all()
         assert (np.abs(got[r] - o) <= tol)[~seen].all()
+
+
+def test_repeated_calls_give_the_same_bits(be):
+    """Cut and whole units, merged and joined: a call gives the same bits each time, decode and prefill."""
+    P = Pool(be, 700, 16, 2, seed=71)
+    lens = [4000, 33, 700, 3000, 1, 129]
+    table = pages_for([n + 40 for n in lens], 16, 700, seed=71)
+    td, cu = ints(table), ints([0, 40, 57, 58, 90, 90, 99])
+    pos, base = ints([n - 1 for n in lens]), ints(lens)
+    d, p = P.inputs(6, 16, 1), P.inputs(99, 16, 1)
+    d32 = P.inputs(6, 16, 0)
+    kept = None
+    for _ in range(30):
+        for x, dtype in ((d, 1), (d32, 0)):
+            x[3].zero_()
+            P.cache.decode_dev(0, 6, *(t.data_ptr() for t in x[:3]), pos.data_ptr(), td.data_ptr(), table.shape[1], x[3].data_ptr(),
+                               dtype=dtype)
+        p[3].zero_()
+        P.cache.prefill_dev(0, 6, 99, cu.data_ptr(), base.data_ptr(), *(t.data_ptr() for t in p[:3]), td.data_ptr(),
+                            table.shape[1], p[3].data_ptr())
+        be.sync()
+        got = [t.clone() for t in (d[3], d32[3], p[3], P.kv)]
+        kept = kept or got
+        for a, b in zip(got, kept):
+            assert P.torch.equal(a, b)
