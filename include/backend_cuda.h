@@ -430,9 +430,9 @@ int  coli_cuda_gqa_decode_pages_dev(ColiCudaPages *pages, int layer, int B, cons
  * that decodes beside others that prefill); rows outside all chunks are left
  * as they were. A request has one chunk in a call, and the pages that it is
  * appended to are that request's alone. q and the probabilities enter the
- * tensor cores as bf16. A non-finite v row of the chunk itself can reach rows
- * up to 127 positions before it (0 * inf in the matrix product); stale rows of
- * pages, of whatever contents, reach none. bf16 activations (dtype 1) only. S <= 2^24,
+ * tensor cores as bf16. Infinities and NaN of a row reach only the rows that
+ * see it (a call with such v rows takes longer), and stale rows of pages, of
+ * whatever contents, reach none. bf16 activations (dtype 1) only. S <= 2^24,
  * max_pages * page <= 2^30 (decode too). */
 int  coli_cuda_gqa_prefill_pages_dev(ColiCudaPages *pages, int layer, int n_seq, int S, const int *cu,
                                      const int *pos_base, const void *qg, const void *k, const void *v,

@@ -1011,7 +1011,9 @@ cudaError_t launch_pages_decode(const CUtensorMap &tkv, const GqaPagesArgs &a, c
 //   1 KiB, for K (K-major) and V (MN-major) alike, whatever the page size.
 //   Keys behind the request's end: K scores are masked, V rows read as zeros
 //   (boxes outside the pool; the last few rows of a group cleared in shared memory),
-//   so non-finite stale rows cannot come through as 0 * inf.
+//   so non-finite stale rows cannot come through as 0 * inf. New v rows that are not finite are
+//   flagged by the append (a word in the workspace, reset by the join); only then the V loader looks
+//   through tiles that hide keys from some row, and clears what would reach it.
 // TMEM (512 columns): scores 128 | O 256 | Q 128 (bf16 pairs). Q and P are
 // rounded to bf16 (2^-9 of each element on average): a second part of either would double
 // its MMAs, and the tensor pipe is the bound here.
@@ -1028,11 +1030,12 @@ constexpr int PP_SOFTMAX = 256, PP_THREADS = 96 + PP_SOFTMAX;
 constexpr int PP_SETUP = 7;                 // a unit's start and end in tiles' time (4: 5-15 % slower, 9 and 12: 1-4 %)
 constexpr int PP_MIN = 4;                   // least work of a CTA
 struct PpBars {
-    uint64_t q_tmem, k_full[2], k_empty[2], v_full, v_empty, s_full, s_free, p_full, pv_done, g_full, epi_done;
+    uint64_t q_tmem, k_full[2], k_empty[2], v_full, v_raw, v_empty, s_full, s_free, p_full, pv_done, g_full, epi_done;
     unsigned long long turn[GQA_HD / 2];
     alignas(16) float w1[GQA_HD];           // 1 + q norm weights
     int4 range[2];
     uint32_t tmem_base;
+    int clean_from[2];                      // of the piece in work and the next: first key whose V tile was cleaned, or -1
     float lsum[PP_BM];
 };
 constexpr int PP_SMEM = 3 * PP_TILE + PP_P + (int)sizeof(PpBars);
@@ -1121,7 +1124,7 @@ __device__ __forceinline__ void pp_plan(const GqaPagesArgs &p, int cta, int ctas
 // behind the tiles of earlier rows; a chunk at position 0 waits for it, about 4 us.
 constexpr int PA_WARPS = 8;
 __global__ void __launch_bounds__(PA_WARPS * 32)
-pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
+pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f, int *odd)
 {
     __shared__ __align__(16) float cs[PA_WARPS][GQA_HD / 2], sn[PA_WARPS][GQA_HD / 2], w1s[GQA_HD];
     griddep_launch();                       // the attention starts now; what reads appended rows waits
@@ -1149,6 +1152,10 @@ pages_append_kernel(GqaPagesArgs p, const __grid_constant__ RopeFreq f)
     if (at < 0) return;
     store8(p.pv.k + at * GQA_HD + lane * 8, x);
     store8(p.pv.v + at * GQA_HD + lane * 8, v);
+    float zero = 0.f;                       // of finite values; NaN with any other
+#pragma unroll
+    for (int i = 0; i < 8; ++i) zero = fmaf(v[i], 0.f, zero);
+    if (zero != 0.f) *odd = 1;
 }
 
 // A CTA's pieces, one after the other.
@@ -1183,6 +1190,24 @@ struct PpWalk {
         while (n == 0 && ++at.x < p.n_req && at.x <= stop.x) n = pages_rows_of(p, at.x, row0, base);
     }
 };
+
+// Sums of the infinities and NaN among the values in dims d .. d + 7 that position pos sees, from key
+// `from` to the end of the piece; 0: there are none. Only for tiles that were cleaned of them.
+__device__ __forceinline__ void pp_cleared(const GqaPagesArgs &p, const PpWalk &w, int from, int pos, int d, float (&sum)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+    const int last = min(pos, min(w.base + w.n, w.t1 * PP_BN) - 1);
+#pragma unroll 1
+    for (int key = from; key <= last; ++key) {
+        const long long at = pages_row(p.pv, w.at.x, w.at.y, key);
+        if (at < 0) continue;
+        float v[8];
+        load8v(p.pv.v + at * GQA_HD + d, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += fabsf(v[e]) <= 3.4e38f ? 0.f : v[e];
+    }
+}
 
 // K-major 128B-swizzled operand whose 8-row groups are 4 KiB apart.
 __device__ __forceinline__ uint64_t pp_desc_k(uint32_t addr)
@@ -1225,7 +1250,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     if (threadIdx.x == 0) {
         mbar_init(&bars.q_tmem, PP_SOFTMAX);
         for (int i = 0; i < 2; ++i) { mbar_init(&bars.k_full[i], 1); mbar_init(&bars.k_empty[i], 1); }
-        mbar_init(&bars.v_full, 1); mbar_init(&bars.v_empty, 1);
+        mbar_init(&bars.v_full, 1); mbar_init(&bars.v_raw, 1); mbar_init(&bars.v_empty, 1);
         mbar_init(&bars.s_full, 1); mbar_init(&bars.s_free, PP_SOFTMAX);
         mbar_init(&bars.p_full, PP_SOFTMAX); mbar_init(&bars.pv_done, 1);
         mbar_init(&bars.g_full, 1); mbar_init(&bars.epi_done, PP_SOFTMAX);
@@ -1250,10 +1275,14 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const int box = p.box_rows, boxes = PP_BN / box, beyond = (int)((long long)p.pv.n_pages * KH * p.pv.page >> 3);
         bool ok = true;
         bool appended = false;              // .. the rows that the kernel before appends are visible
+        int odd = 0, raws = 0;              // *part.odd; tiles cleaned so far
         int gate_in = -1, wholes = 0, pc = 0;   // the stage of the last gate tile, until its epilogue is known to be done
         for (; ok && w.piece(tokens); w.next(p, tokens), ++pc) {
             const int end = w.base + w.n;   // the request's rows
-            if (warp == 1) ok = mbar_wait(&bars.q_tmem, pc & 1);   // Q has left the V buffer
+            if (warp == 1) {
+                ok = mbar_wait(&bars.q_tmem, pc & 1);           // Q has left the V buffer
+                if (lane == 0) bars.clean_from[pc & 1] = -1;
+            }
             for (int j = w.at.w; ok && j < w.t1; ++j, ++jj) {
                 const int s = jj & 1;
                 // a lane's box: `rows` of them from key `key`; 8-row boxes where V ends inside the tile
@@ -1261,7 +1290,12 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     griddep_wait();
                     fence_proxy_async_global();     // written by plain stores, read through the async proxy
                     appended = true;
+                    if (warp == 1) odd = *(volatile int *)part.odd;
                 }
+                // a V tile that hides keys from some row of the unit: hidden keys weigh 0, and 0 * inf would
+                // reach the rows before them, so infinities and NaN are cleared; the epilogue adds them to the
+                // rows that see them
+                const bool clean = warp == 1 && odd != 0 && (j + 1) * PP_BN - 1 > w.base + w.at.z * tokens;
                 const bool tail = warp == 1 && (j + 1) * PP_BN > end;
                 const int rows = tail ? 8 : box, key = j * PP_BN + lane * rows, n_box = tail ? PP_BN / 8 : boxes;
                 int at = beyond;
@@ -1277,12 +1311,30 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 }
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                uint64_t *bar = warp == 0 ? &bars.k_full[s] : &bars.v_full;
+                uint64_t *bar = warp == 0 ? &bars.k_full[s] : clean ? &bars.v_raw : &bars.v_full;
                 uint8_t *to = warp == 0 ? sK + s * PP_TILE : sV;
                 if (lane == 0) mbar_expect_tx(bar, PP_TILE);
                 __syncwarp();
                 if (lane < n_box) tma_load_4d(to + lane * rows * 512, warp == 0 ? &tmK : tail ? &tmV8 : &tmV, 0, 0, 0, at, bar);
                 __syncwarp();
+                if (__builtin_expect(clean, 0)) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bars.v_raw, raws++ & 1));
+                    bool found = false;
+#pragma unroll 4
+                    for (int c = lane; c < PP_TILE / 4; c += 32) {
+                        uint32_t *y = reinterpret_cast<uint32_t *>(sV) + c, was = *y, is = was;
+                        if ((is & 0x7f80u) == 0x7f80u) is &= 0xffff0000u;
+                        if ((is & 0x7f800000u) == 0x7f800000u) is &= 0xffffu;
+                        if (is != was) { *y = is; found = true; }
+                    }
+                    fence_proxy_async();
+                    found = __any_sync(0xffffffffu, found);
+                    if (lane == 0) {
+                        if (found && bars.clean_from[pc & 1] < 0) bars.clean_from[pc & 1] = j * PP_BN;
+                        if (ok) mbar_arrive(&bars.v_full);
+                    }
+                    __syncwarp();
+                }
             }
             if (warp == 0 && ok && w.ends && w.at.w == 0) {
                 // the gate tile, into the stage of the last K tile once S has read it, and once the
@@ -1359,6 +1411,7 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const float sl2 = p.scale_log2;
         const __nv_bfloat16 *qg = static_cast<const __nv_bfloat16 *>(p.qg);
         int wholes = 0;
+        int pc = 0;
         // ---- q of piece x: a warp copies its 16 rows (row = token * group + head) into the V buffer, in
         // 128B-swizzled 64-column blocks, norms and ropes them there, and they go to TMEM as bf16
         // pairs. The V buffer and Q's columns are free: the piece before has done its last product.
@@ -1524,6 +1577,8 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
             mbar_wait(&bars.pv_done, (jj - 1) & 1);
             tc::fence_after();
+            mbar_wait(&bars.v_full, (jj - 1) & 1);   // (long since; the next V tile waits for the next piece's q) ..
+            const int clean_from = bars.clean_from[pc++ & 1];   // .. orders this behind the V loader
             // the next piece's q first: its S runs during this epilogue
             PpWalk nx = w;
             nx.next(p, tokens);
@@ -1565,6 +1620,24 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                     *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.ctx) +
                                                ((size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1))) * GQA_HD + lane * 8) = x;
                 }
+                if (__builtin_expect(clean_from >= 0, 0)) {
+                    // what was cleared of v, to the rows that see it: the thread's 8 dims of the warp's rows
+                    float v[8];
+#pragma unroll 1
+                    for (int r = 16 * sw; r < 16 * sw + 16; ++r) {
+                        const int t = tok0 + (r >> gs);
+                        if (t >= w.n) break;
+                        if (r == 16 * sw || (r & (group - 1)) == 0) pp_cleared(p, w, clean_from, w.base + t, lane * 8, v);
+                        const size_t at = (size_t)(w.row0 + t) * p.H + w.at.y * group + (r & (group - 1));
+                        __nv_bfloat16 *y = static_cast<__nv_bfloat16 *>(p.ctx) + at * GQA_HD + lane * 8;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (v[e] != 0.f) {
+                                const float g = __bfloat162float(qg[at * 2 * GQA_HD + GQA_HD + lane * 8 + e]);
+                                y[e] = __float2bfloat16_rn(__bfloat162float(y[e]) + v[e] * gate_of(g));
+                            }
+                    }
+                }
                 fence_proxy_async();        // read out: the stage takes K tiles again
                 mbar_arrive(&bars.epi_done);
             } else {
@@ -1578,6 +1651,16 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         out[(32 * u + 8 * c + j) * PP_BM] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
+                if (__builtin_expect(clean_from >= 0, 0)) {
+                    float v[8];
+#pragma unroll 1
+                    for (int d = 128 * u; d < 128 * u + 128; d += 8) {
+                        pp_cleared(p, w, clean_from, w.base + tok0 + (row >> gs), d, v);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (v[e] != 0.f) reinterpret_cast<float *>(out + (d >> 2) * PP_BM)[(e >> 2) * PP_BM * 4 + (e & 3)] += v[e];
+                    }
                 }
             }
             tc::fence_before();             // O read: the next piece's products overwrite it (behind p_full)
@@ -1621,6 +1704,7 @@ pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
     __shared__ __align__(16) float turned[32][PJ_DIMS + 4];
     const int a = blockIdx.x, quarter = blockIdx.y & 3, block = blockIdx.y >> 2, tid = threadIdx.x, j = tid >> 5, lane = tid & 31;
     griddep_wait();
+    if (blockIdx.x + blockIdx.y + tid == 0) *part.odd = 0;    // for the next call
     int4 unit;
     int n;
     if (!pp_split_unit(part, a, gridDim.x, unit, n)) return;
@@ -1673,6 +1757,7 @@ pages_prefill_join_deep_kernel(GqaPagesArgs p, PagesPart part)
     __shared__ float2 mls[PJ_THREADS / 32][32];
     const int a = blockIdx.x, quarter = blockIdx.y & 3, block = blockIdx.y >> 2, tid = threadIdx.x, j = tid >> 5, lane = tid & 31;
     griddep_wait();
+    if (blockIdx.x + blockIdx.y + tid == 0) *part.odd = 0;    // for the next call
     int4 unit;
     int n;
     if (!pp_split_unit(part, a, gridDim.x, unit, n)) return;
@@ -1732,7 +1817,7 @@ cudaError_t launch_pages_prefill(const CUtensorMap &tk, const CUtensorMap &tv, c
     const long long units = (long long)a.pv.KH * ((a.S + tokens - 1) / tokens + a.n_req);
     const long long work = units * (((long long)a.pv.max_pages * a.pv.page + PP_BN - 1) / PP_BN + PP_SETUP);
     const int used = (int)std::min<long long>(ctas, (work + PP_MIN - 1) / PP_MIN);
-    pages_append_kernel<<<(int)(((long long)a.S * a.pv.KH + PA_WARPS - 1) / PA_WARPS), PA_WARPS * 32, 0, st>>>(a, f);
+    pages_append_kernel<<<(int)(((long long)a.S * a.pv.KH + PA_WARPS - 1) / PA_WARPS), PA_WARPS * 32, 0, st>>>(a, f, part.odd);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];

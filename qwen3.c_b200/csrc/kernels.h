@@ -220,6 +220,7 @@ struct PagesPart {
     float2 *ml;           // [2 ctas][rows of a unit] (max, sum), log2 domain
     float4 *park;         // [4 ctas][512] a warp's piece, in its own layout, until its range is done
     int4 *plan;           // prefill: [ctas + 1] where each CTA's range starts (request, KV head, query tile, key tile)
+    int *odd;             // prefill: not 0 if a new v row holds an infinity or NaN (0 between calls; anything else costs time only)
     int4 *units;          // decode: [ctas] unit that begins in CTA c and goes on: (last CTA or -1, request, KV head, ..)
 };
 cudaError_t launch_pages_decode(const CUtensorMap &tkv, const GqaPagesArgs &a, const PagesPart &part,

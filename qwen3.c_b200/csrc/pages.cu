@@ -40,7 +40,7 @@ size_t pages_norm_bytes(int layers) { return (size_t)layers * 2 * GQA_HD * 4; }
 size_t pages_list_bytes(int n_pages) { return ((size_t)n_pages * 4 + 255) & ~size_t(255); }
 // the workspace serves one call at a time: a compaction's lists, or an attention call's pieces
 size_t pages_part_rows() { return (size_t)2 * G.num_sms * PP_BM; }   // decode: 8 rows to a piece, prefill: 128
-size_t pages_part_bytes() { return pages_part_rows() * (GQA_HD * 4 + 8) + (size_t)G.num_sms * (4 * 512 + 2) * 16 + 16; }
+size_t pages_part_bytes() { return pages_part_rows() * (GQA_HD * 4 + 8) + (size_t)G.num_sms * (4 * 512 + 2) * 16 + 32; }
 size_t pages_ws_bytes(int n_pages)
 {
     return (std::max(3 * pages_list_bytes(n_pages) + 256, pages_part_bytes()) + 255) & ~size_t(255);
@@ -53,6 +53,7 @@ PagesPart pages_part(uint8_t *ws)
     t.park = (float4 *)(t.ml + pages_part_rows());
     t.units = (int4 *)(t.park + (size_t)G.num_sms * 4 * 512);
     t.plan = t.units + G.num_sms;
+    t.odd = (int *)(t.plan + G.num_sms + 1);
     return t;
 }
 
@@ -257,6 +258,7 @@ int coli_cuda_pages_create(ColiCudaPages **pages, int layers, int n_pages, int p
         if (ok && cudaMemsetAsync(p->base, 0, bytes, stream()) != cudaSuccess) ok = cuda_fail(cudaGetLastError(), "pages memset");
     }
     ok = ok && dev_alloc((void **)&p->norm_w, pages_norm_bytes(layers)) && dev_alloc((void **)&p->own_ws, pages_ws_bytes(n_pages));
+    if (ok && cudaMemsetAsync(pages_part(p->own_ws).odd, 0, 16, stream()) != cudaSuccess) ok = cuda_fail(cudaGetLastError(), "pages memset");
     p->ws = p->own_ws;
     p->box_rows = std::min(PP_BN, page & -page);
     for (int i = 0; ok && i < layers; ++i) {

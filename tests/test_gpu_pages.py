@@ -1253,3 +1253,42 @@ def test_repeated_calls_give_the_same_bits(be):
         kept = kept or got
         for a, b in zip(got, kept):
             assert P.torch.equal(a, b)
+
+
+# chunks whose rows share 128-key tiles with later ones: whole units, cut ones, one query head a group, a start inside a page
+@pytest.mark.parametrize("chunks,page,KH,group", [
+    ([(60, 0), (40, 100), (3, 5)], 16, 2, 8), ([(200, 70)], 64, 1, 1), ([(300, 2100), (9, 0)], 128, 2, 4), ([(24, 9000)], 64, 1, 8)])
+def test_prefill_non_finite_values_reach_no_earlier_row(be, chunks, page, KH, group):
+    """Infinite and NaN values of new rows: rows that do not see them are bit for bit what they are without them, rows that
+    do have the infinity or NaN in its dim and no other; in the call after, nothing is left of them."""
+    import torch
+    total = [n + c for n, c in chunks]
+    n_pages = sum(-(-n // page) for n in total) + 1
+    P = Pool(be, n_pages, page, KH, seed=81)
+    table = pages_for(total, page, n_pages, seed=81)
+    poison(P, table, total)
+    cu = np.concatenate([[0], np.cumsum([n for n, _ in chunks])])
+    S = int(cu[-1])
+    qg, k, v, ctx = P.inputs(S, KH * group, 1)
+    qg[:, :, HD:].clamp_(-4, 4)
+    cu_d, base, td = ints(cu), ints([c for _, c in chunks]), ints(table)
+
+    def call(v):
+        ctx.fill_(7.0)
+        P.cache.prefill_dev(0, len(chunks), S, cu_d.data_ptr(), base.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(),
+                            td.data_ptr(), table.shape[1], ctx.data_ptr(), H=KH * group)
+        be.sync()
+        return ctx.clone()
+
+    plain = call(v)
+    want, odd = plain.clone(), v.clone()
+    for r, (n, _) in enumerate(chunks):
+        mine = slice(int(cu[r]), int(cu[r + 1]))
+        for i, d, x in ((n // 3, 3, float("inf")), (n // 2, 130, float("-inf")), (2 * n // 3, 77, float("nan")), (n - 1, 255, float("inf")),
+                        (n // 3, 200, float("inf")), (n // 2, 200, float("-inf"))):
+            odd[int(cu[r]) + i, KH - 1, d] = x
+        seen = torch.where(odd[mine].isfinite(), 0.0, odd[mine].float()).cumsum(0)   # inf - inf: NaN
+        want[mine] = (plain[mine].float() + seen.repeat_interleave(group, 1)).bfloat16()
+    for _ in range(2):
+        assert torch.equal(call(odd).nan_to_num(nan=1e30), want.nan_to_num(nan=1e30))
+    assert torch.equal(call(v), plain)
