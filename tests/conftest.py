@@ -14,6 +14,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200, sm_100a)")
 
 
+def pytest_collection_modifyitems(items):
+    """Where the engine's programs are not built (that takes the reference's sources), their tests fail; they go last, so
+    that a run that stops at its first failure has run every other test."""
+    if not os.path.exists(os.path.join(PKG_DIR, "engine", "_build", "qwen_vk_cuda")):
+        items.sort(key=lambda item: os.path.basename(str(item.fspath)) == "test_gpu_engine.py")
+
+
 def load_pkg():
     """Import the qwen3.c_b200 package (its directory name is not an identifier)."""
     if "qwen3c_b200" in sys.modules:
