@@ -1577,8 +1577,10 @@ pages_prefill_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             asm volatile("bar.sync 1, %0;" ::"n"(PP_SOFTMAX) : "memory");
             mbar_wait(&bars.pv_done, (jj - 1) & 1);
             tc::fence_after();
-            mbar_wait(&bars.v_full, (jj - 1) & 1);   // (long since; the next V tile waits for the next piece's q) ..
-            const int clean_from = bars.clean_from[pc++ & 1];   // .. orders this behind the V loader
+            // completed before pv_done, and the next V tile waits for the next piece's q: never false; it orders
+            // the read behind the V loader's write
+            mbar_try_wait(&bars.v_full, (jj - 1) & 1);
+            const int clean_from = bars.clean_from[pc++ & 1];
             // the next piece's q first: its S runs during this epilogue
             PpWalk nx = w;
             nx.next(p, tokens);
@@ -1704,7 +1706,7 @@ pages_prefill_join_kernel(GqaPagesArgs p, PagesPart part)
     __shared__ __align__(16) float turned[32][PJ_DIMS + 4];
     const int a = blockIdx.x, quarter = blockIdx.y & 3, block = blockIdx.y >> 2, tid = threadIdx.x, j = tid >> 5, lane = tid & 31;
     griddep_wait();
-    if (blockIdx.x + blockIdx.y + tid == 0) *part.odd = 0;    // for the next call
+    if (blockIdx.x + blockIdx.y + tid == 0 && *part.odd != 0) *part.odd = 0;    // for the next call (a store holds up the grid's end)
     int4 unit;
     int n;
     if (!pp_split_unit(part, a, gridDim.x, unit, n)) return;
@@ -1757,7 +1759,7 @@ pages_prefill_join_deep_kernel(GqaPagesArgs p, PagesPart part)
     __shared__ float2 mls[PJ_THREADS / 32][32];
     const int a = blockIdx.x, quarter = blockIdx.y & 3, block = blockIdx.y >> 2, tid = threadIdx.x, j = tid >> 5, lane = tid & 31;
     griddep_wait();
-    if (blockIdx.x + blockIdx.y + tid == 0) *part.odd = 0;    // for the next call
+    if (blockIdx.x + blockIdx.y + tid == 0 && *part.odd != 0) *part.odd = 0;    // for the next call (a store holds up the grid's end)
     int4 unit;
     int n;
     if (!pp_split_unit(part, a, gridDim.x, unit, n)) return;
