@@ -1292,3 +1292,43 @@ def test_prefill_non_finite_values_reach_no_earlier_row(be, chunks, page, KH, gr
     for _ in range(2):
         assert torch.equal(call(odd).nan_to_num(nan=1e30), want.nan_to_num(nan=1e30))
     assert torch.equal(call(v), plain)
+
+
+@pytest.mark.parametrize("rows,dtype", [(0, 1), (0, 0), (5, 1)])
+def test_contexts_of_a_million_tokens(be, rows, dtype):
+    """A decode step (rows 0) and a chunk at position 10^6, over a table that names a few pages again and again; KV heads
+    and lengths odd."""
+    import torch
+    page, KH, group, T, n_pages = 48, 3, 4, 1000003, 40
+    P = Pool(be, n_pages, page, KH, seed=91)
+    P.kv.mul_(0.25)
+    rng = np.random.default_rng(91)
+    table = rng.integers(0, n_pages - 2, size=(1, -(-T // page)))
+    n = max(rows, 1)
+    table[0, (T - n) // page:] = [n_pages - 2, n_pages - 1][-(table.shape[1] - (T - n) // page):]    # its own
+    qg, k, v, ctx = P.inputs(n, KH * group, dtype)
+    td, at = ints(table), ints([T - n])
+    if rows:
+        cu = ints([0, n])
+        P.cache.prefill_dev(0, 1, n, cu.data_ptr(), at.data_ptr(), qg.data_ptr(), k.data_ptr(), v.data_ptr(), td.data_ptr(),
+                            table.shape[1], ctx.data_ptr(), H=KH * group)
+    else:
+        P.cache.decode_dev(0, 1, qg.data_ptr(), k.data_ptr(), v.data_ptr(), at.data_ptr(), td.data_ptr(), table.shape[1],
+                           ctx.data_ptr(), H=KH * group, dtype=dtype)
+    be.sync()
+    pos = np.arange(T - n, T)
+    q = torch.tensor(ref.norm_rope(qg[..., :HD].double().cpu().numpy(), P.qnw, pos, ROT, EPS, THETA), device="cuda")
+    where = ints(table[0, pos // page]).long(), ints(pos % page).long()
+    kn = torch.tensor(ref.norm_rope(k.double().cpu().numpy(), P.knw, pos, ROT, EPS, THETA), device="cuda")
+    assert ((P.kv[0, 0][where[0], :, where[1]].double() - kn).abs() <= (2.0 ** -8 + 2.0 ** -16) * kn.abs() + 1e-4).all()
+    u, u_out = 2.0 ** (-8 if rows else -16 if dtype else -24) + 2.0 ** -19, 2.0 ** -8 if dtype else 2.0 ** -24
+    for h in range(KH * group):
+        K, V = (P.kv[0, w][td[0].long(), h // group].reshape(-1, HD)[:T].double() for w in (0, 1))
+        s, a = q[:, h] @ K.T / 16, q[:, h].abs() @ K.abs().T / 16
+        s = s.masked_fill(torch.arange(T, device="cuda") > ints(pos)[:, None], -float("inf"))
+        p, gate = s.softmax(-1), torch.sigmoid(qg[:, h, HD:].double())
+        o = p @ V * gate
+        # as in pages_ref; a 32-bit sum takes at most 62500 x 3 / 592 tiles in a warp (8 x 7800 / 148 in a prefill's CTA) and
+        # 592 pieces in the joins, each off by 2^-24 of it: below 2^-14, beside pages_ref's own
+        tol = (torch.expm1(2 * u * a.amax(1, keepdim=True)) + u + 2.0 ** -13) * (p @ V.abs() * gate)
+        assert ((ctx[:, h].double() - o).abs() <= tol + u_out * (o.abs() + tol) + 1e-30).all(), h
