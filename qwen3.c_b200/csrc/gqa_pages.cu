@@ -254,8 +254,8 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
 // the (up to) 8 query heads of the KV head being the N of the MMA: 8 FLOP per
 // byte read, so HBM bounds it, and tcgen05's 64-row minimum would leave 7/8 of
 // its rows empty. The tensor pipe has room to spare, so q and the softmax
-// numerators are not rounded to one bf16 but enter as PARTS of them (hi + lo,
-// 16 bits, for bf16 activations; three parts, 24 bits, for fp32 ones), one MMA
+// numerators are not rounded to one bf16 but enter as PARTS of them (two, good to
+// 2^-16, for bf16 activations; three, all 24 bits, for fp32 ones), one MMA
 // for each.
 //
 // The new token's K and V rows are normed, roped and appended by the warp that
@@ -290,9 +290,9 @@ template <typename TI> struct PdEntry {      // layout of the q entry and of the
     static_assert((GQA_GRP + 2) * ROW <= PD_STAGE && O + GQA_GRP * PD_OROW * 4 <= PD_STAGE && GROW % 16 == 0, "");
 };
 // (x, y) as PARTS bf16 pairs whose sum is (x, y): all parts but the last cut off (one byte
-// permutation), the last rounded, so two leave 2^-16 of it at most and three 2^-23. Every part has
-// the sign of the whole and is not 0 unless it is, since 2^-24 of the whole is added to what a cut
-// leaves (down to numbers of 2^-109): an infinity in the other operand stays that infinity, where
+// permutation), the last rounded, so two leave 2^-16 of it at most and three 2^-31. Every part has
+// the sign of the whole and is not 0 unless it is, since 2^-32 of the whole is added to what a cut
+// leaves (down to numbers of 2^-101): an infinity in the other operand stays that infinity, where
 // rounded parts would make inf - inf or 0 * inf of it. (Rounded ones: 0.2 us less of the 15 of a
 // request of 4k, nothing in the longer cases.)
 template <int PARTS>
@@ -302,8 +302,8 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&out)[PAR
 #pragma unroll
     for (int i = 0; i < PARTS - 1; ++i) {
         out[i] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-        x = fmaf(x0, 0x1p-24f, x - __uint_as_float(out[i] << 16));
-        y = fmaf(y0, 0x1p-24f, y - __uint_as_float(out[i] & 0xffff0000u));
+        x = fmaf(x0, 0x1p-32f, x - __uint_as_float(out[i] << 16));
+        y = fmaf(y0, 0x1p-32f, y - __uint_as_float(out[i] & 0xffff0000u));
     }
     out[PARTS - 1] = pack_bf16(x, y);
 }
