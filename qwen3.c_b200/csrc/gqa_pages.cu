@@ -266,9 +266,10 @@ __device__ __forceinline__ void pages_norm_rope_rows(const Row &row, int q, cons
 // runs once per unit is kept in rolled loops over heads.
 //
 // Measured with the join (H / KH = 8, KH = 2 unless said): 64 requests at 32k tokens,
-// 4.25 GB, 651 us, 6.53 TB/s (the device's copies: 6.56); 48 ragged requests of up to 8k
-// tokens, fp32, KH = 4, 305 MB, 74 us from a graph, 47 at the copy rate; one request of 4k
-// tokens, 15 us from a graph: the join's launch, 4 us, and one pass through cold instructions.
+// 4.25 GB, 651 us from a graph, 660-670 a call, 6.35-6.53 TB/s (the device's copies: 6.56); 48
+// ragged requests of up to 8k tokens, fp32, KH = 4, 305 MB, 73 us from a graph, 47 at the copy
+// rate; one request of 4k tokens, 15 us from a graph, 17 a call: the join's launch, 4 us, and one
+// pass through cold instructions.
 constexpr int PD_WARPS = 4, PD_THREADS = 32 * PD_WARPS, PD_STAGES = 3, PD_STAGE = 2 * GQA_TILE_BYTES;
 // Entries that a unit counts more than it has when the list is cut. A warp pays for the q of
 // every piece; one that starts and ends in its range it also finishes and writes by itself. So a
@@ -1017,11 +1018,11 @@ cudaError_t launch_pages_decode(const CUtensorMap &tkv, const GqaPagesArgs &a, c
 // TMEM (512 columns): scores 128 | O 256 | Q 128 (bf16 pairs). Q and P are
 // rounded to bf16 (2^-9 of each element on average): a second part of either would double
 // its MMAs, and the tensor pipe is the bound here.
-// Measured, H / KH = 8, KH = 2: 4096 rows after 28672, 2.06 TFLOP of causal products, 1.55 ms
-// (1.33 PFLOP/s, 0.82 of the GPU's 8192^3 product; up to 1.79 ms under its power cap); nine
-// chunks of up to 1023 rows after up to 4096, 155 GFLOP, 183 us from a graph (0.84 PFLOP/s; the
+// Measured, H / KH = 8, KH = 2: 4096 rows after 28672, 2.06 TFLOP of causal products, 1.82 ms
+// under the power cap (1.13 PFLOP/s, 0.70 of the GPU's 8192^3 product), 1.55 before it sets in; nine
+// chunks of up to 1023 rows after up to 4096, 155 GFLOP, 185 us from a graph (0.84 PFLOP/s; the
 // rest are units' starts and ends, 15500 cycles each where a tile takes 2750, masked halves of
-// diagonal tiles and the join of units cut at CTAs' ends); three short prompts 19 us, latency of
+// diagonal tiles and the join of units cut at CTAs' ends); three short prompts 20 us, latency of
 // three launches. In a tile's cycles shared memory is read for about 2500 (K and V by the MMAs, P
 // written and read): next to the tensor pipe the second bound.
 constexpr int PP_BM = 128, PP_BN = 128;

@@ -177,7 +177,8 @@ namespace coli {
 struct RopeFreq {
     unsigned long long turn[128];
 };
-// x / d for 0 <= x < 2^31 by a multiplication: with 2^shift >= d > 2^(shift - 1),
+// x / d for 0 <= x < 2^31 by a multiplication (Granlund and Montgomery, Division by Invariant
+// Integers using Multiplication, 1994): with 2^shift >= d > 2^(shift - 1),
 // floor(2^32 (2^shift - d) / d) + 1 and one shift are exact.
 struct FastDiv {
     unsigned mul, shift;
